@@ -43,6 +43,16 @@ typedef enum tk_status {
 
 /* dtype numbering = titan::DType (src/core/types.h:17-21) */
 enum { TK_FP32 = 0, TK_FP16 = 1, TK_BF16 = 2, TK_FP8_E4M3 = 3 };
+/* ... and a storage type that titan::DType does not have: 8-bit integer codes with one f32 scale for each (token, kv head)
+ * row of K and of V, quantised as the row is appended.  For a row x of head_dim values
+ *   amax = min(max(max |x|, 2^-40), 2^64), scale = amax / 127, code = round_half_even(127 x / amax) in [-127, 127]
+ * and the row stands for code * scale; a NaN among the values makes the whole row read as NaN, infinities saturate.
+ * Unlike TK_FP8_E4M3, which seals whole pages and keeps the last one in 16 bits, such a pool has no open page: it may be
+ * cut (tk_kv_truncate), forked and attended to (tk_kv_step_begin_capped, tk_kv_decode_multi) at any token.  head_dim 64
+ * or 128 (v_head_dim equal), page_size 16, chunk_tokens at most 2048, no cold tier, no TK_DECODE_SIMT.  Pool of a layer:
+ * [num_pages][Hkv] tiles of 32 * head_dim + 128 bytes: K codes [16][D], V codes [16][D], f32 K scales [16], V scales
+ * [16]; a code is stored as the unsigned byte code + 128. */
+enum { TK_INT8 = 32 };
 
 /* which decode kernel tk_kv_decode launches */
 enum { TK_DECODE_AUTO = 0, TK_DECODE_SIMT = 1, TK_DECODE_MMA = 2 };
@@ -67,8 +77,9 @@ typedef struct tk_kv_config {
     int32_t num_kv_heads;
     int32_t head_dim;           /* 64 or 128; 192 with v_head_dim 128 for the MLA cache */
     int32_t page_size;          /* tokens per page: 16 */
-    int32_t dtype;              /* storage: TK_FP16 / TK_BF16 / TK_FP8_E4M3 */
-    int32_t io_dtype;           /* type of q, k, v, out and of FP8 open pages: TK_FP16 / TK_BF16; 0 = dtype */
+    int32_t dtype;              /* storage: TK_FP16 / TK_BF16 / TK_FP8_E4M3 / TK_INT8 */
+    int32_t io_dtype;           /* type of q, k, v, out and of FP8 open pages: TK_FP16 / TK_BF16; 0 = dtype (8-bit
+                                   storage: TK_BF16) */
     int32_t num_pages;          /* physical pages per layer */
     int32_t max_seqs;           /* sequence slots */
     int32_t max_pages_per_seq;  /* page-table row length */
@@ -121,7 +132,8 @@ int    tk_kv_get_config(const tk_kv* h, tk_kv_config* out);
 /* KVCache::memory_bytes (kv_cache.cpp:153-156) */
 size_t tk_kv_memory_bytes(const tk_kv* h);
 /* Device address of layer `layer`'s pool: [num_pages][Hkv][2][page_size][D] (parity dumps).
- * FP8: `codes`, plus scales f32 [num_pages][Hkv][2] and open pages [max_seqs][Hkv][2][page_size][D]. */
+ * FP8: `codes`, plus scales f32 [num_pages][Hkv][2] and open pages [max_seqs][Hkv][2][page_size][D].
+ * INT8: tiles that hold codes and scales (TK_INT8); no scales or open pages of their own. */
 int    tk_kv_layer_ptrs(const tk_kv* h, int layer, void** pool, float** scales, void** open_pages);
 
 /* ---- sequences and pages ------------------------------------------------------
@@ -202,6 +214,17 @@ int tk_kv_step_prefill_plan(const tk_kv* h, int32_t cap, int32_t* items, int32_t
  * slots_out (device int64[n_tokens], may be NULL) receives each token's slot index. */
 int tk_kv_append(tk_kv* h, int32_t layer, const void* k, const void* v, int64_t* slots_out,
                  void* stream);
+/* Rows of the cache read back: for each i < n_ranges the K and V rows of tokens start[i] .. start[i]+count[i]-1 of seq_ids[i],
+ * one range after the other, as k_out device [rows][Hkv][D] and v_out device [rows][Hkv][v_head_dim] in out_dtype: the
+ * handle's io dtype or TK_FP32.  8-bit storage gives the values its codes stand for (code * scale in FP32, rounded once),
+ * 16-bit storage the stored bits.  start = NULL: from 0; count = NULL: up to the sequence's length.  Every range must lie
+ * inside its sequence's tokens; a sequence may be named several times.  Reads what the layer's appends before it on
+ * `stream` have written, under the page table of the moment of the call (a fork or truncation since the last step counts);
+ * it needs no step, uploads nothing and may be captured into a graph, which then replays with those pages.
+ * TK_UNSUPPORTED for a token in a cold page.  (The reference hands out the slab: KVCache::k_cache / v_cache,
+ * src/inference/kv_cache.h:42-48.) */
+int tk_kv_read(tk_kv* h, int32_t layer, int32_t n_ranges, const int32_t* seq_ids, const int32_t* start, const int32_t* count,
+               void* k_out, void* v_out, int32_t out_dtype, void* stream);
 /* cuda::attention_decode (src/compute/cuda/attention.cu:315-330) for every sequence
  * of the step: q, out device [n_seqs][H][D] in io_dtype.  Paged GQA attention,
  * online softmax, split-KV partials and log-sum-exp combine. */
@@ -234,8 +257,8 @@ int tk_kv_decode_ex(tk_kv* h, int32_t layer, const void* q, int32_t q_dtype, voi
  * prompt token (src/inference/engine.cpp:182-193, src/inference/batch.cpp:169-198).  When a sequence
  * appends more than 128 / (num_heads / num_kv_heads) tokens, the sequences with many tokens go to a kernel
  * that works on tiles of 64 (token, head) rows sharing each K/V page tile; the others stay with the decode
- * kernel.  16-bit pools with the tensor-core kernels, every sequence of the step appending at least one
- * token, no cold pages; the MLA shape up to 64 / (num_heads / num_kv_heads) tokens per sequence;
+ * kernel.  16-bit pools with the tensor-core kernels or INT8 pools, every sequence of the step appending at least one
+ * token, no cold pages, no capped lengths on an INT8 pool; the MLA shape up to 64 / (num_heads / num_kv_heads) tokens per sequence;
  * TK_UNSUPPORTED otherwise. */
 int tk_kv_decode_multi(tk_kv* h, int32_t layer, const void* q, void* out, void* stream);
 /* tk_kv_decode_multi with the output type given: TK_FP32 (the reference's float* interface,

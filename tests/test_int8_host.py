@@ -1,0 +1,87 @@
+"""INT8 pools without a GPU: the rounding of the codes, the configuration, and the calls that are refused."""
+import numpy as np
+import pytest
+
+from titan_engine_b200 import KvError, PagedKVCache
+from titan_engine_b200 import _lib as L
+
+from int8_plain import quantise, stands_for
+
+
+def _cache(**kw):
+    args = dict(num_layers=1, num_heads=8, num_kv_heads=2, head_dim=64, num_pages=8, max_seqs=4, max_pages_per_seq=8, max_step_tokens=64, dtype="int8",
+                host_only=True)
+    args.update(kw)
+    return PagedKVCache(**args)
+
+
+def test_code_rounding_is_exact_for_every_pair_of_significands():
+    """The kernel's float32 steps (one product with the rounded 127/amax, the snap to 22 significant bits, one addition of a constant) against integer
+    arithmetic, for every value / amax of 11-bit significands and every exponent gap at which a code is not 0."""
+    f32 = np.float32
+    b = np.arange(1024, 2048, dtype=np.int64)[:, None]                     # amax = b
+    to_code = (f32(127.0) / b.astype(f32)).astype(f32)
+    for gap in range(0, 10):
+        a = np.arange(1024, 2048, dtype=np.int64)[None, :]                 # x = a / 2^gap <= amax
+        x = a.astype(f32) / f32(2.0 ** gap)
+        y = np.clip((x * to_code).astype(f32), f32(-127), f32(127))
+        snapped = ((y.view(np.uint32) + np.uint32(2)) & np.uint32(0xFFFFFFFC)).view(f32)
+        got = (snapped + f32(12582912.0 + 128.0)).astype(f32).view(np.uint32).astype(np.int64) & 0xFF
+        num, den = 2 * 127 * a, 2 * b * 2 ** gap                            # 127 x / amax = num / den
+        q, rem = (num + den // 2) // den, (num + den // 2) % den
+        want = np.where((rem == 0) & (q % 2 == 1), q - 1, q)                # a tie went up: take the even neighbour
+        ok = (x <= b)
+        assert (np.broadcast_to(got - 128, ok.shape)[ok] == want[ok]).all(), gap
+
+
+def test_plain_rounding_of_ties_zeros_and_extremes():
+    codes, scale = quantise(np.array([[2.0, 1.0, -1.0, 0.0], [0.0, 0.0, 0.0, 0.0], [np.inf, 1.0, -np.inf, 2.0 ** 64]]))
+    assert codes[0].tolist() == [127, 64, -64, 0]                           # 63.5 -> 64 (even)
+    assert codes[1].tolist() == [0, 0, 0, 0] and scale[1] > 0
+    assert codes[2].tolist() == [127, 0, -127, 127]
+    assert np.isfinite(stands_for(np.array([[np.inf, 1.0]]))).all()
+
+
+@pytest.mark.parametrize("bad", [
+    dict(page_size=32), dict(decode_impl="simt"), dict(chunk_tokens=4096), dict(hot_window=64, cold_pages=4),
+    dict(head_dim=192, v_head_dim=128), dict(head_dim=96), dict(num_heads=6, num_kv_heads=2),
+])
+def test_refused_configurations(bad):
+    with pytest.raises(KvError) as e:
+        _cache(**bad)
+    assert e.value.status == L.TK_INVALID_ARG
+
+
+def test_arena_holds_codes_and_scales():
+    c = _cache(num_layers=3, num_pages=5, head_dim=128)
+    assert c.memory_bytes == 3 * ((5 * 2 * (2 * 16 * 128 + 2 * 16 * 4) + 1023) // 1024 * 1024)
+    assert c.cfg.io_dtype == L.TK_BF16 and _cache(io_dtype="fp16").cfg.io_dtype == L.TK_FP16
+
+
+def test_any_length_may_be_cut_adopted_and_capped():
+    c = _cache()
+    s = c.seq_alloc()
+    c.step_begin([s], [37])
+    c.truncate(s, 21)                                       # inside a full page
+    assert c.seq_len(s) == 21
+    t = c.seq_alloc()
+    c.adopt(t, [6, 7], 19)
+    assert c.seq_len(t) == 19
+    a, b = np.array([s, t], np.int32), np.array([1, 1], np.int32)
+    cap = np.array([5, 0], np.int32)
+    import ctypes as C
+    p = lambda x: x.ctypes.data_as(C.POINTER(C.c_int32))  # noqa: E731
+    assert c._lib.tk_kv_step_begin_capped(c._h, 2, p(a), p(b), p(cap), None) == L.TK_OK
+
+
+def test_compute_calls_need_a_device():
+    c = _cache()
+    s = c.seq_alloc()
+    c.step_begin([s], [3])
+    with pytest.raises(KvError) as e:
+        c.read(0, [s])
+    assert e.value.status == L.TK_CUDA_ERROR
+    assert c._lib.tk_kv_read(c._h, 0, 0, None, None, None, None, None, L.TK_BF16, None) == L.TK_CUDA_ERROR
+    assert c._lib.tk_kv_read(c._h, 1, 0, None, None, None, None, None, L.TK_BF16, None) == L.TK_INVALID_ARG
+    assert c._lib.tk_kv_read(None, 0, 0, None, None, None, None, None, L.TK_BF16, None) == L.TK_INVALID_ARG
+    assert c._lib.tk_kv_decode_multi(c._h, 0, None, None, None) == L.TK_CUDA_ERROR

@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libtitan_kv.so")
 
 TK_OK, TK_INVALID_ARG, TK_OUT_OF_PAGES, TK_CUDA_ERROR, TK_TIMEOUT, TK_OUT_OF_SEQS, TK_UNSUPPORTED = range(7)
-TK_FP32, TK_FP16, TK_BF16, TK_FP8_E4M3 = 0, 1, 2, 3
+TK_FP32, TK_FP16, TK_BF16, TK_FP8_E4M3, TK_INT8 = 0, 1, 2, 3, 32
 TK_DECODE_AUTO, TK_DECODE_SIMT, TK_DECODE_MMA = 0, 1, 2
 TK_MERGE_IN_KERNEL, TK_MERGE_SEPARATE = 0, 1
 TK_OVERLAP_AUTO, TK_OVERLAP_OFF = 0, 1
@@ -83,6 +83,7 @@ SIGNATURES = {
     "tk_kv_step_chunk_tokens": (C.c_int, [_P]),
     "tk_kv_step_prefill_plan": (C.c_int, [_P, C.c_int32, _I32P, _I32P, _I32P, _I32P]),
     "tk_kv_append": (C.c_int, [_P, C.c_int32, _P, _P, _P, _P]),
+    "tk_kv_read": (C.c_int, [_P, C.c_int32, C.c_int32, _I32P, _I32P, _I32P, _P, _P, C.c_int32, _P]),
     "tk_kv_decode": (C.c_int, [_P, C.c_int32, _P, _P, _P]),
     "tk_kv_append_decode": (C.c_int, [_P, C.c_int32, _P, _P, _P, _P, _P]),
     "tk_kv_rope_append_decode": (C.c_int, [_P, C.c_int32, _P, _P, _P, _P, C.c_float, C.c_float, _P]),

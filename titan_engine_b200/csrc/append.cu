@@ -256,6 +256,10 @@ cudaError_t launch_append(const Geometry& g, const LayerPtrs& lp, const StepDev&
                           int64_t* slots_out, cudaStream_t s, int* n_launches) {
     *n_launches = 0;
     if (st.n_tokens <= 0) return cudaSuccess;
+    if (g.dtype == DT_INT8) {
+        *n_launches = 1;
+        return launch_append_int8(g, lp, st, page_table, k, v, slots_out, s);
+    }
     if (g.dtype == DT_FP8 && st.n_seals > 0) {
         cudaError_t e = g.io_dtype == DT_BF16
             ? launch_seal<true>(g, lp, st, (const uint16_t*)k, (const uint16_t*)v, s)

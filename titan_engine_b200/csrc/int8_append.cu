@@ -1,0 +1,67 @@
+// int8_append.cu — a step's K/V rows quantised into an INT8 pool as they are appended: one scale per (token, kv head) row
+// of K and of V, no open page, so that a sequence may be cut or continued at any token.
+//
+// The FP8 pool seals whole pages when they are complete (append.cu); the reference has neither (its KVCache::update copies
+// FP32 rows, src/inference/kv_cache.cpp:121-151; its one absmax quantiser is FP4, src/compute/cuda/fp4.cu:102-113).
+// HBM-bound byte movement for a prompt (2 D bytes read and D + 4 written per row), launch latency for a decode step.
+#include "int8_cache.cuh"
+
+namespace tk {
+
+namespace {
+
+constexpr int kI8AppendThreads = 256;
+
+// D / 8 lanes hold a row (8 values each); a row's K and V are separate rows here: unit u = (token, K|V, kv head).
+template <bool BF16, int D>
+__global__ void __launch_bounds__(kI8AppendThreads)
+append_int8_kernel(Geometry g, uint8_t* __restrict__ pool, StepDev st, const int32_t* __restrict__ page_table,
+                   const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int64_t* __restrict__ slots_out) {
+    constexpr int LANES = D / 8, ROWS = kI8AppendThreads / LANES;
+    const int c = threadIdx.x % LANES;
+    const long long u = (long long)blockIdx.x * ROWS + threadIdx.x / LANES;
+    const int per_tok = 2 * g.Hkv;
+    const bool live = u < (long long)st.n_tokens * per_tok;
+    const int t = live ? (int)(u / per_tok) : 0, rem = live ? (int)(u % per_tok) : 0;
+    const int kv = rem >= g.Hkv, h = kv ? rem - g.Hkv : rem;
+    const uint4 x = live ? *reinterpret_cast<const uint4*>((kv ? v : k) + ((size_t)t * g.Hkv + h) * D + c * 8) : make_uint4(0, 0, 0, 0);
+    uint32_t m = i8_absmax8(x);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    if (!live) return;
+    const I8Row row = i8_row(i8_amax_value<BF16>(m));
+    const int slot = st.tok_dst[t];
+    uint8_t* tile = pool + ((size_t)(slot / kI8Page) * g.Hkv + h) * i8_tile_bytes(D);
+    const int r = slot % kI8Page;
+    *reinterpret_cast<uint2*>(tile + i8_row_off(D, kv, r) + c * 8) = i8_codes8<BF16>(x, row.to_code);
+    if (c == 0) {
+        *reinterpret_cast<float*>(tile + i8_scale_off(D, kv, r)) = row.scale;
+        if (slots_out && rem == 0) {
+            const int pos = st.tok_pos[t];
+            slots_out[t] = (int64_t)page_table[(size_t)st.seq[st.tok_b[t]] * g.max_pages_per_seq + pos / kI8Page] * kI8Page + pos % kI8Page;
+        }
+    }
+}
+
+template <bool BF16, int D>
+cudaError_t launch_d(const Geometry& g, const LayerPtrs& lp, const StepDev& st, const int32_t* page_table, const void* k,
+                     const void* v, int64_t* slots_out, cudaStream_t s) {
+    constexpr int ROWS = kI8AppendThreads / (D / 8);
+    const long long units = (long long)st.n_tokens * 2 * g.Hkv;
+    append_int8_kernel<BF16, D><<<(unsigned)((units + ROWS - 1) / ROWS), kI8AppendThreads, 0, s>>>(
+        g, (uint8_t*)lp.pool, st, page_table, (const uint16_t*)k, (const uint16_t*)v, slots_out);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_append_int8(const Geometry& g, const LayerPtrs& lp, const StepDev& st, const int32_t* page_table,
+                               const void* k, const void* v, int64_t* slots_out, cudaStream_t s) {
+    if (st.n_tokens <= 0) return cudaSuccess;
+    if (g.io_dtype == DT_BF16) return g.D == 128 ? launch_d<true, 128>(g, lp, st, page_table, k, v, slots_out, s)
+                                                 : launch_d<true, 64>(g, lp, st, page_table, k, v, slots_out, s);
+    return g.D == 128 ? launch_d<false, 128>(g, lp, st, page_table, k, v, slots_out, s)
+                      : launch_d<false, 64>(g, lp, st, page_table, k, v, slots_out, s);
+}
+
+}  // namespace tk

@@ -1,0 +1,79 @@
+// int8_cache.cuh — the tile of an INT8 pool and the rounding its rows are defined by.
+//
+// Tile (page, kv head), contiguous: 16 K rows of D codes, 16 V rows of D codes, 16 K scales, 16 V scales (f32): codes and
+// scales of a page travel in ONE copy (4224 bytes at D = 128, 2176 at D = 64), and whatever moves pages (a fork's
+// copy) moves the scales with them.  A code is stored as code + 128: an unsigned byte u is the 16-bit float 1024 + u
+// when it is put under the byte 0x64, so that expanding two codes costs one byte permute and one subtraction.
+#pragma once
+
+#include "tk_kernels.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace tk {
+
+constexpr int kI8Page = 16;                             // tokens per page of an INT8 pool
+constexpr float kI8AmaxMin = 9.094947017729282e-13f;    // 2^-40: the scale of an all-zero row stays positive
+constexpr float kI8AmaxMax = 18446744073709551616.0f;   // 2^64: larger values saturate, scales of one pool span < 2^105
+
+__host__ __device__ constexpr int i8_tile_bytes(int D) { return 2 * kI8Page * D + 2 * kI8Page * (int)sizeof(float); }
+// byte offset of a row of codes / of its scale inside a tile
+__host__ __device__ constexpr int i8_row_off(int D, int kv, int r) { return (kv * kI8Page + r) * D; }
+__host__ __device__ constexpr int i8_scale_off(int D, int kv, int r) { return 2 * kI8Page * D + (kv * kI8Page + r) * (int)sizeof(float); }
+
+// What a row's largest magnitude makes of it: `to_code` = 127 / amax and the scale amax / 127, both single IEEE divisions.
+// A NaN among the values makes the scale NaN, so that the row reads as NaN; infinities saturate like any large value.
+struct I8Row { float to_code, scale; };
+__device__ __forceinline__ I8Row i8_row(float amax) {
+    const float a = fminf(fmaxf(amax, kI8AmaxMin), kI8AmaxMax);           // (a NaN becomes the minimum here)
+    return I8Row{__fdiv_rn(127.0f, a), amax != amax ? amax : __fdiv_rn(a, 127.0f)};
+}
+
+// code + 128 in the low byte: the integer nearest to 127 x / amax, ties to even, EXACTLY.
+// x and amax have at most 11 significant bits, A and B: the quotient Q = 127 x / amax is 127 A 2^-n / B for some n, so it is a
+// half-integer or at least 1 / (2 B 2^n) = Q / (254 A) > Q 2^-19 away from every one.  y = x * fl(127 / amax) has two
+// roundings of 2^-24 relative: less than two units in the last place (ulp) from Q.  Snapped to a multiple of 4 ulps (22
+// significant bits, half-integers among them) y is the half-integer itself where Q is one, and otherwise within 4 ulps
+// of a Q that is at least 16 ulps from it: on the right side.  The addition of a constant whose neighbours are 1 apart then
+// rounds to the nearest integer, ties to even.  Checked against exact arithmetic for every pair of significands.
+__device__ __forceinline__ uint32_t i8_code(float x, float to_code) {
+    const float y = fminf(fmaxf(x * to_code, -127.0f), 127.0f);
+    const float snapped = __uint_as_float((__float_as_uint(y) + 2u) & ~3u);
+    return __float_as_uint(__fadd_rn(snapped, 12582912.0f + 128.0f)) & 0xFFu;
+}
+
+// two 16-bit values held in one word -> floats
+template <bool BF16>
+__device__ __forceinline__ float2 i8_unpack2(uint32_t w) {
+    if (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    const __half2 h = *reinterpret_cast<const __half2*>(&w);
+    return __half22float2(h);
+}
+
+// Eight 16-bit values (16 bytes) -> eight codes (8 bytes).
+template <bool BF16>
+__device__ __forceinline__ uint2 i8_codes8(const uint4& x, float to_code) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint32_t c[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = i8_unpack2<BF16>(w[i]);
+        c[2 * i] = i8_code(f.x, to_code);
+        c[2 * i + 1] = i8_code(f.y, to_code);
+    }
+    return make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+}
+
+// Largest magnitude of eight 16-bit values, as the 16-bit pattern without its sign: patterns order like the magnitudes, and
+// a NaN's is above every number's.
+__device__ __forceinline__ uint32_t i8_absmax8(const uint4& x) {
+    uint32_t m = __vmaxu2(__vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu), __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu));
+    return max(m & 0xFFFFu, m >> 16);
+}
+template <bool BF16>
+__device__ __forceinline__ float i8_amax_value(uint32_t pattern) {
+    return BF16 ? __uint_as_float(pattern << 16) : __half2float(__ushort_as_half((unsigned short)pattern));
+}
+
+}  // namespace tk

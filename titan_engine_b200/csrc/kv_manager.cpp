@@ -375,6 +375,7 @@ int PageManager::plan_step(int n_seqs, const int32_t* seqs, const int32_t* n_new
     plan->q_base.assign(n_seqs, 0);
     plan->nq.assign(n_seqs, 0);
     plan->nq_max = 0;
+    plan->capped = len_cap != nullptr;
     plan->nq_min = n_seqs > 0 ? INT32_MAX : 0;
     plan->one_token_steps = true;
     plan->has_empty_seq = false;

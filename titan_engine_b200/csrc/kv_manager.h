@@ -53,6 +53,7 @@ struct StepPlan {
     int32_t nq_max = 0, nq_min = 0;  // over the step's sequences
     bool one_token_steps = false;    // every sequence appends at most one token (a decode step)
     bool has_empty_seq = false;      // some sequence attends to zero tokens
+    bool capped = false;             // the step was begun with caps on the attended lengths
     std::vector<WorkItem> items;
     std::vector<SealItem> seals;
     std::vector<Eviction> evictions; // pages that went cold in this step (copy out before reuse)

@@ -2,6 +2,7 @@
 // metadata upload and kernel launches.  Host bookkeeping lives in kv_manager.cpp.
 #include "../../include/titan_kv.h"
 
+#include "int8_cache.cuh"
 #include "kv_manager.h"
 #include "tk_kernels.cuh"
 #include "tk_peer.cuh"
@@ -42,6 +43,7 @@ ArenaLayout arena_layout(const tk_kv_config& c) {
     const size_t esize = c.dtype == TK_FP8_E4M3 ? 1 : 2;
     const size_t tile = (size_t)c.num_kv_heads * c.page_size * (c.head_dim + c.v_head_dim);   // K rows + V rows
     a.pool_layer = align_up((size_t)c.num_pages * tile * esize, 1024);
+    if (c.dtype == TK_INT8) a.pool_layer = align_up((size_t)c.num_pages * c.num_kv_heads * tk::i8_tile_bytes(c.head_dim), 1024);
     if (c.dtype == TK_FP8_E4M3) {
         a.scales_layer = align_up((size_t)c.num_pages * c.num_kv_heads * 2 * sizeof(float), 1024);
         a.open_layer = align_up((size_t)c.max_seqs * tile * 2, 1024);
@@ -61,11 +63,17 @@ const char* validate(const tk_kv_config& c) {
     const bool mla = c.head_dim == 192 && c.v_head_dim == 128;      // K = nope + rope dims, V = nope dims
     if (!mla && ((c.head_dim != 64 && c.head_dim != 128) || c.v_head_dim != c.head_dim))
         return "head_dim must be 64 or 128 (v_head_dim equal), or 192 with v_head_dim 128 (MLA)";
-    if (mla && c.dtype == TK_FP8_E4M3) return "the MLA shape needs 16-bit storage";
+    if (mla && (c.dtype == TK_FP8_E4M3 || c.dtype == TK_INT8)) return "the MLA shape needs 16-bit storage";
     if (c.page_size <= 0 || c.page_size % 8 != 0) return "page_size must be a positive multiple of 8";
-    if (c.dtype != TK_FP16 && c.dtype != TK_BF16 && c.dtype != TK_FP8_E4M3) return "dtype must be FP16, BF16 or FP8_E4M3";
+    if (c.dtype != TK_FP16 && c.dtype != TK_BF16 && c.dtype != TK_FP8_E4M3 && c.dtype != TK_INT8)
+        return "dtype must be FP16, BF16, FP8_E4M3 or INT8";
     if (c.io_dtype != TK_FP16 && c.io_dtype != TK_BF16) return "io_dtype must be FP16 or BF16";
-    if (c.dtype != TK_FP8_E4M3 && c.io_dtype != c.dtype) return "io_dtype must equal dtype for 16-bit storage";
+    if (c.dtype == TK_INT8) {
+        if (c.page_size != tk::kI8Page) return "INT8 storage needs page_size 16";
+        if (c.decode_impl == TK_DECODE_SIMT) return "INT8 storage has no SIMT decode kernel";
+        if (c.chunk_tokens > 2048) return "INT8 storage: chunk_tokens must not exceed 2048";
+    }
+    if (c.dtype != TK_FP8_E4M3 && c.dtype != TK_INT8 && c.io_dtype != c.dtype) return "io_dtype must equal dtype for 16-bit storage";
     if (c.num_pages <= 0 || c.max_seqs <= 0 || c.max_pages_per_seq <= 0) return "num_pages/max_seqs/max_pages_per_seq must be positive";
     if ((int64_t)c.max_seqs * c.max_pages_per_seq > (int64_t)1 << 30) return "page table too large";
     if ((int64_t)c.num_pages * c.page_size >= (int64_t)1 << 31 || (int64_t)c.max_seqs * c.page_size >= (int64_t)1 << 31)
@@ -80,7 +88,7 @@ const char* validate(const tk_kv_config& c) {
     if (c.hot_window > 0) {
         if (c.hot_window < c.page_size) return "hot_window must cover at least one page";
         if (c.cold_pages == 0) return "hot_window needs cold_pages > 0";
-        if (c.dtype == TK_FP8_E4M3) return "the cold tier needs 16-bit storage";
+        if (c.dtype == TK_FP8_E4M3 || c.dtype == TK_INT8) return "the cold tier needs 16-bit storage";
     }
     return nullptr;
 }
@@ -267,7 +275,7 @@ int create_impl(const tk_kv_config* cfg_in, void* arena, size_t arena_bytes, boo
     if (!cfg_in || !out) return fail(nullptr, TK_INVALID_ARG, "null argument");
     *out = nullptr;
     tk_kv_config c = *cfg_in;
-    if (c.io_dtype == 0) c.io_dtype = c.dtype == TK_FP8_E4M3 ? TK_BF16 : c.dtype;
+    if (c.io_dtype == 0) c.io_dtype = c.dtype == TK_FP8_E4M3 || c.dtype == TK_INT8 ? TK_BF16 : c.dtype;
     if (c.max_step_tokens == 0) c.max_step_tokens = c.max_seqs;
     if (c.v_head_dim == 0) c.v_head_dim = c.head_dim;
     if (const char* why = validate(c)) return fail(nullptr, TK_INVALID_ARG, "config: %s", why);
@@ -282,6 +290,7 @@ int create_impl(const tk_kv_config* cfg_in, void* arena, size_t arena_bytes, boo
     h->lay = arena_layout(c);
     h->host_only = c.device == TK_DEVICE_NONE;
     h->page_bytes = (size_t)c.num_kv_heads * c.page_size * (c.head_dim + c.v_head_dim) * (c.dtype == TK_FP8_E4M3 ? 1 : 2);
+    if (c.dtype == TK_INT8) h->page_bytes = (size_t)c.num_kv_heads * tk::i8_tile_bytes(c.head_dim);
     if (c.hot_window > 0) h->mgr->enable_cold(c.hot_window, c.cold_pages);
     h->stats.pages_total = c.num_pages;
 
@@ -384,7 +393,7 @@ int create_impl(const tk_kv_config* cfg_in, void* arena, size_t arena_bytes, boo
     // MLA shape: tensor-core kernel of its own; cold pages stay on the generic kernel
     h->mla_mma = tk::decode_mma_mla_supported(h->geo) && c.hot_window == 0;
     const bool mma_ok = tk::decode_mma_supported(h->geo) || h->mla_mma;
-    if (c.decode_impl == TK_DECODE_MMA && !mma_ok) {
+    if (c.decode_impl == TK_DECODE_MMA && !mma_ok && c.dtype != TK_INT8) {
         release(h);
         return fail(nullptr, TK_UNSUPPORTED, "decode_impl=MMA needs page_size 16 and head_dim 64/128 (128 for FP8), or the "
                                              "192/128 shape with 16-bit storage, groups of <= 8 heads and no cold tier");
@@ -535,7 +544,7 @@ void tk_kv_config_default(tk_kv_config* c) {
 size_t tk_kv_arena_bytes(const tk_kv_config* cfg) {
     if (!cfg) return 0;
     tk_kv_config c = *cfg;
-    if (c.io_dtype == 0) c.io_dtype = c.dtype == TK_FP8_E4M3 ? TK_BF16 : c.dtype;
+    if (c.io_dtype == 0) c.io_dtype = c.dtype == TK_FP8_E4M3 || c.dtype == TK_INT8 ? TK_BF16 : c.dtype;
     if (c.max_step_tokens == 0) c.max_step_tokens = c.max_seqs;
     if (c.v_head_dim == 0) c.v_head_dim = c.head_dim;
     if (validate(c)) return 0;
@@ -868,6 +877,45 @@ int tk_kv_append(tk_kv* h, int32_t layer, const void* k, const void* v, int64_t*
     return TK_OK;
 }
 
+// Rows of token ranges, dequantised, in the order of the ranges.
+int tk_kv_read(tk_kv* h, int32_t layer, int32_t n_ranges, const int32_t* seq_ids, const int32_t* start, const int32_t* count,
+               void* k_out, void* v_out, int32_t out_dtype, void* stream) {
+    if (!h || layer < 0 || layer >= h->cfg.num_layers || n_ranges < 0 || (n_ranges > 0 && !seq_ids)) return TK_INVALID_ARG;
+    if (const int fs = host_flush(h)) return fs;               // launches the host-buffer calls still hold back come first
+    if (h->host_only) return fail(h, TK_CUDA_ERROR, "read: handle has no device (bookkeeping only)");
+    if (out_dtype != TK_FP32 && out_dtype != h->cfg.io_dtype)
+        return fail(h, TK_INVALID_ARG, "read: out dtype must be FP32 or the handle's io dtype");
+    std::lock_guard<std::mutex> lock(h->mgr_mu);
+    const int ps = h->cfg.page_size;
+    const bool fp8 = h->cfg.dtype == TK_FP8_E4M3;
+    std::vector<tk::ReadItem> items;
+    int64_t rows = 0;
+    for (int i = 0; i < n_ranges; i++) {
+        const int seq = seq_ids[i], len = h->mgr->seq_len(seq);
+        const int64_t lo = start ? start[i] : 0, n = count ? count[i] : len - lo;
+        if (len < 0 || lo < 0 || n < 0 || lo + n > len)
+            return fail(h, TK_INVALID_ARG, "read: range %d is not inside a live sequence's tokens (sequence %d)", i, seq);
+        if (rows + n >= (int64_t)1 << 31) return fail(h, TK_INVALID_ARG, "read: more than 2^31 rows in one call");
+        const int32_t* pages = h->mgr->row(seq);
+        const int64_t sealed = fp8 ? len / ps * ps : len;      // FP8: later tokens are in the 16-bit open page
+        for (int64_t at = lo; at < lo + n;) {
+            const int r = (int)(at % ps), m = (int)std::min<int64_t>(ps - r, lo + n - at);
+            const int32_t page = at < sealed ? pages[at / ps] : -1 - seq;
+            if (at < sealed && page < 0) return fail(h, TK_UNSUPPORTED, "read: token %lld of sequence %d lies in a cold page", (long long)at, seq);
+            items.push_back(tk::ReadItem{page, r, m, (int)rows});
+            rows += m;
+            at += m;
+        }
+    }
+    if (rows == 0) return TK_OK;
+    if (!k_out || !v_out) return fail(h, TK_INVALID_ARG, "read: null output");
+    int n = 0;
+    const cudaError_t e = tk::launch_read_rows(h->geo, h->layer(layer), items.data(), (int)items.size(), k_out, v_out, out_dtype,
+                                               (cudaStream_t)stream, &n);
+    h->launches += n;
+    return e == cudaSuccess ? TK_OK : fail(h, TK_CUDA_ERROR, "read launch: %s", cudaGetErrorString(e));
+}
+
 static int decode_impl(tk_kv* h, int layer, const void* q, void* out, float* partial_out, cudaStream_t s,
                        int q_dtype = -1, int out_dtype = -1, const void* fuse_k = nullptr,
                        const void* fuse_v = nullptr, const float* rope = nullptr,
@@ -900,6 +948,15 @@ static int decode_impl(tk_kv* h, int layer, const void* q, void* out, float* par
     if (out_dtype < 0) out_dtype = h->cfg.io_dtype;
     if (out_dtype != TK_FP32 && out_dtype != h->cfg.io_dtype)
         return fail(h, TK_INVALID_ARG, "decode: out dtype must be FP32 or the handle's io dtype");
+    if (h->cfg.dtype == TK_INT8) {
+        if (peer_ctx || fuse_k || rope) return fail(h, TK_UNSUPPORTED, "decode: not fused on an INT8 pool");
+        const bool bracket = h->profiling && h->prof_used + 2 <= h->prof_ev.size();
+        if (bracket) cudaEventRecord(h->prof_ev[h->prof_used], s);
+        e = tk::launch_attn_int8(h->geo, lp, h->dev, h->d_table, q, out, out_dtype, partial_out, h->d_status, false, s);
+        h->launches++;
+        if (bracket) { cudaEventRecord(h->prof_ev[h->prof_used + 1], s); h->prof_used += 2; }
+        return e == cudaSuccess ? TK_OK : fail(h, TK_CUDA_ERROR, "decode launch: %s", cudaGetErrorString(e));
+    }
     const bool mma = h->use_mma && h->dev.chunk_tokens <= 2048;
     // the last CTA of each (sequence, kv head) merges the split-KV rows itself; a sequence that
     // attends to nothing has no CTA, so such steps keep the separate combine kernel
@@ -1036,6 +1093,13 @@ static int decode_multi_impl(tk_kv* h, int32_t layer, const void* q, void* out, 
     if (!q || !out) return fail(h, TK_INVALID_ARG, "decode_multi: null q/out");
     const tk::StepPlan& p = h->plan;
     if (p.nq_min < 1) return fail(h, TK_INVALID_ARG, "decode_multi: every sequence of the step must append at least one token");
+    if (h->cfg.dtype == TK_INT8) {
+        if (p.capped) return fail(h, TK_UNSUPPORTED, "decode_multi: not available on a step with capped lengths (INT8 storage)");
+        const cudaError_t e = tk::launch_attn_int8(h->geo, h->layer(layer), h->dev, h->d_table, q, out, out_dtype, nullptr, h->d_status,
+                                                   true, (cudaStream_t)stream);
+        h->launches++;
+        return e == cudaSuccess ? TK_OK : fail(h, TK_CUDA_ERROR, "decode_multi launch: %s", cudaGetErrorString(e));
+    }
     if (p.pf_built && h->use_mma && !h->mla_mma && tk::prefill_mma_supported(h->geo)) {
         // a prefill-sized step: the sequences with one tile of rows keep the decode kernel, the prefill
         // kernel takes the others; the two write disjoint rows of `out`
@@ -1124,7 +1188,7 @@ int tk_kv_decode_exchange(tk_kv* h, int32_t layer, const void* q, tk_peer* peer,
     if (h->dev.n_seqs == 0) return TK_OK;
     // a merging CTA waits for its peers while it holds a CTA slot: keep those few against the slots of a
     // launch, or ranks could fill their GPUs with CTAs that wait for CTAs the other ranks cannot start
-    const bool in_kernel = !h->plan.has_empty_seq && !h->separate_combine && h->dev.n_items > 0 &&
+    const bool in_kernel = h->cfg.dtype != TK_INT8 && !h->plan.has_empty_seq && !h->separate_combine && h->dev.n_items > 0 &&
                            h->dev.n_seqs * h->geo.Hkv <= h->num_sms / 2;
     if (in_kernel) {
         int st = decode_impl(h, layer, q, out, nullptr, (cudaStream_t)stream, -1, -1, nullptr, nullptr, nullptr, ctx);

@@ -11,7 +11,8 @@
 namespace tk {
 
 // Storage numbering = titan::DType (reference: src/core/types.h:17-21).
-enum : int { DT_FP32 = 0, DT_FP16 = 1, DT_BF16 = 2, DT_FP8 = 3 };
+// DT_INT8 has no counterpart there: codes with a scale per row (int8_cache.cuh).
+enum : int { DT_FP32 = 0, DT_FP16 = 1, DT_BF16 = 2, DT_FP8 = 3, DT_INT8 = 32 };
 
 struct Geometry {
     int H, Hkv, D, ps;          // query heads, kv heads, head dim, tokens per page
@@ -183,6 +184,22 @@ bool        decode_mma_mla_multi_supported(const Geometry& g, int nq_max);
 cudaError_t launch_decode_mma_mla_multi(const Geometry& g, const LayerPtrs& lp, const CUtensorMap* k_map,
                                         const CUtensorMap* v_map, const StepDev& st, const int32_t* page_table,
                                         const void* q, float* partials, int* status, cudaStream_t s, const MergeOut& mo);
+
+// INT8 pools (int8_cache.cuh): the step's rows quantised into their pages; attention of one token per sequence, or of every
+// token the step appended.
+cudaError_t launch_append_int8(const Geometry& g, const LayerPtrs& lp, const StepDev& st, const int32_t* page_table,
+                               const void* k, const void* v, int64_t* slots_out, cudaStream_t s);
+cudaError_t launch_attn_int8(const Geometry& g, const LayerPtrs& lp, const StepDev& st, const int32_t* page_table, const void* q,
+                             void* out, int out_dtype, float* partial_out, const int* status, bool every_token, cudaStream_t s);
+
+// Rows of the cache read back (read_back.cu): n_rows rows from row0 of a page, to token rows out_row, ... of the outputs.
+struct ReadItem {
+    int page;                   // physical page; -1 - s: the FP8 open page of sequence slot s
+    int row0, n_rows, out_row;
+};
+constexpr int kReadItemsSmall = 128, kReadItemsBig = 2000;   // pages per launch (the list is a kernel argument)
+cudaError_t launch_read_rows(const Geometry& g, const LayerPtrs& lp, const ReadItem* items, int n_items, void* k_out, void* v_out,
+                             int out_dtype, cudaStream_t s, int* n_launches);
 
 // n FP32 values -> the 16-bit type `dtype` (round to nearest even).
 cudaError_t launch_f32_to_16(const float* src, void* dst, size_t n, int dtype, cudaStream_t s);

@@ -17,7 +17,8 @@ import torch
 
 from . import _lib as L
 
-_DTYPES = {"fp16": L.TK_FP16, "bf16": L.TK_BF16, "fp8_e4m3": L.TK_FP8_E4M3, "fp8": L.TK_FP8_E4M3}
+_DTYPES = {"fp16": L.TK_FP16, "bf16": L.TK_BF16, "fp8_e4m3": L.TK_FP8_E4M3, "fp8": L.TK_FP8_E4M3,
+           "int8": L.TK_INT8}
 _TORCH16 = {L.TK_FP16: torch.float16, L.TK_BF16: torch.bfloat16}
 _IMPLS = {"auto": L.TK_DECODE_AUTO, "simt": L.TK_DECODE_SIMT, "mma": L.TK_DECODE_MMA}
 
@@ -53,7 +54,7 @@ class PagedKVCache:
         self._lib.tk_kv_config_default(C.byref(cfg))
         cfg.num_layers, cfg.num_heads, cfg.num_kv_heads, cfg.head_dim = num_layers, num_heads, num_kv_heads, head_dim
         cfg.page_size, cfg.dtype = page_size, _DTYPES[dtype]
-        cfg.io_dtype = _DTYPES[io_dtype] if io_dtype else (L.TK_BF16 if cfg.dtype == L.TK_FP8_E4M3 else cfg.dtype)
+        cfg.io_dtype = _DTYPES[io_dtype] if io_dtype else (L.TK_BF16 if cfg.dtype in (L.TK_FP8_E4M3, L.TK_INT8) else cfg.dtype)
         cfg.num_pages, cfg.max_seqs, cfg.max_pages_per_seq = num_pages, max_seqs, max_pages_per_seq
         cfg.max_step_tokens = max_step_tokens or max_seqs
         cfg.chunk_tokens, cfg.decode_impl = chunk_tokens, _IMPLS[decode_impl]
@@ -97,9 +98,8 @@ class PagedKVCache:
         if st != L.TK_OK:
             raise KvError(st, self._lib.tk_kv_last_error(self._h).decode())
 
-    @staticmethod
-    def _stream() -> int:
-        return torch.cuda.current_stream().cuda_stream
+    def _stream(self) -> int:
+        return torch.cuda.current_stream(self.device).cuda_stream
 
     def close(self) -> None:
         if getattr(self, "_h", None) and self._h.value:
@@ -237,6 +237,30 @@ class PagedKVCache:
             assert slots_out.dtype == torch.int64 and slots_out.numel() >= self._n_tokens
             sp = slots_out.data_ptr()
         self._check(self._lib.tk_kv_append(self._h, layer, k.data_ptr(), v.data_ptr(), sp, self._stream()))
+
+    def read(self, layer: int, seq_ids: Sequence[int], start: Optional[Sequence[int]] = None,
+             count: Optional[Sequence[int]] = None, out_dtype: Optional[torch.dtype] = None):
+        """K and V rows of tokens start[i] .. start[i] + count[i] - 1 of seq_ids[i], one range after the other:
+        -> (k [rows, Hkv, D], v [rows, Hkv, Dv]) in the io dtype or torch.float32, 8-bit storage dequantised.
+        start None: from 0; count None: up to each sequence's length."""
+        s = _i32(seq_ids)
+        lens = np.array([self.seq_len(int(x)) for x in s], dtype=np.int64)
+        a = np.zeros(len(s), dtype=np.int32) if start is None else _i32(start)
+        n = np.maximum(lens - a, -1).astype(np.int32) if count is None else _i32(count)
+        if len(a) != len(s) or len(n) != len(s):
+            raise KvError(L.TK_INVALID_ARG, "read: start and count need one entry for each sequence")
+        if out_dtype is None:
+            out_dtype = self.io_torch_dtype
+        if out_dtype not in (self.io_torch_dtype, torch.float32):
+            raise KvError(L.TK_INVALID_ARG, f"read: out dtype must be {self.io_torch_dtype} or torch.float32")
+        if self.host_only:
+            raise KvError(L.TK_CUDA_ERROR, "read: handle has no device (bookkeeping only)")
+        rows = int(np.maximum(n, 0).astype(np.int64).sum()) if (n.size and (a >= 0).all() and (a + n.astype(np.int64) <= lens).all()) else 0
+        k = torch.empty(rows, self.cfg.num_kv_heads, self.cfg.head_dim, dtype=out_dtype, device=self.device)
+        v = torch.empty(rows, self.cfg.num_kv_heads, self.cfg.v_head_dim, dtype=out_dtype, device=self.device)
+        self._check(self._lib.tk_kv_read(self._h, layer, len(s), _ptr(s), _ptr(a), _ptr(n), k.data_ptr(), v.data_ptr(),
+                                         L.TK_FP32 if out_dtype == torch.float32 else self.cfg.io_dtype, self._stream()))
+        return k, v
 
     def decode(self, layer: int, q: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """q: [n_seqs, H, D] -> out [n_seqs, H, D], io dtype."""
@@ -383,8 +407,8 @@ class PagedKVCache:
 
     def layer_views(self, layer: int):
         """(pool, scales, open_pages) tensors aliasing layer `layer` of the arena.
-        pool: [num_pages, Hkv, 2, page, D] (uint8 codes for FP8); scales: [num_pages, Hkv, 2] f32 or None;
-        open_pages: [max_seqs, Hkv, 2, page, D] io dtype or None."""
+        pool: [num_pages, Hkv, 2, page, D] (uint8 codes for FP8, uint8 code + 128 for INT8); scales: [num_pages, Hkv, 2] f32
+        (INT8: [num_pages, Hkv, 2, page]) or None; open_pages: [max_seqs, Hkv, 2, page, D] io dtype or None."""
         p, s, o = C.c_void_p(), C.c_void_p(), C.c_void_p()
         self._check(self._lib.tk_kv_layer_ptrs(self._h, layer, C.byref(p), C.byref(s), C.byref(o)))
         c = self.cfg
@@ -397,6 +421,12 @@ class PagedKVCache:
             oshape = (c.max_seqs, c.num_kv_heads, 2, c.page_size, c.head_dim)
             open_pages = self._view(o.value, int(np.prod(oshape)) * 2).view(self.io_torch_dtype).view(oshape)
             return pool, scales, open_pages
+        if c.dtype == L.TK_INT8:              # a tile: page_size K rows and V rows of codes, then their scales
+            codes = 2 * c.page_size * c.head_dim
+            tiles = self._view(p.value, c.num_pages * c.num_kv_heads * (codes + 8 * c.page_size)).view(
+                c.num_pages, c.num_kv_heads, codes + 8 * c.page_size)
+            return (tiles[..., :codes].unflatten(-1, (2, c.page_size, c.head_dim)),
+                    tiles[..., codes:].view(torch.float32).unflatten(-1, (2, c.page_size)), None)
         if c.v_head_dim != c.head_dim:        # MLA tile: page_size K rows of head_dim, then V rows of v_head_dim
             shape = (c.num_pages, c.num_kv_heads, c.page_size * (c.head_dim + c.v_head_dim))
             n = int(np.prod(shape))
