@@ -33,11 +33,15 @@ def attention(q, k, v, limits, out_type):
     most 2 r sum(p |v|) / sum(p) (numerator and denominator).  r adds up: 2^-11 for that rounding; the error of a score,
     (D + 8) products, sums and scalings of at most 2^-24 of sum |q k| / sqrt(D) each, which moves exp by as much; 2^-20 for
     the exponentials (two units in the last place each, a handful of factors) and the FP32 sums of the split and merged
-    rows.  The result is rounded to its type once more: half an eps of it."""
+    rows.  The result is rounded to its type once more: half an eps of it.
+    What is rounded to fp16 is w_j = p_j vs_j / 2^m (vs the value's scale), 2^m at most the largest p_j vs_j: where w_j is
+    below fp16's normal range its error is not 2^-11 of itself but half of fp16's smallest step, 2^-25.  It multiplies the
+    code, v_j / vs_j, and 2^m: at most 2^-25 max(p vs) sum |v_j / vs_j| / sum(p) in all."""
     q, k, v = (np.asarray(a, dtype=np.float64) for a in (q, k, v))
     T, H, D = q.shape
     G = H // k.shape[1]
     out, bound = np.zeros((T, H, D)), np.zeros((T, H, D))
+    vs = np.maximum(np.abs(v).max(axis=-1), 127.0 * 2.0 ** -48) / 127.0     # a row's largest code is 127 (or the row is zero)
     for h in range(H):
         s = q[:, h] @ k[:, h // G].T / np.sqrt(D)
         mag = np.abs(q[:, h]) @ np.abs(k[:, h // G]).T / np.sqrt(D)
@@ -48,7 +52,8 @@ def attention(q, k, v, limits, out_type):
         total = p.sum(axis=-1, keepdims=True) + 1e-8
         out[:, h] = p @ v[:, h // G] / total
         r = 2.0 ** -11 + (D + 8) * 2.0 ** -24 * np.where(seen, mag, 0.0).max(axis=-1, keepdims=True, initial=0.0) + 2.0 ** -20
-        bound[:, h] = 2.0 * r * (p @ np.abs(v[:, h // G]) / total)
+        w, codes = (p * vs[:, h // G]).max(axis=-1, keepdims=True, initial=0.0), np.abs(v[:, h // G]) / vs[:, h // G, None]
+        bound[:, h] = 2.0 * r * (p @ np.abs(v[:, h // G]) / total) + 2.0 ** -25 * w * (seen @ codes) / total
     return out, bound + EPS[out_type] / 2 * (np.abs(out) + bound) + 1e-30
 
 

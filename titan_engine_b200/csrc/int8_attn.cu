@@ -1,4 +1,4 @@
-// int8_attn.cu — attention over an INT8 pool, one CTA per (query token, head): decode steps and chunks of new tokens.
+// int8_attn.cu — attention over an INT8 pool, one CTA per (query token, head): chunks of new tokens.
 //
 // out = sum_j p_j v_j with p = softmax(q k_j / sqrt(D)) over the positions up to the query's own, k_j and v_j the rows the
 // codes stand for; running maximum from -1e30, FP32 sums, normaliser 1 / (sum + 1e-8): the arithmetic of
@@ -15,14 +15,12 @@ constexpr int kI8Warps = 4;
 template <bool BF16, int D>
 __global__ void __launch_bounds__(kI8Warps * 32)
 attn_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, StepDev st, const int32_t* __restrict__ page_table,
-                 const uint16_t* __restrict__ q, void* __restrict__ out, int out_dtype, float* __restrict__ partial_out,
-                 const int* __restrict__ status, int every_token) {
+                 const uint16_t* __restrict__ q, void* __restrict__ out, int out_dtype, const int* __restrict__ status) {
     constexpr int E = D / 32;
     __shared__ float red[kI8Warps][D + 2];
     if (__ldcg(status) != 0) return;                        // fail closed: a wait timed out on this handle
     const int row = blockIdx.x, h = blockIdx.y, kvh = h / (g.H / g.Hkv);
-    const int b = every_token ? st.tok_b[row] : row;
-    const int lim = every_token ? st.tok_pos[row] + 1 : st.len[b];
+    const int b = st.tok_b[row], lim = st.tok_pos[row] + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float qf[E], o[E];
 #pragma unroll
@@ -60,25 +58,19 @@ attn_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, StepDev st, const
     for (int d = threadIdx.x; d < D; d += kI8Warps * 32) {
         float acc = 0.0f;
         for (int w = 0; w < kI8Warps; w++) acc += red[w][d] * expf(red[w][D] - M);
-        if (out) store_out(out, ((size_t)row * g.H + h) * D + d, acc * inv, out_dtype);
-        if (partial_out) partial_out[partial_off(row, h, g.H, D) + d] = acc;
-    }
-    if (partial_out && threadIdx.x == 0) {
-        partial_out[partial_off(row, h, g.H, D) + D] = M;
-        partial_out[partial_off(row, h, g.H, D) + D + 1] = L;
+        store_out(out, ((size_t)row * g.H + h) * D + d, acc * inv, out_dtype);
     }
 }
 
 }  // namespace
 
 cudaError_t launch_attn_int8(const Geometry& g, const LayerPtrs& lp, const StepDev& st, const int32_t* page_table, const void* q,
-                             void* out, int out_dtype, float* partial_out, const int* status, bool every_token, cudaStream_t s) {
-    const dim3 grid(every_token ? st.n_tokens : st.n_seqs, g.H);
+                             void* out, int out_dtype, const int* status, cudaStream_t s) {
+    const dim3 grid(st.n_tokens, g.H);
     if (grid.x == 0) return cudaSuccess;
     auto kern = g.io_dtype == DT_BF16 ? (g.D == 128 ? attn_int8_kernel<true, 128> : attn_int8_kernel<true, 64>)
                                       : (g.D == 128 ? attn_int8_kernel<false, 128> : attn_int8_kernel<false, 64>);
-    kern<<<grid, kI8Warps * 32, 0, s>>>(g, (const uint8_t*)lp.pool, st, page_table, (const uint16_t*)q, out, out_dtype, partial_out,
-                                        status, every_token ? 1 : 0);
+    kern<<<grid, kI8Warps * 32, 0, s>>>(g, (const uint8_t*)lp.pool, st, page_table, (const uint16_t*)q, out, out_dtype, status);
     return cudaGetLastError();
 }
 

@@ -392,8 +392,9 @@ int create_impl(const tk_kv_config* cfg_in, void* arena, size_t arena_bytes, boo
 
     // MLA shape: tensor-core kernel of its own; cold pages stay on the generic kernel
     h->mla_mma = tk::decode_mma_mla_supported(h->geo) && c.hot_window == 0;
-    const bool mma_ok = tk::decode_mma_supported(h->geo) || h->mla_mma;
-    if (c.decode_impl == TK_DECODE_MMA && !mma_ok && c.dtype != TK_INT8) {
+    const bool int8 = c.dtype == TK_INT8;
+    const bool mma_ok = tk::decode_mma_supported(h->geo) || h->mla_mma || int8;
+    if (c.decode_impl == TK_DECODE_MMA && !mma_ok) {
         release(h);
         return fail(nullptr, TK_UNSUPPORTED, "decode_impl=MMA needs page_size 16 and head_dim 64/128 (128 for FP8), or the "
                                              "192/128 shape with 16-bit storage, groups of <= 8 heads and no cold tier");
@@ -404,7 +405,8 @@ int create_impl(const tk_kv_config* cfg_in, void* arena, size_t arena_bytes, boo
         h->maps.resize(c.num_layers);
         if (h->mla_mma) h->maps_v.resize(c.num_layers);
         for (int l = 0; l < c.num_layers; l++) {
-            if (h->mla_mma) CREATE_CUDA(tk::make_mla_tensor_maps(h->geo, h->layer(l).pool, &h->maps[l], &h->maps_v[l]));
+            if (int8) CREATE_CUDA(tk::make_int8_tensor_map(h->geo, h->layer(l).pool, &h->maps[l]));
+            else if (h->mla_mma) CREATE_CUDA(tk::make_mla_tensor_maps(h->geo, h->layer(l).pool, &h->maps[l], &h->maps_v[l]));
             else CREATE_CUDA(tk::make_pool_tensor_map(h->geo, h->layer(l).pool, &h->maps[l]));
         }
         h->prefill_tc = !h->mla_mma && c.prefill_impl != TK_PREFILL_MMA_SYNC && c.hot_window == 0 && tk::prefill_tc_supported(h->geo);
@@ -948,15 +950,6 @@ static int decode_impl(tk_kv* h, int layer, const void* q, void* out, float* par
     if (out_dtype < 0) out_dtype = h->cfg.io_dtype;
     if (out_dtype != TK_FP32 && out_dtype != h->cfg.io_dtype)
         return fail(h, TK_INVALID_ARG, "decode: out dtype must be FP32 or the handle's io dtype");
-    if (h->cfg.dtype == TK_INT8) {
-        if (peer_ctx || fuse_k || rope) return fail(h, TK_UNSUPPORTED, "decode: not fused on an INT8 pool");
-        const bool bracket = h->profiling && h->prof_used + 2 <= h->prof_ev.size();
-        if (bracket) cudaEventRecord(h->prof_ev[h->prof_used], s);
-        e = tk::launch_attn_int8(h->geo, lp, h->dev, h->d_table, q, out, out_dtype, partial_out, h->d_status, false, s);
-        h->launches++;
-        if (bracket) { cudaEventRecord(h->prof_ev[h->prof_used + 1], s); h->prof_used += 2; }
-        return e == cudaSuccess ? TK_OK : fail(h, TK_CUDA_ERROR, "decode launch: %s", cudaGetErrorString(e));
-    }
     const bool mma = h->use_mma && h->dev.chunk_tokens <= 2048;
     // the last CTA of each (sequence, kv head) merges the split-KV rows itself; a sequence that
     // attends to nothing has no CTA, so such steps keep the separate combine kernel
@@ -974,7 +967,10 @@ static int decode_impl(tk_kv* h, int layer, const void* q, void* out, float* par
             // not touch, and it waits for the earlier kernel before it writes split-KV rows or `out`.
             const bool overlap = h->cfg.launch_overlap == TK_OVERLAP_AUTO && !cold && !timed &&
                                  h->chain_launches == h->launches && h->chain_stream == s && h->chain_layer != layer;
-            if (h->mla_mma)
+            if (h->cfg.dtype == TK_INT8)
+                e = tk::launch_decode_int8(h->geo, lp, &h->maps[layer], h->dev, h->d_table, q, h->d_partials, h->d_status, s, mo, fa,
+                                           false, overlap);
+            else if (h->mla_mma)
                 e = tk::launch_decode_mma_mla(h->geo, lp, &h->maps[layer], &h->maps_v[layer], h->dev, h->d_table, q,
                                               h->d_partials, h->d_status, s, &mo, &fa, overlap);
             else
@@ -1020,7 +1016,7 @@ int tk_kv_append_decode(tk_kv* h, int32_t layer, const void* k, const void* v, c
     // goes into the sequence's 16-bit open page, unless this step completes (seals) a page.
     const bool fusable = h->use_mma && h->plan.one_token_steps && h->dev.chunk_tokens <= 2048 &&
                          h->dev.n_tokens > 0 && h->dev.n_seqs > 0 && !h->plan.has_empty_seq &&
-                         (h->cfg.dtype != TK_FP8_E4M3 || h->plan.seals.empty());
+                         (h->cfg.dtype != TK_FP8_E4M3 || h->plan.seals.empty()) && !(h->cfg.dtype == TK_INT8 && h->plan.capped);
     if (!fusable) {
         int st = tk_kv_append(h, layer, k, v, nullptr, stream);
         if (st != TK_OK) return st;
@@ -1039,7 +1035,7 @@ int tk_kv_rope_append_decode(tk_kv* h, int32_t layer, const void* k, const void*
     if (!q || !out || (h->dev.n_tokens > 0 && (!k || !v))) return fail(h, TK_INVALID_ARG, "rope_append_decode: null argument");
     const bool fusable = h->use_mma && h->cfg.dtype != TK_FP8_E4M3 && h->plan.one_token_steps &&
                          h->dev.chunk_tokens <= 2048 && h->dev.n_tokens > 0 && h->dev.n_seqs > 0 &&
-                         !h->plan.has_empty_seq;
+                         !h->plan.has_empty_seq && !(h->cfg.dtype == TK_INT8 && h->plan.capped);
     if (fusable) {
         const float rope[2] = {theta, scaling};
         // cos/sin of each sequence's newest position: computed once per step, shared by all layers
@@ -1095,8 +1091,16 @@ static int decode_multi_impl(tk_kv* h, int32_t layer, const void* q, void* out, 
     if (p.nq_min < 1) return fail(h, TK_INVALID_ARG, "decode_multi: every sequence of the step must append at least one token");
     if (h->cfg.dtype == TK_INT8) {
         if (p.capped) return fail(h, TK_UNSUPPORTED, "decode_multi: not available on a step with capped lengths (INT8 storage)");
-        const cudaError_t e = tk::launch_attn_int8(h->geo, h->layer(layer), h->dev, h->d_table, q, out, out_dtype, nullptr, h->d_status,
-                                                   true, (cudaStream_t)stream);
+        cudaError_t e;
+        if (h->geo.H / h->geo.Hkv * p.nq_max <= tk::kDecodeTileRows) {       // a few tokens: together through the decode kernel
+            float* ws = multi_workspace(h, (size_t)p.chunk_base[h->dev.n_seqs] * h->geo.H * p.nq_max * (h->geo.Dv + 2), (cudaStream_t)stream);
+            if (!ws) return TK_CUDA_ERROR;
+            e = tk::launch_decode_int8(h->geo, h->layer(layer), &h->maps[layer], h->dev, h->d_table, q, ws, h->d_status, (cudaStream_t)stream,
+                                       tk::MergeOut{h->d_counters, out, nullptr, out_dtype, nullptr, h->d_status},
+                                       tk::FuseAppend{nullptr, nullptr, nullptr}, true, false);
+        } else {
+            e = tk::launch_attn_int8(h->geo, h->layer(layer), h->dev, h->d_table, q, out, out_dtype, h->d_status, (cudaStream_t)stream);
+        }
         h->launches++;
         return e == cudaSuccess ? TK_OK : fail(h, TK_CUDA_ERROR, "decode_multi launch: %s", cudaGetErrorString(e));
     }

@@ -244,9 +244,12 @@ class PagedKVCache:
         -> (k [rows, Hkv, D], v [rows, Hkv, Dv]) in the io dtype or torch.float32, 8-bit storage dequantised.
         start None: from 0; count None: up to each sequence's length."""
         s = _i32(seq_ids)
-        lens = np.array([self.seq_len(int(x)) for x in s], dtype=np.int64)
         a = np.zeros(len(s), dtype=np.int32) if start is None else _i32(start)
-        n = np.maximum(lens - a, -1).astype(np.int32) if count is None else _i32(count)
+        if count is None:
+            n = np.array([self.seq_len(int(x)) for x in s], dtype=np.int32)
+            n = n - a if len(a) == len(s) else n
+        else:
+            n = _i32(count)
         if len(a) != len(s) or len(n) != len(s):
             raise KvError(L.TK_INVALID_ARG, "read: start and count need one entry for each sequence")
         if out_dtype is None:
@@ -255,7 +258,9 @@ class PagedKVCache:
             raise KvError(L.TK_INVALID_ARG, f"read: out dtype must be {self.io_torch_dtype} or torch.float32")
         if self.host_only:
             raise KvError(L.TK_CUDA_ERROR, "read: handle has no device (bookkeeping only)")
-        rows = int(np.maximum(n, 0).astype(np.int64).sum()) if (n.size and (a >= 0).all() and (a + n.astype(np.int64) <= lens).all()) else 0
+        if n.size and (n.min() < 0 or n.max() > self.cfg.num_pages * self.cfg.page_size):
+            raise KvError(L.TK_INVALID_ARG, "read: ranges must lie inside live sequences' tokens")
+        rows = int(n.sum(dtype=np.int64))
         k = torch.empty(rows, self.cfg.num_kv_heads, self.cfg.head_dim, dtype=out_dtype, device=self.device)
         v = torch.empty(rows, self.cfg.num_kv_heads, self.cfg.v_head_dim, dtype=out_dtype, device=self.device)
         self._check(self._lib.tk_kv_read(self._h, layer, len(s), _ptr(s), _ptr(a), _ptr(n), k.data_ptr(), v.data_ptr(),
