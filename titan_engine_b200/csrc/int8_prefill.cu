@@ -1,0 +1,536 @@
+// int8_prefill.cu — attention for every token of a chunk over an INT8 pool on the 5th-generation tensor cores.
+//
+// Mathematics: that of int8_decode.cu.  With codes K, V and the scales ks, vs of their rows,
+//   x_j = ks_j (q K_j) log2(e)/sqrt(D) + log2(vs_j),   w_j = 2^(x_j - m),   out = sum_j w_j V_j / sum_j w_j / vs_j
+// the codes enter the products as fp16 without rounding, w_j <= 2^8 is the only value rounded to 16 bits, sums are FP32,
+// a bf16 query row is scaled by a power of two to fit fp16.
+//
+// One CTA per SM = one tile of 256 (token, head) rows of a (sequence, kv head) x a range of the context, as two halves of
+// 128 rows (the lanes of tensor memory) that take turns on the tensor pipe.  Per block of 64 tokens (4 pages):
+//   loader warp      one bulk copy per page: the page's tile - codes and scales - is contiguous; 3 stages
+//   4 expander warps codes -> fp16 into the 128-byte-swizzled slabs the MMAs read (2 K and 2 V stages), and the three
+//                    numbers per token the softmax needs: ks log2(e)/sqrt(D), log2 vs, 1/vs (4 stages)
+//   MMA thread       S = Q K^T (M 128, N 64) and O += W V (M 128, N D, W from tensor memory) for both halves
+//   8 softmax warps  thread t owns row t: a speculative pass against the current reference, redone when a score exceeds it
+//                    by 2^8 or the block is cut; only then O is rescaled (prefill_tc.cu describes the scheme)
+// The expansion is what an 8-bit cache costs over a 16-bit one: 2 D values per token, shared here by 256 rows - about an
+// eighth of the issue slots - where two CTAs of 128 rows would each do it.  Tensor memory: per half two S buffers of 64
+// columns and O of D: all 512 columns at D = 128.
+// Bound: tensor pipe and special-function unit together, 512 clocks each per 128 x 64 block at D = 128.
+// Every wait is bounded; on expiry the status word is set, nothing is written, and the CTA waits for its copies and frees its
+// tensor memory before it returns.  No cluster, no multicast, this GPU's memory only.
+#include "int8_cache.cuh"
+#include "tk_merge.cuh"
+#include "tk_mma.cuh"
+#include "tk_tcgen05.cuh"
+
+namespace tk {
+
+namespace {
+
+constexpr int kPfRows = kPrefillRowsInt8;       // 256: two halves of kTcRows
+constexpr int kPfBlock = 64;                    // context tokens per block (4 pages)
+constexpr int kPfRaw = 3;                       // stages of raw tiles
+constexpr int kPfSoftWarps = kPfRows / 32, kPfExpWarps = 4;
+constexpr int kPfMmaWarp = kPfSoftWarps + kPfExpWarps, kPfLoadWarp = kPfMmaWarp + 1;
+constexpr int kPfThreads = (kPfLoadWarp + 1) * 32;
+constexpr int kPfExpThreads = kPfExpWarps * 32;
+constexpr uint32_t kPfTmemCols = 512, kPfHalfCols = 256, kPfColO = 128;   // half h: S at 256h and 256h + 64, O at 256h + 128
+
+template <int D>
+struct PfCfg {
+    static constexpr int HALVES = D / 64;                   // 64-dim halves of a row: 128 bytes of fp16 each
+    static constexpr int TILE = i8_tile_bytes(D);
+    static constexpr int Q_BYTES = HALVES * kPfRows * 128;  // [tile half][dim half][128 rows][128 B]
+    static constexpr int SLAB = HALVES * kPfBlock * 128;    // K or V of a block: [dim half][64 tokens][128 B]
+    static constexpr int HALF = kPfBlock * 128;
+    static constexpr int RAW = 4 * TILE;
+    static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + 2 * SLAB, OFF_RAW = OFF_V + 2 * SLAB, OFF_SC = OFF_RAW + kPfRaw * RAW,
+                         OFF_E = OFF_SC + 4 * 3 * kPfBlock * 4, OFF_PAGES = OFF_E + kPfRows * 4, OFF_BARS = OFF_PAGES + kPrefillMaxPages * 4,
+                         SMEM = OFF_BARS + 256 + 1024;
+};
+
+__device__ __forceinline__ uint32_t pf_expand(uint32_t w, uint32_t sel) {      // two codes as fp16, exact: 1024 + u, minus 1152
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0x64646464u), "r"(sel));
+    const uint32_t bias = 0x64806480u;
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&bias));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void fma2v(float& r0, float& r1, float a0, float a1, float b0, float b1, float c0, float c1) {
+    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}" : "=f"(r0), "=f"(r1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mul2v(float& r0, float& r1, float a0, float a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+        "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}" : "=f"(r0), "=f"(r1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ float pf_lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float pf_pow2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+// contiguous copy, global -> this CTA's shared memory; the other tiles of the sequence read the same pages: keep them in L2
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(policy));
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(policy) : "memory");
+}
+
+template <int D, bool IO_BF16>
+__global__ void __launch_bounds__(kPfThreads, 1)
+prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf, const int32_t* __restrict__ page_table,
+                    const uint16_t* __restrict__ q, void* __restrict__ out, int out_dtype, float* __restrict__ partials,
+                    int* __restrict__ counters, int* __restrict__ status) {
+    using C = PfCfg<D>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t *s_q = smem, *s_k = smem + C::OFF_K, *s_v = smem + C::OFF_V, *s_raw = smem + C::OFF_RAW;
+    float* s_sc = (float*)(smem + C::OFF_SC);               // [4][3][64]: ks log2(e)/sqrt(D), log2 vs, 1/vs
+    float* s_e = (float*)(smem + C::OFF_E);                 // [256] power of two of the row's query
+    int32_t* s_pages = (int32_t*)(smem + C::OFF_PAGES);
+    uint64_t* bars = (uint64_t*)(smem + C::OFF_BARS);
+    uint64_t *rawfull = bars, *rawempty = bars + 3, *kfull = bars + 6, *kempty = bars + 8, *vfull = bars + 10, *vempty = bars + 12,
+             *scfull = bars + 14, *bar_s = bars + 18 /* [half][2] */, *p_ready = bars + 22 /* [half][2] */, *bar_o = bars + 26 /* [half] */;
+    uint32_t* s_tmem = (uint32_t*)(bars + 28);
+    int* s_flag = (int*)(s_tmem + 1);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int G = g.H / g.Hkv;
+    const int4 it = pf.items[blockIdx.x], i0 = pf.info[2 * blockIdx.x], i1 = pf.info[2 * blockIdx.x + 1];
+    const int b = it.x, chunk = it.y, kvh = it.z, tile = it.w;
+    const int seq = i0.x, len = i0.y, nq = i0.z, ct = i0.w;
+    const int q_base = i1.x, poff = i1.y, cbase = i1.z;
+    const int tpt = kPfRows / G;                            // query tokens per tile
+    const int tok_first = tile * tpt;
+    const int tok_cnt = min(nq - tok_first, tpt);
+    const int halves = tok_cnt * G > kTcRows ? 2 : 1;
+    const int base_pos = len - nq;
+    const int p_last = base_pos + tok_first + tok_cnt - 1;
+    const int t0 = chunk * ct, t1 = min(t0 + ct, p_last + 1);
+    const int n_pages = (t1 - t0 + kI8Page - 1) / kI8Page;
+    const int n_blocks = (n_pages + 3) / 4;
+    const int n_chunks = p_last / ct + 1;
+    const int32_t* pt_row = page_table + (size_t)seq * g.max_pages_per_seq + t0 / kI8Page;
+
+    // this thread's row (softmax warps): query token tid / G of the tile, head tid % G of the group
+    const bool valid = tid < kPfRows && tid / G < tok_cnt;
+    const int lim = base_pos + tok_first + tid / G + 1;     // positions the row sees: [0, lim)
+    const size_t qo_row = (size_t)(q_base + tok_first + tid / G) * g.H + (size_t)kvh * G + tid % G;
+
+    // ---- prologue ----
+    constexpr int LPR = D / 8;                              // lanes (16-byte vectors) per query row
+    uint4 qv[LPR];
+    if (tid < kPfRows) {
+        const int sh = __ffs(G) - 1;                        // G divides 128: a power of two
+#pragma unroll
+        for (int i = 0; i < LPR; i++) {
+            const int r = (i * kPfRows + tid) / LPR, c = tid % LPR;
+            const size_t row = (size_t)(q_base + tok_first + (r >> sh)) * g.H + (size_t)kvh * G + (r & (G - 1));
+            qv[i] = (r >> sh) < tok_cnt ? __ldg(reinterpret_cast<const uint4*>(q + row * D) + c) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(smem_u32(&kfull[i]), kPfExpThreads); mbar_init(smem_u32(&vfull[i]), kPfExpThreads);
+            mbar_init(smem_u32(&kempty[i]), 1); mbar_init(smem_u32(&vempty[i]), 1);
+            mbar_init(smem_u32(&bar_o[i]), 1);
+        }
+        for (int i = 0; i < 4; i++) {
+            mbar_init(smem_u32(&scfull[i]), kPfBlock);
+            mbar_init(smem_u32(&bar_s[i]), 1);
+            mbar_init(smem_u32(&p_ready[i]), kTcRows);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kPfMmaWarp) {
+        tmem_alloc(smem_u32(s_tmem), kPfTmemCols);
+        tmem_relinquish();
+    }
+    // one copy per page of the block; `pages_of` = the page table itself for the first blocks, its copy in shared memory later
+    auto load_block = [&](int blk, const int32_t* pages_of) {
+        const int s = blk % kPfRaw, pages = min(4, n_pages - 4 * blk);
+        const uint32_t bar = smem_u32(&rawfull[s]);
+        if (lane == 0) mbar_expect_tx(bar, pages * C::TILE);
+        __syncwarp();
+        if (lane < pages)
+            bulk_load(smem_u32(s_raw + s * C::RAW + lane * C::TILE), pool + ((size_t)pages_of[4 * blk + lane] * g.Hkv + kvh) * C::TILE, C::TILE, bar);
+    };
+    if (warp == kPfLoadWarp) {
+        if (lane == 0) {
+            for (int i = 0; i < kPfRaw; i++) { mbar_init(smem_u32(&rawfull[i]), 1); mbar_init(smem_u32(&rawempty[i]), kPfExpThreads); }
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        for (int blk = 0; blk < kPfRaw && blk < n_blocks; blk++) load_block(blk, pt_row);
+    }
+    for (int i = tid; i < n_pages; i += kPfThreads) s_pages[i] = pt_row[i];
+    if (tid < kPfRows) {
+#pragma unroll
+        for (int i = 0; i < LPR; i++) {
+            const int r = (i * kPfRows + tid) / LPR, c = tid % LPR;
+            uint4 x = qv[i];
+            if (IO_BF16) {
+                uint32_t m = i8_absmax8(x);
+#pragma unroll
+                for (int off = LPR / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
+                const int e = m ? max((int)(m >> 7) - 127 - 14, -100) : 0;      // the largest element becomes 2^14 .. 2^15
+                const float down = pf_pow2i(-e);
+                uint32_t* w = &x.x;
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const float2 f = i8_unpack2<true>(w[u]);
+                    w[u] = pack2<false>(f.x * down, f.y * down);
+                }
+                if (c == 0) s_e[r] = pf_pow2i(e);
+            }
+            // 128-byte-swizzled K-major rows: 16-byte chunk c of a row sits at chunk c ^ (row & 7)
+            *reinterpret_cast<uint4*>(s_q + ((r / kTcRows) * C::HALVES + (c >> 3)) * (kTcRows * 128) + (r % kTcRows) * 128 +
+                                      (((c & 7) ^ (r & 7)) << 4)) = x;
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // generic writes above -> visible to the MMAs
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *s_tmem;
+
+    bool alive = true;
+    float m2 = -1e30f, l_run = 0.0f;                        // softmax state of this thread's row, m2 in base-2 units
+    constexpr float kLazy = 8.0f;
+
+    if (warp == kPfMmaWarp) {
+        // ===== MMA warp: one thread feeds the tensor pipe =====
+        if (lane == 0) {
+            constexpr uint32_t kIdescS = instr_desc(false, false, kPfBlock), kIdescO = instr_desc(false, true, D);
+            const uint64_t desc_q = smem_desc(smem_u32(s_q), 16), desc_k = smem_desc(smem_u32(s_k), 16),
+                           desc_v = smem_desc(smem_u32(s_v), C::HALF);
+            auto issue_s = [&](int half, int blk) {
+                const uint64_t dq = desc_q + (uint64_t)((half * C::HALVES * kTcRows * 128) >> 4);
+                const uint64_t dk = desc_k + (uint64_t)(((blk & 1) * C::SLAB) >> 4);
+                const uint32_t d_s = tmem + half * kPfHalfCols + 64u * (blk & 1);
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ks++)
+                    tc_mma_ss(d_s, dq + (uint64_t)(((ks >> 2) * (kTcRows * 128) + (ks & 3) * 32) >> 4),
+                              dk + (uint64_t)(((ks >> 2) * C::HALF + (ks & 3) * 32) >> 4), kIdescS, ks > 0);
+                tc_commit(smem_u32(&bar_s[2 * half + (blk & 1)]));
+                if (half == halves - 1) tc_commit(smem_u32(&kempty[blk & 1]));       // (covers the other half's too)
+            };
+            bool ok = true;
+            for (int blk = 0; blk < 2 && blk < n_blocks && ok; blk++) {
+                ok = mbar_wait_bounded_idle(smem_u32(&kfull[blk]), 0u, status);
+                if (!ok) break;
+                tc_fence_after();
+                for (int half = 0; half < halves; half++) issue_s(half, blk);
+            }
+            for (int blk = 0; blk < n_blocks && ok; blk++) {
+                const int s = blk & 1;
+                const uint32_t ph = (uint32_t)((blk >> 1) & 1);
+                const uint64_t dv = desc_v + (uint64_t)((s * C::SLAB) >> 4);
+                ok = mbar_wait_bounded_idle(smem_u32(&vfull[s]), ph, status);
+                for (int half = 0; half < halves && ok; half++) {
+                    // every row's W of this block is in tensor memory (and O rescaled): O += W V, then S of the block after next
+                    ok = mbar_wait_bounded_idle(smem_u32(&p_ready[2 * half + s]), ph, status);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t base = tmem + half * kPfHalfCols;
+#pragma unroll
+                    for (int ks = 0; ks < 4; ks++)           // 16 tokens per MMA: 8 columns of W, 16 rows of the V slab
+                        tc_mma_ts(base + kPfColO, base + 64u * s + 8 * ks, dv + (uint64_t)((ks * 2048) >> 4), kIdescO, (blk > 0 || ks > 0) ? 1u : 0u);
+                    tc_commit(smem_u32(&bar_o[half]));
+                    if (half == halves - 1) tc_commit(smem_u32(&vempty[s]));
+                    if (blk + 2 < n_blocks) {                // MMAs run in order: S(blk+2) overwrites the columns after W V has read them
+                        if (half == 0) {
+                            ok = mbar_wait_bounded_idle(smem_u32(&kfull[s]), (uint32_t)(((blk + 2) >> 1) & 1), status);
+                            tc_fence_after();
+                        }
+                        if (ok) issue_s(half, blk + 2);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == kPfLoadWarp) {
+        // ===== loader warp (the first kPfRaw blocks left in the prologue) =====
+        int issued = min(kPfRaw, n_blocks);
+        for (int blk = kPfRaw; blk < n_blocks; blk++) {
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded_idle(smem_u32(&rawempty[blk % kPfRaw]), (uint32_t)((blk / kPfRaw - 1) & 1), status))) break;
+            load_block(blk, s_pages);
+            issued = blk + 1;
+        }
+        // no copy of this CTA may be in flight when it returns, whatever became of the other roles
+        for (int blk = max(0, issued - kPfRaw); blk < issued; blk++)
+            (void)__all_sync(0xFFFFFFFFu, mbar_wait_bounded_idle(smem_u32(&rawfull[blk % kPfRaw]), (uint32_t)((blk / kPfRaw) & 1), status));
+    } else if (warp >= kPfSoftWarps) {
+        // ===== expander warps: codes -> fp16 slabs =====
+        const int et = tid - kPfSoftWarps * 32;
+        const float sc2 = kLog2e / sqrtf((float)D);
+        constexpr int CPR = D / 16;                         // 16-code chunks per row
+        auto expand = [&](const uint8_t* raw, int kv, uint8_t* slab) {
+#pragma unroll
+            for (int i = 0; i < kPfBlock * CPR / kPfExpThreads; i++) {
+                const int u = i * kPfExpThreads + et, r = u / CPR, c = u % CPR;
+                uint4 w = *reinterpret_cast<const uint4*>(raw + (r / kI8Page) * C::TILE + i8_row_off(D, kv, r % kI8Page) + c * 16);
+                // 16 codes = two 16-byte chunks 2c, 2c+1 of the fp16 row.  At D = 128 a quarter warp stores one row: lanes of the
+                // second dim half store their chunks in the other order, or both halves would meet in the same banks.
+                const int swap = D == 128 ? c >> 2 : 0;
+                if (swap) w = make_uint4(w.z, w.w, w.x, w.y);
+                const uint4 lo = make_uint4(pf_expand(w.x, 0x4140), pf_expand(w.x, 0x4342), pf_expand(w.y, 0x4140), pf_expand(w.y, 0x4342));
+                const uint4 hi = make_uint4(pf_expand(w.z, 0x4140), pf_expand(w.z, 0x4342), pf_expand(w.w, 0x4140), pf_expand(w.w, 0x4342));
+                uint8_t* row = slab + (c >> 2) * C::HALF + r * 128;
+                const int c2 = 2 * (c & 3);
+                *reinterpret_cast<uint4*>(row + (((c2 + swap) ^ (r & 7)) << 4)) = lo;
+                *reinterpret_cast<uint4*>(row + (((c2 + 1 - swap) ^ (r & 7)) << 4)) = hi;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        };
+        for (int blk = 0; blk < n_blocks; blk++) {
+            const int s = blk & 1, rs = blk % kPfRaw;
+            const uint8_t* raw = s_raw + rs * C::RAW;
+            if (!mbar_wait_bounded(smem_u32(&rawfull[rs]), (uint32_t)((blk / kPfRaw) & 1), status)) break;
+            if (blk >= 2 && !mbar_wait_bounded(smem_u32(&kempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) break;
+            expand(raw, 0, s_k + s * C::SLAB);
+            if (et < kPfBlock) {
+                // (the numbers of block blk - 4 are out of use: S of block blk - 2, whose slab was just handed back, was
+                // issued after every row's W of block blk - 4)
+                const uint8_t* t = raw + (et / kI8Page) * C::TILE;
+                const bool in = t0 + blk * kPfBlock + et < t1;      // behind the range: whatever the page's last owner left
+                const float ks = *reinterpret_cast<const float*>(t + i8_scale_off(D, 0, et % kI8Page));
+                const float vs = *reinterpret_cast<const float*>(t + i8_scale_off(D, 1, et % kI8Page));
+                float* o = s_sc + (blk & 3) * 3 * kPfBlock + et;
+                o[0] = in ? ks * sc2 : 0.0f;
+                o[kPfBlock] = in ? pf_lg2(vs) : 0.0f;
+                o[2 * kPfBlock] = in ? __fdividef(1.0f, vs) : 0.0f;
+                mbar_arrive(smem_u32(&scfull[blk & 3]));
+            }
+            mbar_arrive(smem_u32(&kfull[s]));
+            if (blk >= 2 && !mbar_wait_bounded(smem_u32(&vempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) break;
+            expand(raw, 1, s_v + s * C::SLAB);
+            mbar_arrive(smem_u32(&vfull[s]));
+            mbar_arrive(smem_u32(&rawempty[rs]));
+        }
+    } else if (warp < halves * (kTcRows / 32)) {
+        // ===== softmax warps: thread t owns row t =====
+        const int half = warp >> 2;
+        const uint32_t base = tmem + half * kPfHalfCols + ((uint32_t)((warp & 3) * 32) << 16);    // this warp's 32 lanes
+        const float E = IO_BF16 ? s_e[tid] : 1.0f;
+        for (int blk = 0; blk < n_blocks; blk++) {
+            const int buf = blk & 1;
+            const uint32_t col_s = base + 64u * buf;         // S of this block; its first 32 columns become W
+            const int tok_base = t0 + blk * kPfBlock;
+            const float* sc = s_sc + (blk & 3) * 3 * kPfBlock;
+            bool ok = mbar_wait_bounded(smem_u32(&scfull[blk & 3]), (uint32_t)((blk >> 2) & 1), status) &&
+                      mbar_wait_bounded(smem_u32(&bar_s[2 * half + buf]), (uint32_t)((blk >> 1) & 1), status);
+            if (!__all_sync(0xFFFFFFFFu, ok)) { alive = false; break; }
+            tc_fence_after();
+            const int nv = valid ? max(0, min(min(kPfBlock, t1 - tok_base), lim - tok_base)) : 0;
+            const bool full = __all_sync(0xFFFFFFFFu, nv == kPfBlock && m2 > -1e29f);
+            bool moved = false, settled = false;
+            float alpha = 1.0f;
+            if (full) {
+                // One pass against the current reference, 16 columns of S at a time, the next 16 on their way; S stays in tensor
+                // memory until no row of the warp needs it again.
+                uint32_t sr[2][16], pr[32];
+                float l0 = 0.0f, l1 = 0.0f, top = -1e30f;    // top: largest x - m2 of the block
+                const float nm = -m2;
+                tmem_ld16(col_s, sr[0]);
+#pragma unroll
+                for (int qt = 0; qt < 4; qt++) {
+                    tc_wait_ld16(sr[qt & 1]);
+                    if (qt < 3) tmem_ld16(col_s + 16 * (qt + 1), sr[(qt + 1) & 1]);
+#pragma unroll
+                    for (int c4 = 0; c4 < 4; c4++) {         // tokens 16 qt + 4 c4 .. + 3
+                        const int t = 16 * qt + 4 * c4;
+                        const float4 ks = *reinterpret_cast<const float4*>(sc + t), lv = *reinterpret_cast<const float4*>(sc + kPfBlock + t),
+                                     iv = *reinterpret_cast<const float4*>(sc + 2 * kPfBlock + t);
+                        const float a0 = __uint_as_float(sr[qt & 1][4 * c4]), a1 = __uint_as_float(sr[qt & 1][4 * c4 + 1]),
+                                    a2 = __uint_as_float(sr[qt & 1][4 * c4 + 2]), a3 = __uint_as_float(sr[qt & 1][4 * c4 + 3]);
+                        float x0, x1, x2, x3;
+                        if (IO_BF16) {
+                            mul2v(x0, x1, a0, a1, ks.x, ks.y); mul2v(x2, x3, a2, a3, ks.z, ks.w);
+                            float u0 = lv.x, u1 = lv.y, u2 = lv.z, u3 = lv.w;
+                            add2(u0, u1, nm, nm); add2(u2, u3, nm, nm);
+                            fma2v(x0, x1, x0, x1, E, E, u0, u1); fma2v(x2, x3, x2, x3, E, E, u2, u3);
+                        } else {
+                            fma2v(x0, x1, a0, a1, ks.x, ks.y, lv.x, lv.y); fma2v(x2, x3, a2, a3, ks.z, ks.w, lv.z, lv.w);
+                            add2(x0, x1, nm, nm); add2(x2, x3, nm, nm);
+                        }
+                        top = fmaxf(fmaxf(top, fmaxf(x0, x1)), fmaxf(x2, x3));
+                        const float w0 = ex2(x0), w1 = ex2(x1), w2 = ex2(x2), w3 = ex2(x3);
+                        fma2v(l0, l1, w0, w1, iv.x, iv.y, l0, l1); fma2v(l0, l1, w2, w3, iv.z, iv.w, l0, l1);
+                        pr[t / 2] = pack2<false>(w0, w1); pr[t / 2 + 1] = pack2<false>(w2, w3);
+                    }
+                }
+                moved = top > kLazy;
+                if (!__any_sync(0xFFFFFFFFu, moved)) {
+                    l_run += l0 + l1;
+                    tmem_st32(col_s, pr);                    // W over the columns S was read from
+                    settled = true;
+                }
+            }
+            if (!settled) {
+                // the careful pass: masks, the new reference of every row that moved, and its weights
+                float mx = -INFINITY;
+                uint32_t sr[32];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    tmem_ld32(col_s + 32 * h, sr);
+                    tc_wait_ld(sr);
+#pragma unroll
+                    for (int c = 0; c < 32; c++) {
+                        const int t = 32 * h + c;
+                        const float x = fmaf(__uint_as_float(sr[c]) * sc[t], E, sc[kPfBlock + t]);
+                        if (t < nv) mx = fmaxf(mx, x);
+                    }
+                }
+                moved = mx > m2 + kLazy;
+                const float m_new = moved ? mx : m2;
+                alpha = moved ? ex2(m2 - m_new) : 1.0f;      // a row's first block: 0
+                float sum = 0.0f;
+                uint32_t pr[32];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    tmem_ld32(col_s + 32 * h, sr);
+                    tc_wait_ld(sr);
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) {
+                        const int t = 32 * h + c;
+                        float w0 = ex2(fmaf(__uint_as_float(sr[c]) * sc[t], E, sc[kPfBlock + t]) - m_new);
+                        float w1 = ex2(fmaf(__uint_as_float(sr[c + 1]) * sc[t + 1], E, sc[kPfBlock + t + 1]) - m_new);
+                        float e0 = w0 * sc[2 * kPfBlock + t], e1 = w1 * sc[2 * kPfBlock + t + 1];
+                        if (t >= nv) w0 = e0 = 0.0f;         // (also where the scale of a token the row does not see is a NaN)
+                        if (t + 1 >= nv) w1 = e1 = 0.0f;
+                        sum += e0 + e1;
+                        pr[t / 2] = pack2<false>(w0, w1);
+                    }
+                }
+                tmem_st32(col_s, pr);
+                l_run = l_run * alpha + sum;
+                m2 = m_new;
+            }
+            // O += W V of the previous block must be done before O is rescaled.  S of this block was committed behind W V of
+            // block blk-2, so the barrier's phase is blk-1 or later; the last block waits in any case, so that the wait after
+            // the loop cannot meet a barrier that is two phases away
+            const bool rescale = __any_sync(0xFFFFFFFFu, moved);
+            if (blk > 0 && (rescale || blk == n_blocks - 1)) {
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(smem_u32(&bar_o[half]), (uint32_t)((blk - 1) & 1), status))) { alive = false; break; }
+                tc_fence_after();
+                if (rescale) {
+#pragma unroll
+                    for (int part = 0; part < D / 32; part++) {
+                        uint32_t orow[32];
+                        tmem_ld32(base + kPfColO + 32 * part, orow);
+                        tc_wait_ld(orow);
+#pragma unroll
+                        for (int c = 0; c < 32; c++) orow[c] = __float_as_uint(__uint_as_float(orow[c]) * alpha);
+                        tmem_st32(base + kPfColO + 32 * part, orow);
+                    }
+                }
+            }
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(smem_u32(&p_ready[2 * half + buf])); // this row's W (and O) are ready for the tensor pipe
+        }
+        if (alive && !__all_sync(0xFFFFFFFFu, mbar_wait_bounded(smem_u32(&bar_o[half]), (uint32_t)((n_blocks - 1) & 1), status))) alive = false;
+        tc_fence_after();
+
+        const bool poisoned = __any_sync(0xFFFFFFFFu, !alive || __ldcg(status) != 0);   // fail closed, whole warps at a time
+        if (!poisoned) {
+            float* prow = nullptr;
+            float f = l_run == 0.0f ? 0.0f : 1.0f / l_run;   // l counts weights over value scales: at least one term of any size
+            float m_row = m2;
+            if (n_chunks > 1) {                              // (o, m, l) of this chunk, brought to l in [1, 2)
+                prow = partials + (size_t)poff * g.H * (D + 2) +
+                       partial_off(chunk, (tok_first + tid / G) * g.H + kvh * G + tid % G, nq * g.H, D);
+                const uint32_t ex = (__float_as_uint(l_run) >> 23) & 0xFFu;
+                const int k = ex == 0 || ex >= 254 ? 0 : (int)ex - 127;
+                f = pf_pow2i(-k);
+                m_row = l_run == 0.0f ? -1e30f : (m2 + (float)k) * 0.6931471805599453f;
+            }
+#pragma unroll
+            for (int part = 0; part < D / 32; part++) {
+                uint32_t orow[32];
+                tmem_ld32(base + kPfColO + 32 * part, orow);
+                tc_wait_ld(orow);
+                if (!valid) continue;
+                if (n_chunks > 1) {
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2)
+                        *reinterpret_cast<float2*>(prow + 32 * part + c) = make_float2(__uint_as_float(orow[c]) * f, __uint_as_float(orow[c + 1]) * f);
+                } else if (out_dtype == DT_FP32) {
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4)
+                        *reinterpret_cast<float4*>((float*)out + qo_row * D + 32 * part + c) =
+                            make_float4(__uint_as_float(orow[c]) * f, __uint_as_float(orow[c + 1]) * f, __uint_as_float(orow[c + 2]) * f,
+                                        __uint_as_float(orow[c + 3]) * f);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 32; c += 8) {
+                        uint4 w;
+                        w.x = pack2<IO_BF16>(__uint_as_float(orow[c]) * f, __uint_as_float(orow[c + 1]) * f);
+                        w.y = pack2<IO_BF16>(__uint_as_float(orow[c + 2]) * f, __uint_as_float(orow[c + 3]) * f);
+                        w.z = pack2<IO_BF16>(__uint_as_float(orow[c + 4]) * f, __uint_as_float(orow[c + 5]) * f);
+                        w.w = pack2<IO_BF16>(__uint_as_float(orow[c + 6]) * f, __uint_as_float(orow[c + 7]) * f);
+                        *reinterpret_cast<uint4*>((uint16_t*)out + qo_row * D + 32 * part + c) = w;
+                    }
+                }
+            }
+            if (n_chunks > 1 && valid) *reinterpret_cast<float2*>(prow + D) = make_float2(m_row, l_run * f);
+        }
+    }
+
+    // ---- tensor memory goes back on every path ----
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kPfMmaWarp) tmem_dealloc(tmem, kPfTmemCols);
+    if (n_chunks == 1) return;
+    // the CTA that arrives last for the tile merges its chunks (nothing is written while the status word is set)
+    if (tid == 0) {
+        __threadfence();
+        const int tiles = (nq + tpt - 1) / tpt;
+        int* c = counters + cbase + kvh * tiles + tile;
+        const int last = atomicAdd(c, 1) == n_chunks - 1;
+        if (last) *c = 0;
+        *s_flag = last;
+    }
+    __syncthreads();
+    if (*s_flag) {
+        const MergeOut mo{nullptr, out, nullptr, out_dtype, nullptr, status};
+        merge_rows(g, mo, b, kvh, G, 0, n_chunks, partials + (size_t)poff * g.H * (D + 2),
+                   MergeMap{G * tok_cnt, nq * g.H, q_base + tok_first, tok_first, 0});
+    }
+}
+
+template <int D, bool IO_BF16>
+cudaError_t launch_d(const Geometry& g, const LayerPtrs& lp, const PrefillDev& pf, const int32_t* page_table, const void* q, void* out,
+                     int out_dtype, float* partials, int* counters, int* status, cudaStream_t s) {
+    auto kern = prefill_int8_kernel<D, IO_BF16>;
+    static bool attr_done[64] = {};                         // per instantiation and device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !attr_done[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PfCfg<D>::SMEM);
+        if (e != cudaSuccess) return e;
+        if (dev >= 0 && dev < 64) attr_done[dev] = true;
+    }
+    kern<<<pf.n_items, kPfThreads, PfCfg<D>::SMEM, s>>>(g, (const uint8_t*)lp.pool, pf, page_table, (const uint16_t*)q, out, out_dtype, partials,
+                                                        counters, status);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+// Work list, counters and split regions as for launch_prefill_mma, laid out for tiles of kPrefillRowsInt8 rows.
+cudaError_t launch_prefill_int8(const Geometry& g, const LayerPtrs& lp, const PrefillDev& pf, const int32_t* page_table, const void* q,
+                                void* out, int out_dtype, float* partials, int* counters, int* status, cudaStream_t s) {
+    if (pf.n_items <= 0) return cudaSuccess;
+    if (out_dtype != DT_FP32 && out_dtype != g.io_dtype) return cudaErrorInvalidValue;
+    if (g.io_dtype == DT_BF16) return g.D == 128 ? launch_d<128, true>(g, lp, pf, page_table, q, out, out_dtype, partials, counters, status, s)
+                                                 : launch_d<64, true>(g, lp, pf, page_table, q, out, out_dtype, partials, counters, status, s);
+    return g.D == 128 ? launch_d<128, false>(g, lp, pf, page_table, q, out, out_dtype, partials, counters, status, s)
+                      : launch_d<64, false>(g, lp, pf, page_table, q, out, out_dtype, partials, counters, status, s);
+}
+
+}  // namespace tk

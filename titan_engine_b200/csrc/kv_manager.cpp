@@ -292,7 +292,7 @@ void radix_pass(const std::vector<uint32_t>& key, std::vector<int32_t>& idx, std
 int PageManager::plan_step(int n_seqs, const int32_t* seqs, const int32_t* n_new, int num_kv_heads,
                            bool fp8, int chunk_tokens, int target_items, int max_step_tokens,
                            int max_partial_rows, StepPlan* plan, const int32_t* len_cap, int heads_per_kv,
-                           int prefill_rows) {
+                           int prefill_rows, int decode_groups) {
     if (n_seqs < 0 || (n_seqs > 0 && !seqs) || !plan) return ST_INVALID_ARG;
     const int ps = page_size_;
     if (chunk_tokens < 0 || chunk_tokens % ps != 0) return ST_INVALID_ARG;
@@ -471,7 +471,7 @@ int PageManager::plan_step(int n_seqs, const int32_t* seqs, const int32_t* n_new
     plan->pf_small_nq_max = 0; plan->pf_partial_rows = 0; plan->pf_groups = 0;
     const int G = heads_per_kv;
     if (!fp8 && !len_cap && G > 0 && G <= kDecodeTileRows && prefill_rows % G == 0 && plan->nq_min >= 1 &&
-        (int64_t)plan->nq_max * G > (int64_t)kDecodeTileRows * kDecodeMaxTokenGroups) {
+        (int64_t)plan->nq_max * G > (int64_t)kDecodeTileRows * decode_groups) {
         const int tpt = prefill_rows / G;                      // query tokens per tile
         plan->pf_rows = prefill_rows;
         const int max_ct = kPrefillMaxPages * ps;

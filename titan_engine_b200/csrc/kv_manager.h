@@ -78,6 +78,7 @@ struct StepPlan {
 // Geometry of the prefill kernel's work list, shared by the planner and the kernel.
 constexpr int kPrefillRows = 64;           // (token, head) rows per tile of the mma.sync prefill kernel
 constexpr int kPrefillRowsTc = 128;        // ... of the tcgen05 prefill kernel
+constexpr int kPrefillRowsInt8 = 256;     // ... of the kernel over INT8 pools (two halves of 128)
 constexpr int kPrefillMaxPages = 2048;     // pages per item: a split-KV chunk holds at most 32768 tokens
 constexpr int kDecodeTileRows = 16;        // rows of the decode kernel's tile
 constexpr int kDecodeMaxTokenGroups = 8;   // token groups per sequence the decode kernel's multi-token form takes
@@ -135,11 +136,11 @@ public:
     // chunk_tokens == 0 picks a chunk so that about `target_items` items exist.
     // len_cap (optional, 16-bit storage only) limits the attended prefix of each sequence.
     // heads_per_kv > 0 (16-bit storage): also lay out the prefill work lists when a sequence appends
-    // more tokens than the decode kernel's token groups hold, in tiles of prefill_rows (token, head) rows.
+    // more tokens than the decode kernel's decode_groups token groups hold, in tiles of prefill_rows (token, head) rows.
     int plan_step(int n_seqs, const int32_t* seqs, const int32_t* n_new, int num_kv_heads,
                   bool fp8, int chunk_tokens, int target_items, int max_step_tokens,
                   int max_partial_rows, StepPlan* plan, const int32_t* len_cap = nullptr, int heads_per_kv = 0,
-                  int prefill_rows = kPrefillRows);
+                  int prefill_rows = kPrefillRows, int decode_groups = kDecodeMaxTokenGroups);
 
     // Snapshot of the whole bookkeeping state (lengths, page tables, free lists, reference counts, cold ids)
     // as a flat int32 image, and its restore into a manager of the same geometry: a failing churn run can be

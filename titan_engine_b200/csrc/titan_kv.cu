@@ -706,11 +706,14 @@ static int step_begin_impl(tk_kv* h, int32_t n_seqs, const int32_t* seq_ids, con
     std::lock_guard<std::mutex> lock(h->mgr_mu);
     h->have_step = false;
     const int chunk = h->cfg.chunk_tokens;
+    const bool int8 = h->cfg.dtype == TK_INT8;
     const int target = 8 * h->num_sms;       // work items the planner aims for when it picks the chunk itself
     // the tensor-core kernel keeps one page id per lane per warp: chunk <= 16*4*32 tokens
     int st = h->mgr->plan_step(n_seqs, seq_ids, n_new, h->cfg.num_kv_heads, h->cfg.dtype == TK_FP8_E4M3,
                                chunk, target, h->cfg.max_step_tokens, h->max_partial_rows, &h->plan, len_cap,
-                               h->geo.H / h->geo.Hkv, h->prefill_tc ? tk::kPrefillRowsTc : tk::kPrefillRows);
+                               h->geo.H / h->geo.Hkv,
+                              int8 ? tk::kPrefillRowsInt8 : h->prefill_tc ? tk::kPrefillRowsTc : tk::kPrefillRows,
+                              int8 ? 1 : tk::kDecodeMaxTokenGroups);
     if (st != TK_OK) return fail(h, st, "step_begin: %s", tk_status_str(st));
     tk::StepPlan& p = h->plan;
     if (chunk == 0 && p.chunk_tokens > 2048) {
@@ -1091,18 +1094,27 @@ static int decode_multi_impl(tk_kv* h, int32_t layer, const void* q, void* out, 
     if (p.nq_min < 1) return fail(h, TK_INVALID_ARG, "decode_multi: every sequence of the step must append at least one token");
     if (h->cfg.dtype == TK_INT8) {
         if (p.capped) return fail(h, TK_UNSUPPORTED, "decode_multi: not available on a step with capped lengths (INT8 storage)");
-        cudaError_t e;
-        if (h->geo.H / h->geo.Hkv * p.nq_max <= tk::kDecodeTileRows) {       // a few tokens: together through the decode kernel
-            float* ws = multi_workspace(h, (size_t)p.chunk_base[h->dev.n_seqs] * h->geo.H * p.nq_max * (h->geo.Dv + 2), (cudaStream_t)stream);
-            if (!ws) return TK_CUDA_ERROR;
-            e = tk::launch_decode_int8(h->geo, h->layer(layer), &h->maps[layer], h->dev, h->d_table, q, ws, h->d_status, (cudaStream_t)stream,
-                                       tk::MergeOut{h->d_counters, out, nullptr, out_dtype, nullptr, h->d_status},
-                                       tk::FuseAppend{nullptr, nullptr, nullptr}, true, false);
-        } else {
-            e = tk::launch_attn_int8(h->geo, h->layer(layer), h->dev, h->d_table, q, out, out_dtype, h->d_status, (cudaStream_t)stream);
+        // sequences whose (token, head) rows fit one tile of the decode kernel go through it together, the others through the
+        // prefill kernel; the two write disjoint rows of `out`.  Split-KV rows: the decode kernel's first, the prefill regions behind
+        const tk::StepDev& sd = p.pf_built ? h->small_dev : h->dev;
+        const size_t row_floats = (size_t)h->geo.H * (h->geo.Dv + 2);
+        const size_t small_rows = sd.n_items > 0 ? (size_t)p.chunk_base[h->dev.n_seqs] * sd.nq_max : 0;
+        float* ws = multi_workspace(h, (small_rows + (p.pf_built ? (size_t)p.pf_partial_rows : 0)) * row_floats, (cudaStream_t)stream);
+        if (!ws) return TK_CUDA_ERROR;
+        if (sd.n_items > 0) {
+            const cudaError_t e = tk::launch_decode_int8(h->geo, h->layer(layer), &h->maps[layer], sd, h->d_table, q, ws, h->d_status,
+                                                         (cudaStream_t)stream, tk::MergeOut{h->d_counters, out, nullptr, out_dtype, nullptr, h->d_status},
+                                                         tk::FuseAppend{nullptr, nullptr, nullptr}, true, false);
+            h->launches++;
+            if (e != cudaSuccess) return fail(h, TK_CUDA_ERROR, "decode_multi launch: %s", cudaGetErrorString(e));
         }
-        h->launches++;
-        return e == cudaSuccess ? TK_OK : fail(h, TK_CUDA_ERROR, "decode_multi launch: %s", cudaGetErrorString(e));
+        if (p.pf_built && h->pf_dev.n_items > 0) {
+            const cudaError_t e = tk::launch_prefill_int8(h->geo, h->layer(layer), h->pf_dev, h->d_table, q, out, out_dtype, ws + small_rows * row_floats,
+                                                          h->d_pf_counters, h->d_status, (cudaStream_t)stream);
+            h->launches++;
+            if (e != cudaSuccess) return fail(h, TK_CUDA_ERROR, "prefill attention launch: %s", cudaGetErrorString(e));
+        }
+        return TK_OK;
     }
     if (p.pf_built && h->use_mma && !h->mla_mma && tk::prefill_mma_supported(h->geo)) {
         // a prefill-sized step: the sequences with one tile of rows keep the decode kernel, the prefill

@@ -186,15 +186,15 @@ cudaError_t launch_decode_mma_mla_multi(const Geometry& g, const LayerPtrs& lp, 
                                         const void* q, float* partials, int* status, cudaStream_t s, const MergeOut& mo);
 
 // INT8 pools (int8_cache.cuh): the step's rows quantised into their pages; attention of one token per sequence or of a few
-// (int8_decode.cu), and of every token the step appended.
+// (int8_decode.cu), and of every token of a chunk (int8_prefill.cu; pf.items laid out for tiles of kPrefillRowsInt8 rows).
 cudaError_t launch_append_int8(const Geometry& g, const LayerPtrs& lp, const StepDev& st, const int32_t* page_table,
                                const void* k, const void* v, int64_t* slots_out, cudaStream_t s);
 cudaError_t make_int8_tensor_map(const Geometry& g, void* layer_pool, CUtensorMap* out);
 cudaError_t launch_decode_int8(const Geometry& g, const LayerPtrs& lp, const CUtensorMap* map, const StepDev& st,
                                const int32_t* page_table, const void* q, float* partials, int* status, cudaStream_t s,
                                const MergeOut& mo, const FuseAppend& fa, bool multi, bool overlap_prev);
-cudaError_t launch_attn_int8(const Geometry& g, const LayerPtrs& lp, const StepDev& st, const int32_t* page_table, const void* q,
-                             void* out, int out_dtype, const int* status, cudaStream_t s);
+cudaError_t launch_prefill_int8(const Geometry& g, const LayerPtrs& lp, const PrefillDev& pf, const int32_t* page_table, const void* q,
+                                void* out, int out_dtype, float* partials, int* counters, int* status, cudaStream_t s);
 
 // Rows of the cache read back (read_back.cu): n_rows rows from row0 of a page, to token rows out_row, ... of the outputs.
 struct ReadItem {
