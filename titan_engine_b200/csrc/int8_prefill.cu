@@ -11,7 +11,7 @@
 //   4 expander warps codes -> fp16 into the 128-byte-swizzled slabs the MMAs read (2 K and 2 V stages), and the three
 //                    numbers per token the softmax needs: ks log2(e)/sqrt(D), log2 vs, 1/vs (4 stages)
 //   MMA thread       S = Q K^T (M 128, N 64) and O += W V (M 128, N D, W from tensor memory) for both halves
-//   8 softmax warps  thread t owns row t: a speculative pass against the current reference, redone when a score exceeds it
+//   8 softmax warps  32 rows each, as fragments: a speculative pass against the current reference, redone when a score exceeds it
 //                    by 2^8 or the block is cut; only then O is rescaled (prefill_tc.cu describes the scheme)
 // The expansion is what an 8-bit cache costs over a 16-bit one: 2 D values per token, shared here by 256 rows - about an
 // eighth of the issue slots - where two CTAs of 128 rows would each do it.  Tensor memory: per half two S buffers of 64
@@ -46,7 +46,7 @@ struct PfCfg {
     static constexpr int HALF = kPfBlock * 128;
     static constexpr int RAW = 4 * TILE;
     static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + 2 * SLAB, OFF_RAW = OFF_V + 2 * SLAB, OFF_SC = OFF_RAW + kPfRaw * RAW,
-                         OFF_E = OFF_SC + 4 * 3 * kPfBlock * 4, OFF_PAGES = OFF_E + kPfRows * 4, OFF_BARS = OFF_PAGES + kPrefillMaxPages * 4,
+                         OFF_E = OFF_SC + 4 * 3 * kPfBlock * 4, OFF_PAGES = OFF_E + 2 * kPfRows * 4, OFF_BARS = OFF_PAGES + kPrefillMaxPages * 4,
                          SMEM = OFF_BARS + 256 + 1024;
 };
 
@@ -89,7 +89,8 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *s_q = smem, *s_k = smem + C::OFF_K, *s_v = smem + C::OFF_V, *s_raw = smem + C::OFF_RAW;
     float* s_sc = (float*)(smem + C::OFF_SC);               // [4][3][64]: ks log2(e)/sqrt(D), log2 vs, 1/vs
-    float* s_e = (float*)(smem + C::OFF_E);                 // [256] power of two of the row's query
+    float* s_e = (float*)(smem + C::OFF_E);                 // [256] power of two of the row's query; at the end the row's reference
+    float* s_l = s_e + kPfRows;                             // [256] at the end the row's sum
     int32_t* s_pages = (int32_t*)(smem + C::OFF_PAGES);
     uint64_t* bars = (uint64_t*)(smem + C::OFF_BARS);
     uint64_t *rawfull = bars, *rawempty = bars + 3, *kfull = bars + 6, *kempty = bars + 8, *vfull = bars + 10, *vempty = bars + 12,
@@ -115,9 +116,8 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     const int n_chunks = p_last / ct + 1;
     const int32_t* pt_row = page_table + (size_t)seq * g.max_pages_per_seq + t0 / kI8Page;
 
-    // this thread's row (softmax warps): query token tid / G of the tile, head tid % G of the group
+    // this thread's row of the tile at the end (softmax warps): query token tid / G of the tile, head tid % G of the group
     const bool valid = tid < kPfRows && tid / G < tok_cnt;
-    const int lim = base_pos + tok_first + tid / G + 1;     // positions the row sees: [0, lim)
     const size_t qo_row = (size_t)(q_base + tok_first + tid / G) * g.H + (size_t)kvh * G + tid % G;
 
     // ---- prologue ----
@@ -198,60 +198,72 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     const uint32_t tmem = *s_tmem;
 
     bool alive = true;
-    float m2 = -1e30f, l_run = 0.0f;                        // softmax state of this thread's row, m2 in base-2 units
     constexpr float kLazy = 8.0f;
 
     if (warp == kPfMmaWarp) {
-        // ===== MMA warp: one thread feeds the tensor pipe =====
-        if (lane == 0) {
-            constexpr uint32_t kIdescS = instr_desc(false, false, kPfBlock), kIdescO = instr_desc(false, true, D);
-            const uint64_t desc_q = smem_desc(smem_u32(s_q), 16), desc_k = smem_desc(smem_u32(s_k), 16),
-                           desc_v = smem_desc(smem_u32(s_v), C::HALF);
-            auto issue_s = [&](int half, int blk) {
-                const uint64_t dq = desc_q + (uint64_t)((half * C::HALVES * kTcRows * 128) >> 4);
-                const uint64_t dk = desc_k + (uint64_t)(((blk & 1) * C::SLAB) >> 4);
-                const uint32_t d_s = tmem + half * kPfHalfCols + 64u * (blk & 1);
+        // ===== MMA warp: an elected lane feeds the tensor pipe =====
+        constexpr uint32_t kIdescS = instr_desc(false, false, kPfBlock), kIdescO = instr_desc(false, true, D);
+        const uint64_t desc_q = smem_desc(smem_u32(s_q), 16), desc_k = smem_desc(smem_u32(s_k), 16),
+                       desc_v = smem_desc(smem_u32(s_v), C::HALF);
+        auto await = [&](uint64_t* bar, uint32_t parity) {
+            const bool done = __all_sync(0xFFFFFFFFu, mbar_wait_bounded_idle(smem_u32(bar), parity, status));
+            tc_fence_after();
+            return done;
+        };
+        auto issue_s = [&](int half, int blk) {              // S = Q K^T of a half's rows
+            const uint64_t dq = desc_q + (uint64_t)((half * C::HALVES * kTcRows * 128) >> 4);
+            const uint64_t dk = desc_k + (uint64_t)(((blk & 1) * C::SLAB) >> 4);
+            const uint32_t d_s = tmem + half * kPfHalfCols + 64u * (blk & 1);
+            if (elect_one()) {
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ks++)
                     tc_mma_ss(d_s, dq + (uint64_t)(((ks >> 2) * (kTcRows * 128) + (ks & 3) * 32) >> 4),
                               dk + (uint64_t)(((ks >> 2) * C::HALF + (ks & 3) * 32) >> 4), kIdescS, ks > 0);
                 tc_commit(smem_u32(&bar_s[2 * half + (blk & 1)]));
                 if (half == halves - 1) tc_commit(smem_u32(&kempty[blk & 1]));       // (covers the other half's too)
-            };
-            bool ok = true;
-            for (int blk = 0; blk < 2 && blk < n_blocks && ok; blk++) {
-                ok = mbar_wait_bounded_idle(smem_u32(&kfull[blk]), 0u, status);
-                if (!ok) break;
-                tc_fence_after();
-                for (int half = 0; half < halves; half++) issue_s(half, blk);
             }
-            for (int blk = 0; blk < n_blocks && ok; blk++) {
-                const int s = blk & 1;
-                const uint32_t ph = (uint32_t)((blk >> 1) & 1);
-                const uint64_t dv = desc_v + (uint64_t)((s * C::SLAB) >> 4);
-                ok = mbar_wait_bounded_idle(smem_u32(&vfull[s]), ph, status);
-                for (int half = 0; half < halves && ok; half++) {
-                    // every row's W of this block is in tensor memory (and O rescaled): O += W V, then S of the block after next
-                    ok = mbar_wait_bounded_idle(smem_u32(&p_ready[2 * half + s]), ph, status);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t base = tmem + half * kPfHalfCols;
+            __syncwarp();
+        };
+        auto issue_o = [&](int half, int blk) {              // O += W V, 16 tokens per MMA: 8 columns of W, 16 rows of the V slab
+            const uint64_t dv = desc_v + (uint64_t)(((blk & 1) * C::SLAB) >> 4);
+            const uint32_t at = tmem + half * kPfHalfCols;
+            const uint32_t acc = blk > 0 ? 1u : 0u;
+            if (elect_one()) {
 #pragma unroll
-                    for (int ks = 0; ks < 4; ks++)           // 16 tokens per MMA: 8 columns of W, 16 rows of the V slab
-                        tc_mma_ts(base + kPfColO, base + 64u * s + 8 * ks, dv + (uint64_t)((ks * 2048) >> 4), kIdescO, (blk > 0 || ks > 0) ? 1u : 0u);
-                    tc_commit(smem_u32(&bar_o[half]));
-                    if (half == halves - 1) tc_commit(smem_u32(&vempty[s]));
-                    if (blk + 2 < n_blocks) {                // MMAs run in order: S(blk+2) overwrites the columns after W V has read them
-                        if (half == 0) {
-                            ok = mbar_wait_bounded_idle(smem_u32(&kfull[s]), (uint32_t)(((blk + 2) >> 1) & 1), status);
-                            tc_fence_after();
-                        }
-                        if (ok) issue_s(half, blk + 2);
-                    }
-                }
+                for (int ks = 0; ks < 4; ks++)
+                    tc_mma_ts(at + kPfColO, at + 64u * (blk & 1) + 8 * ks, dv + (uint64_t)((ks * 2048) >> 4), kIdescO, ks > 0 ? 1u : acc);
+                tc_commit(smem_u32(&bar_o[half]));
+                if (half == halves - 1) tc_commit(smem_u32(&vempty[blk & 1]));
+            }
+            __syncwarp();
+        };
+        bool ok = true;
+        for (int blk = 0; blk < 2 && blk < n_blocks && ok; blk++) {
+            ok = await(&kfull[blk], 0u);
+            if (!ok) break;
+            issue_s(0, blk);
+            if (halves == 2) issue_s(1, blk);
+        }
+        for (int blk = 0; blk < n_blocks && ok; blk++) {
+            const int s = blk & 1;
+            const uint32_t ph = (uint32_t)((blk >> 1) & 1);
+            // a half's W of this block is in tensor memory (and O rescaled): O += W V, then S of the block after next.  MMAs run
+            // in order: S(blk+2) overwrites the columns after W V has read them
+            ok = await(&vfull[s], ph) && await(&p_ready[s], ph);
+            if (!ok) break;
+            issue_o(0, blk);
+            if (blk + 2 < n_blocks) {
+                ok = await(&kfull[s], ph ^ 1u);
+                if (!ok) break;
+                issue_s(0, blk + 2);
+            }
+            if (halves == 2) {
+                ok = await(&p_ready[2 + s], ph);
+                if (!ok) break;
+                issue_o(1, blk);
+                if (blk + 2 < n_blocks) issue_s(1, blk + 2);
             }
         }
-        __syncwarp();
     } else if (warp == kPfLoadWarp) {
         // ===== loader warp (the first kPfRaw blocks left in the prologue) =====
         int issued = min(kPfRaw, n_blocks);
@@ -312,142 +324,204 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             mbar_arrive(smem_u32(&rawempty[rs]));
         }
     } else if (warp < halves * (kTcRows / 32)) {
-        // ===== softmax warps: thread t owns row t =====
-        const int half = warp >> 2;
+        // ===== softmax warps =====
+        // A warp owns 32 rows (tensor-memory lanes), as fragments: thread t holds, of rows t/4, +8, +16, +24, the columns
+        // 2 (t%4), +1 of every eight.  The numbers of a token are then read once for four rows (with a row per thread each
+        // would be a broadcast of its own: 192 shared-memory wavefronts per warp and block instead of 24).
+        const int half = warp >> 2, quad = lane & 3;
         const uint32_t base = tmem + half * kPfHalfCols + ((uint32_t)((warp & 3) * 32) << 16);    // this warp's 32 lanes
-        const float E = IO_BF16 ? s_e[tid] : 1.0f;
+        float E[4], m2[4], la[4], lb[4];                     // per row: query's power of two, reference (base 2), sums over this thread's columns
+        int lim[4];                                          // positions the row sees
+#pragma unroll
+        for (int rr = 0; rr < 4; rr++) {
+            const int row = warp * 32 + 8 * rr + (lane >> 2);
+            E[rr] = IO_BF16 ? s_e[row] : 1.0f;
+            m2[rr] = -1e30f;
+            la[rr] = lb[rr] = 0.0f;
+            // (rows without a token: zero queries, nothing of theirs is written; unmasked, so that they cost no careful pass)
+            lim[rr] = row / G < tok_cnt ? base_pos + tok_first + row / G + 1 : len;
+        }
+        const bool idle = (warp * 32) / G >= tok_cnt;        // no row of this warp has a token: whatever W holds, nobody reads its O
+        const int lim_min = min(min(lim[0], lim[1]), min(lim[2], lim[3]));
+        bool started = false;
         for (int blk = 0; blk < n_blocks; blk++) {
             const int buf = blk & 1;
             const uint32_t col_s = base + 64u * buf;         // S of this block; its first 32 columns become W
             const int tok_base = t0 + blk * kPfBlock;
-            const float* sc = s_sc + (blk & 3) * 3 * kPfBlock;
+            const float* sc = s_sc + (blk & 3) * 3 * kPfBlock + 2 * quad;
             bool ok = mbar_wait_bounded(smem_u32(&scfull[blk & 3]), (uint32_t)((blk >> 2) & 1), status) &&
                       mbar_wait_bounded(smem_u32(&bar_s[2 * half + buf]), (uint32_t)((blk >> 1) & 1), status);
             if (!__all_sync(0xFFFFFFFFu, ok)) { alive = false; break; }
             tc_fence_after();
-            const int nv = valid ? max(0, min(min(kPfBlock, t1 - tok_base), lim - tok_base)) : 0;
-            const bool full = __all_sync(0xFFFFFFFFu, nv == kPfBlock && m2 > -1e29f);
-            bool moved = false, settled = false;
-            float alpha = 1.0f;
-            if (full) {
-                // One pass against the current reference, 16 columns of S at a time, the next 16 on their way; S stays in tensor
-                // memory until no row of the warp needs it again.
-                uint32_t sr[2][16], pr[32];
-                float l0 = 0.0f, l1 = 0.0f, top = -1e30f;    // top: largest x - m2 of the block
-                const float nm = -m2;
-                tmem_ld16(col_s, sr[0]);
+            bool rescale = false;
+            float alpha[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+            if (!idle) {
+                const bool full = started && tok_base + kPfBlock <= t1 && __all_sync(0xFFFFFFFFu, lim_min >= tok_base + kPfBlock);
+                bool settled = false;
+                uint32_t pr[2][16];                          // W of rows (0, 8) and (16, 24) + t/4 as 16x128b fragments
+                if (full) {
+                    // One pass against the current references, 16 columns at a time, the next 16 on their way; S stays in
+                    // tensor memory until no row of the warp needs it again.
+                    uint32_t sr[2][2][8];
+                    float ta[4], tb[4], top = -1e30f;        // top: largest x - m of the block
 #pragma unroll
-                for (int qt = 0; qt < 4; qt++) {
-                    tc_wait_ld16(sr[qt & 1]);
-                    if (qt < 3) tmem_ld16(col_s + 16 * (qt + 1), sr[(qt + 1) & 1]);
+                    for (int rr = 0; rr < 4; rr++) ta[rr] = tb[rr] = 0.0f;
+                    tmem_ld_frag16(col_s, sr[0][0]);
+                    tmem_ld_frag16(col_s + (16u << 16), sr[0][1]);
 #pragma unroll
-                    for (int c4 = 0; c4 < 4; c4++) {         // tokens 16 qt + 4 c4 .. + 3
-                        const int t = 16 * qt + 4 * c4;
-                        const float4 ks = *reinterpret_cast<const float4*>(sc + t), lv = *reinterpret_cast<const float4*>(sc + kPfBlock + t),
-                                     iv = *reinterpret_cast<const float4*>(sc + 2 * kPfBlock + t);
-                        const float a0 = __uint_as_float(sr[qt & 1][4 * c4]), a1 = __uint_as_float(sr[qt & 1][4 * c4 + 1]),
-                                    a2 = __uint_as_float(sr[qt & 1][4 * c4 + 2]), a3 = __uint_as_float(sr[qt & 1][4 * c4 + 3]);
-                        float x0, x1, x2, x3;
-                        if (IO_BF16) {
-                            mul2v(x0, x1, a0, a1, ks.x, ks.y); mul2v(x2, x3, a2, a3, ks.z, ks.w);
-                            float u0 = lv.x, u1 = lv.y, u2 = lv.z, u3 = lv.w;
-                            add2(u0, u1, nm, nm); add2(u2, u3, nm, nm);
-                            fma2v(x0, x1, x0, x1, E, E, u0, u1); fma2v(x2, x3, x2, x3, E, E, u2, u3);
-                        } else {
-                            fma2v(x0, x1, a0, a1, ks.x, ks.y, lv.x, lv.y); fma2v(x2, x3, a2, a3, ks.z, ks.w, lv.z, lv.w);
-                            add2(x0, x1, nm, nm); add2(x2, x3, nm, nm);
+                    for (int qt = 0; qt < 4; qt++) {
+                        tc_wait_ld_frag16(sr[qt & 1][0], sr[qt & 1][1]);
+                        if (qt < 3) {
+                            tmem_ld_frag16(col_s + 16 * (qt + 1), sr[(qt + 1) & 1][0]);
+                            tmem_ld_frag16(col_s + 16 * (qt + 1) + (16u << 16), sr[(qt + 1) & 1][1]);
                         }
-                        top = fmaxf(fmaxf(top, fmaxf(x0, x1)), fmaxf(x2, x3));
-                        const float w0 = ex2(x0), w1 = ex2(x1), w2 = ex2(x2), w3 = ex2(x3);
-                        fma2v(l0, l1, w0, w1, iv.x, iv.y, l0, l1); fma2v(l0, l1, w2, w3, iv.z, iv.w, l0, l1);
-                        pr[t / 2] = pack2<false>(w0, w1); pr[t / 2 + 1] = pack2<false>(w2, w3);
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {        // tokens 16 qt + 8 k + 2 quad, +1
+                            const int t = 16 * qt + 8 * k;
+                            const float2 ks = *reinterpret_cast<const float2*>(sc + t), lv = *reinterpret_cast<const float2*>(sc + kPfBlock + t),
+                                         iv = *reinterpret_cast<const float2*>(sc + 2 * kPfBlock + t);
+#pragma unroll
+                            for (int rr = 0; rr < 4; rr++) {
+                                const float a0 = __uint_as_float(sr[qt & 1][rr >> 1][4 * k + 2 * (rr & 1)]),
+                                            a1 = __uint_as_float(sr[qt & 1][rr >> 1][4 * k + 2 * (rr & 1) + 1]);
+                                float x0, x1;
+                                if (IO_BF16) {
+                                    float u0 = lv.x, u1 = lv.y;
+                                    mul2v(x0, x1, a0, a1, ks.x, ks.y);
+                                    add2(u0, u1, -m2[rr], -m2[rr]);
+                                    fma2v(x0, x1, x0, x1, E[rr], E[rr], u0, u1);
+                                } else {
+                                    fma2v(x0, x1, a0, a1, ks.x, ks.y, lv.x, lv.y);
+                                    add2(x0, x1, -m2[rr], -m2[rr]);
+                                }
+                                top = fmaxf(top, fmaxf(x0, x1));
+                                const float w0 = ex2(x0), w1 = ex2(x1);
+                                fma2v(ta[rr], tb[rr], w0, w1, iv.x, iv.y, ta[rr], tb[rr]);
+                                pr[rr >> 1][4 * qt + 2 * k + (rr & 1)] = pack2<false>(w0, w1);
+                            }
+                        }
+                    }
+                    if (!__any_sync(0xFFFFFFFFu, top > kLazy)) {
+#pragma unroll
+                        for (int rr = 0; rr < 4; rr++) { la[rr] += ta[rr]; lb[rr] += tb[rr]; }
+                        settled = true;
                     }
                 }
-                moved = top > kLazy;
-                if (!__any_sync(0xFFFFFFFFu, moved)) {
-                    l_run += l0 + l1;
-                    tmem_st32(col_s, pr);                    // W over the columns S was read from
-                    settled = true;
-                }
-            }
-            if (!settled) {
-                // the careful pass: masks, the new reference of every row that moved, and its weights
-                float mx = -INFINITY;
-                uint32_t sr[32];
+                if (!settled) {
+                    // the careful pass: masks, the new reference of every row that moved, and its weights
+                    float mx[4], sum[4], m_new[4];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    tmem_ld32(col_s + 32 * h, sr);
-                    tc_wait_ld(sr);
+                    for (int rr = 0; rr < 4; rr++) { mx[rr] = -INFINITY; sum[rr] = 0.0f; }
+                    for (int ph = 0; ph < 2; ph++) {         // 0: maxima, 1: weights
 #pragma unroll
-                    for (int c = 0; c < 32; c++) {
-                        const int t = 32 * h + c;
-                        const float x = fmaf(__uint_as_float(sr[c]) * sc[t], E, sc[kPfBlock + t]);
-                        if (t < nv) mx = fmaxf(mx, x);
+                        for (int h = 0; h < 2; h++)
+#pragma unroll
+                            for (int gi = 0; gi < 2; gi++) {
+                                uint32_t sf[16];
+                                tmem_ld_frag32(col_s + 32 * h + ((uint32_t)(16 * gi) << 16), sf);
+                                tc_wait_ld16(sf);
+#pragma unroll
+                                for (int k = 0; k < 4; k++) {
+                                    const int t = 32 * h + 8 * k;
+                                    const float2 ks = *reinterpret_cast<const float2*>(sc + t), lv = *reinterpret_cast<const float2*>(sc + kPfBlock + t),
+                                                 iv = *reinterpret_cast<const float2*>(sc + 2 * kPfBlock + t);
+                                    const int p0 = tok_base + t + 2 * quad;
+#pragma unroll
+                                    for (int hh = 0; hh < 2; hh++) {
+                                        const int rr = 2 * gi + hh;
+                                        const bool on0 = p0 < min(lim[rr], t1), on1 = p0 + 1 < min(lim[rr], t1);
+                                        const float x0 = fmaf(__uint_as_float(sf[4 * k + 2 * hh]) * ks.x, E[rr], lv.x),
+                                                    x1 = fmaf(__uint_as_float(sf[4 * k + 2 * hh + 1]) * ks.y, E[rr], lv.y);
+                                        if (ph == 0) {
+                                            if (on0) mx[rr] = fmaxf(mx[rr], x0);
+                                            if (on1) mx[rr] = fmaxf(mx[rr], x1);
+                                        } else {             // (masked: also where the scale of a token the row does not see is a NaN)
+                                            const float w0 = on0 ? ex2(x0 - m_new[rr]) : 0.0f, w1 = on1 ? ex2(x1 - m_new[rr]) : 0.0f;
+                                            if (on0) sum[rr] += w0 * iv.x;
+                                            if (on1) sum[rr] += w1 * iv.y;
+                                            pr[gi][8 * h + 2 * k + hh] = pack2<false>(w0, w1);
+                                        }
+                                    }
+                                }
+                            }
+                        if (ph == 0) {
+#pragma unroll
+                            for (int rr = 0; rr < 4; rr++) { // the four threads of a row agree
+                                mx[rr] = fmaxf(mx[rr], __shfl_xor_sync(0xFFFFFFFFu, mx[rr], 1));
+                                mx[rr] = fmaxf(mx[rr], __shfl_xor_sync(0xFFFFFFFFu, mx[rr], 2));
+                                const bool moved = mx[rr] > m2[rr] + kLazy;
+                                m_new[rr] = moved ? mx[rr] : m2[rr];
+                                alpha[rr] = moved ? ex2(m2[rr] - mx[rr]) : 1.0f;     // a row's first block: 0
+                                rescale = rescale || moved;
+                            }
+                        }
                     }
-                }
-                moved = mx > m2 + kLazy;
-                const float m_new = moved ? mx : m2;
-                alpha = moved ? ex2(m2 - m_new) : 1.0f;      // a row's first block: 0
-                float sum = 0.0f;
-                uint32_t pr[32];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    tmem_ld32(col_s + 32 * h, sr);
-                    tc_wait_ld(sr);
-#pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        const int t = 32 * h + c;
-                        float w0 = ex2(fmaf(__uint_as_float(sr[c]) * sc[t], E, sc[kPfBlock + t]) - m_new);
-                        float w1 = ex2(fmaf(__uint_as_float(sr[c + 1]) * sc[t + 1], E, sc[kPfBlock + t + 1]) - m_new);
-                        float e0 = w0 * sc[2 * kPfBlock + t], e1 = w1 * sc[2 * kPfBlock + t + 1];
-                        if (t >= nv) w0 = e0 = 0.0f;         // (also where the scale of a token the row does not see is a NaN)
-                        if (t + 1 >= nv) w1 = e1 = 0.0f;
-                        sum += e0 + e1;
-                        pr[t / 2] = pack2<false>(w0, w1);
+                    for (int rr = 0; rr < 4; rr++) {
+                        la[rr] = la[rr] * alpha[rr] + sum[rr];
+                        lb[rr] *= alpha[rr];
+                        m2[rr] = m_new[rr];
                     }
+                    started = true;
+                    if (blk == 0 || !full) started = __all_sync(0xFFFFFFFFu, fminf(fminf(m2[0], m2[1]), fminf(m2[2], m2[3])) > -1e29f);
                 }
-                tmem_st32(col_s, pr);
-                l_run = l_run * alpha + sum;
-                m2 = m_new;
+                tmem_st_half32(col_s, pr[0]);                // W over the columns S was read from
+                tmem_st_half32(col_s + (16u << 16), pr[1]);
+                rescale = __any_sync(0xFFFFFFFFu, rescale);
             }
             // O += W V of the previous block must be done before O is rescaled.  S of this block was committed behind W V of
             // block blk-2, so the barrier's phase is blk-1 or later; the last block waits in any case, so that the wait after
             // the loop cannot meet a barrier that is two phases away
-            const bool rescale = __any_sync(0xFFFFFFFFu, moved);
             if (blk > 0 && (rescale || blk == n_blocks - 1)) {
                 if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(smem_u32(&bar_o[half]), (uint32_t)((blk - 1) & 1), status))) { alive = false; break; }
                 tc_fence_after();
                 if (rescale) {
 #pragma unroll
-                    for (int part = 0; part < D / 32; part++) {
-                        uint32_t orow[32];
-                        tmem_ld32(base + kPfColO + 32 * part, orow);
-                        tc_wait_ld(orow);
+                    for (int part = 0; part < D / 32; part++)
 #pragma unroll
-                        for (int c = 0; c < 32; c++) orow[c] = __float_as_uint(__uint_as_float(orow[c]) * alpha);
-                        tmem_st32(base + kPfColO + 32 * part, orow);
-                    }
+                        for (int gi = 0; gi < 2; gi++) {
+                            uint32_t of[16];
+                            const uint32_t at = base + kPfColO + 32 * part + ((uint32_t)(16 * gi) << 16);
+                            tmem_ld_frag32(at, of);
+                            tc_wait_ld16(of);
+#pragma unroll
+                            for (int c = 0; c < 16; c++) of[c] = __float_as_uint(__uint_as_float(of[c]) * alpha[2 * gi + ((c >> 1) & 1)]);
+                            tmem_st_frag32(at, of);
+                        }
                 }
             }
             tc_wait_st();
             tc_fence_before();
-            mbar_arrive(smem_u32(&p_ready[2 * half + buf])); // this row's W (and O) are ready for the tensor pipe
+            mbar_arrive(smem_u32(&p_ready[2 * half + buf])); // these rows' W (and O) are ready for the tensor pipe
         }
         if (alive && !__all_sync(0xFFFFFFFFu, mbar_wait_bounded(smem_u32(&bar_o[half]), (uint32_t)((n_blocks - 1) & 1), status))) alive = false;
         tc_fence_after();
 
         const bool poisoned = __any_sync(0xFFFFFFFFu, !alive || __ldcg(status) != 0);   // fail closed, whole warps at a time
-        if (!poisoned) {
+        if (!poisoned && !idle) {
+            // a row per thread from here on: (m, l) of row t through shared memory (each warp's own entries)
+#pragma unroll
+            for (int rr = 0; rr < 4; rr++) {
+                float l = la[rr] + lb[rr];
+                l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+                l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+                if (quad == 0) {
+                    s_e[warp * 32 + 8 * rr + (lane >> 2)] = m2[rr];
+                    s_l[warp * 32 + 8 * rr + (lane >> 2)] = l;
+                }
+            }
+            __syncwarp();
+            const float m_run = s_e[tid], l_run = s_l[tid];
             float* prow = nullptr;
             float f = l_run == 0.0f ? 0.0f : 1.0f / l_run;   // l counts weights over value scales: at least one term of any size
-            float m_row = m2;
+            float m_row = m_run;
             if (n_chunks > 1) {                              // (o, m, l) of this chunk, brought to l in [1, 2)
                 prow = partials + (size_t)poff * g.H * (D + 2) +
                        partial_off(chunk, (tok_first + tid / G) * g.H + kvh * G + tid % G, nq * g.H, D);
                 const uint32_t ex = (__float_as_uint(l_run) >> 23) & 0xFFu;
                 const int k = ex == 0 || ex >= 254 ? 0 : (int)ex - 127;
                 f = pf_pow2i(-k);
-                m_row = l_run == 0.0f ? -1e30f : (m2 + (float)k) * 0.6931471805599453f;
+                m_row = l_run == 0.0f ? -1e30f : (m_run + (float)k) * 0.6931471805599453f;
             }
 #pragma unroll
             for (int part = 0; part < D / 32; part++) {
