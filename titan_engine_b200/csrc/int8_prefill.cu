@@ -7,7 +7,7 @@
 //
 // One CTA per SM = one tile of 256 (token, head) rows of a (sequence, kv head) x a range of the context, as two halves of
 // 128 rows (the lanes of tensor memory) that take turns on the tensor pipe.  Per block of 64 tokens (4 pages):
-//   loader warp      one bulk copy per page: the page's tile - codes and scales - is contiguous; 3 stages
+//   loader warp      one bulk copy per page: the page's tile - codes and scales - is contiguous; 4 stages
 //   4 expander warps codes -> fp16 into the 128-byte-swizzled slabs the MMAs read (2 K and 2 V stages), and the three
 //                    numbers per token the softmax needs: ks log2(e)/sqrt(D), log2 vs, 1/vs (4 stages)
 //   MMA thread       S = Q K^T (M 128, N 64) and O += W V (M 128, N D, W from tensor memory) for both halves
@@ -30,7 +30,7 @@ namespace {
 
 constexpr int kPfRows = kPrefillRowsInt8;       // 256: two halves of kTcRows
 constexpr int kPfBlock = 64;                    // context tokens per block (4 pages)
-constexpr int kPfRaw = 3;                       // stages of raw tiles
+constexpr int kPfRaw = 4;                       // stages of raw tiles: K is expanded two blocks ahead of V
 constexpr int kPfSoftWarps = kPfRows / 32, kPfExpWarps = 4;
 constexpr int kPfMmaWarp = kPfSoftWarps + kPfExpWarps, kPfLoadWarp = kPfMmaWarp + 1;
 constexpr int kPfThreads = (kPfLoadWarp + 1) * 32;
@@ -93,9 +93,9 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     float* s_l = s_e + kPfRows;                             // [256] at the end the row's sum
     int32_t* s_pages = (int32_t*)(smem + C::OFF_PAGES);
     uint64_t* bars = (uint64_t*)(smem + C::OFF_BARS);
-    uint64_t *rawfull = bars, *rawempty = bars + 3, *kfull = bars + 6, *kempty = bars + 8, *vfull = bars + 10, *vempty = bars + 12,
-             *scfull = bars + 14, *bar_s = bars + 18 /* [half][2] */, *p_ready = bars + 22 /* [half][2] */, *bar_o = bars + 26 /* [half] */;
-    uint32_t* s_tmem = (uint32_t*)(bars + 28);
+    uint64_t *rawfull = bars, *rawempty = bars + 4, *kfull = bars + 8, *kempty = bars + 10, *vfull = bars + 12, *vempty = bars + 14,
+             *scfull = bars + 16, *bar_s = bars + 20 /* [half][2] */, *p_ready = bars + 24 /* [half][2] */, *bar_o = bars + 28 /* [half] */;
+    uint32_t* s_tmem = (uint32_t*)(bars + 30);
     int* s_flag = (int*)(s_tmem + 1);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -298,12 +298,13 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };
-        for (int blk = 0; blk < n_blocks; blk++) {
+        auto expand_k = [&](int blk) {
             const int s = blk & 1, rs = blk % kPfRaw;
             const uint8_t* raw = s_raw + rs * C::RAW;
-            if (!mbar_wait_bounded(smem_u32(&rawfull[rs]), (uint32_t)((blk / kPfRaw) & 1), status)) break;
-            if (blk >= 2 && !mbar_wait_bounded(smem_u32(&kempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) break;
+            if (!mbar_wait_bounded(smem_u32(&rawfull[rs]), (uint32_t)((blk / kPfRaw) & 1), status)) return false;
+            if (blk >= 2 && !mbar_wait_bounded(smem_u32(&kempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
             expand(raw, 0, s_k + s * C::SLAB);
+            mbar_arrive(smem_u32(&kfull[s]));
             if (et < kPfBlock) {
                 // (the numbers of block blk - 4 are out of use: S of block blk - 2, whose slab was just handed back, was
                 // issued after every row's W of block blk - 4)
@@ -317,12 +318,19 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                 o[2 * kPfBlock] = in ? __fdividef(1.0f, vs) : 0.0f;
                 mbar_arrive(smem_u32(&scfull[blk & 3]));
             }
-            mbar_arrive(smem_u32(&kfull[s]));
-            if (blk >= 2 && !mbar_wait_bounded(smem_u32(&vempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) break;
-            expand(raw, 1, s_v + s * C::SLAB);
+            return true;
+        };
+        auto expand_v = [&](int blk) {
+            const int s = blk & 1, rs = blk % kPfRaw;
+            if (blk >= 2 && !mbar_wait_bounded(smem_u32(&vempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
+            expand(s_raw + rs * C::RAW, 1, s_v + s * C::SLAB);
             mbar_arrive(smem_u32(&vfull[s]));
             mbar_arrive(smem_u32(&rawempty[rs]));
-        }
+            return true;
+        };
+        // W V of block i - 2 and S of block i end together: they hand back the slabs of V(i) and K(i + 2), needed in this order
+        bool ok = expand_k(0) && (n_blocks < 2 || expand_k(1));
+        for (int blk = 0; blk < n_blocks && ok; blk++) ok = expand_v(blk) && (blk + 2 >= n_blocks || expand_k(blk + 2));
     } else if (warp < halves * (kTcRows / 32)) {
         // ===== softmax warps =====
         // A warp owns 32 rows (tensor-memory lanes), as fragments: thread t holds, of rows t/4, +8, +16, +24, the columns
