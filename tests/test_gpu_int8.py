@@ -380,6 +380,73 @@ def test_chunk_value_scales(vscale):
     p.check_chunk(p.c.append_decode_multi(0, k, v, q), [s], [150], q)
 
 
+def test_chunk_large_queries():
+    """bf16 queries far outside fp16's range next to ordinary ones, tiny ones and zeros in one tile."""
+    p = Pair(8, 2, 128, "bf16")
+    s = p.alloc()
+    p.grow([s], [200])
+    k, v = p.begin([s], [90])
+    q = p.rows(90, 8)
+    q[3, 1::2] *= 1e-30
+    q[4] = 0
+    q[40:44, 0] *= 2.0 ** 60
+    got = p.c.append_decode_multi(0, k, v, q).float().cpu().numpy()
+    want, bound = attention(q.float().cpu().numpy(), p.k[s], p.v[s], np.arange(200, 290) + 1, "bf16")
+    plain = np.ones((90, 8), bool)
+    plain[40:44, 0] = False
+    check(got[plain], want[plain], bound[plain])
+    for t in range(40, 44):                                 # with such a query one key takes all: its value row
+        best = np.einsum("d,ld->l", q[t, 0].double().cpu().numpy(), p.k[s][:201 + t, 0].astype(np.float64)).argmax()
+        np.testing.assert_allclose(got[t, 0], p.v[s][best, 0], rtol=2 ** -8)
+
+
+@pytest.mark.parametrize("H,Hkv,D,io", [(8, 2, 128, "bf16"), (8, 1, 64, "fp16"), (16, 1, 128, "fp16")])
+def test_chunk_rows_around_the_tile_halves(H, Hkv, D, io):
+    """(token, head) rows just below, at and above 128 and 256 of them, over contexts that end inside a page and a block."""
+    G = H // Hkv
+    new = [n for r in (128, 256) for n in (r // G - 1, r // G, r // G + 1)]
+    ctx = [0, 63, 64, 65, 15, 449]
+    p = Pair(H, Hkv, D, io, seqs=6, pages=512)
+    seqs = [p.alloc() for _ in new]
+    p.grow(seqs, ctx)
+    k, v = p.begin(seqs, new)
+    q = p.rows(sum(new), H, 1.5)
+    p.check_chunk(p.c.append_decode_multi(0, k, v, q), seqs, new, q)
+
+
+def test_chunk_split_over_a_long_context():
+    """Few rows and a long context: the chunk's tile is split along the context and the parts merge."""
+    p = Pair(8, 2, 128, "bf16", pages=1400, mpps=700)
+    a, b = p.alloc(), p.alloc()
+    p.grow([a, b], [9001, 5000], 1.0)
+    new = [30, 7]
+    for vscale in (1.0, 2.0 ** 30):
+        k, v = p.begin([a, b], new, vscale)
+        q = p.rows(37, 8, 2.0)
+        p.check_chunk(p.c.append_decode_multi(0, k, v, q), [a, b], new, q)
+        items, ct, _ = p.c.step_prefill_plan()
+        assert len(items) and ct[0] < 9000                  # really split
+
+
+def test_nan_rows_poison_only_the_queries_that_see_them():
+    p = Pair(4, 1, 64, "bf16")
+    a, b = p.alloc(), p.alloc()
+    p.grow([a, b], [30, 30])
+    k, v = p.begin([a, b], [100, 3])
+    k[60, 0, 5] = float("nan")
+    v[80, 0, 1] = float("nan")
+    q = p.rows(103, 4)
+    got = p.c.append_decode_multi(0, k, v, q)
+    assert torch.isnan(got[60:100]).all() and torch.isfinite(got[:60]).all() and torch.isfinite(got[100:]).all()
+    p.k[a][90], p.v[a][110] = 0, 0
+    n = 60
+    want, bound = attention(q[:n].float().cpu().numpy(), p.k[a][:90], p.v[a][:90], np.arange(30, 30 + n) + 1, "bf16")
+    check(got[:n].float().cpu().numpy(), want, bound)
+    p.c.step_begin([b, a])
+    out = p.c.decode(0, q[:2].contiguous())
+    assert torch.isfinite(out[0]).all() and torch.isnan(out[1]).all()
+
+
 def test_chunk_refusals():
     from titan_engine_b200 import KvError
     from titan_engine_b200 import _lib as L

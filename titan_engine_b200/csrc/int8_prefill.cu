@@ -24,6 +24,8 @@
 #include "tk_mma.cuh"
 #include "tk_tcgen05.cuh"
 
+#include <type_traits>
+
 namespace tk {
 
 namespace {
@@ -33,7 +35,7 @@ constexpr int kPfBlock = 64;                    // context tokens per block (4 p
 constexpr int kPfRaw = 4;                       // stages of raw tiles: K is expanded two blocks ahead of V
 constexpr int kPfSoftWarps = kPfRows / 32, kPfExpWarps = 4;
 constexpr int kPfMmaWarp = kPfSoftWarps + kPfExpWarps, kPfLoadWarp = kPfMmaWarp + 1;
-constexpr int kPfThreads = (kPfLoadWarp + 1) * 32;
+constexpr int kPfThreads = 512;                  // 4 warpgroups: softmax, softmax, expanders, (MMA, loader, two idle warps)
 constexpr int kPfExpThreads = kPfExpWarps * 32;
 constexpr uint32_t kPfTmemCols = 512, kPfHalfCols = 256, kPfColO = 128;   // half h: S at 256h and 256h + 64, O at 256h + 128
 
@@ -47,7 +49,7 @@ struct PfCfg {
     static constexpr int RAW = 4 * TILE;
     static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + 2 * SLAB, OFF_RAW = OFF_V + 2 * SLAB, OFF_SC = OFF_RAW + kPfRaw * RAW,
                          OFF_E = OFF_SC + 4 * 3 * kPfBlock * 4, OFF_PAGES = OFF_E + 2 * kPfRows * 4, OFF_BARS = OFF_PAGES + kPrefillMaxPages * 4,
-                         SMEM = OFF_BARS + 256 + 1024;
+                         SMEM = OFF_BARS + 512 + 1024;
 };
 
 __device__ __forceinline__ uint32_t pf_expand(uint32_t w, uint32_t sel) {      // two codes as fp16, exact: 1024 + u, minus 1152
@@ -57,13 +59,37 @@ __device__ __forceinline__ uint32_t pf_expand(uint32_t w, uint32_t sel) {      /
     const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&bias));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ void fma2v(float& r0, float& r1, float a0, float a1, float b0, float b1, float c0, float c1) {
-    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
-        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}" : "=f"(r0), "=f"(r1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+// two FP32 values in one 64-bit register
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack_x2(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
 }
-__device__ __forceinline__ void mul2v(float& r0, float& r1, float a0, float a1, float b0, float b1) {
-    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
-        "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}" : "=f"(r0), "=f"(r1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+__device__ __forceinline__ f32x2 pack_x2(uint32_t lo, uint32_t hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_x2(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma_x2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul_x2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 add_x2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 __device__ __forceinline__ float pf_lg2(float x) {
     float y;
@@ -97,6 +123,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
              *scfull = bars + 16, *bar_s = bars + 20 /* [half][2] */, *p_ready = bars + 24 /* [half][2] */, *bar_o = bars + 28 /* [half] */;
     uint32_t* s_tmem = (uint32_t*)(bars + 30);
     int* s_flag = (int*)(s_tmem + 1);
+    uint32_t* s_wmax = (uint32_t*)(bars + 32);              // [warps] prologue: largest query magnitude
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = g.H / g.Hkv;
@@ -167,16 +194,40 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         for (int blk = 0; blk < kPfRaw && blk < n_blocks; blk++) load_block(blk, pt_row);
     }
     for (int i = tid; i < n_pages; i += kPfThreads) s_pages[i] = pt_row[i];
+    // bf16 queries as fp16: the largest element of the tile becomes 2^14 .. 2^15, one power of two 2^e0 for all rows.  Elements
+    // below fp16's normal range are off by at most 2^-40 of that largest element, a score by 2^-40 of what it could make of
+    // the key: nothing, unless such scores pass 2^28.  Where a query reaches 2^15 (`wide`) every row therefore has a power of
+    // its own, and its scores are multiplied by it.
+    int e0 = 0;
+    bool wide = false;
+    uint32_t row_max[LPR];                                  // bf16 pattern of each of this thread's vectors' rows' largest magnitude
+    if (IO_BF16) {
+        uint32_t m_all = 0;
+        if (tid < kPfRows) {
+#pragma unroll
+            for (int i = 0; i < LPR; i++) {
+                uint32_t m = i8_absmax8(qv[i]);
+#pragma unroll
+                for (int off = LPR / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
+                row_max[i] = m;
+                m_all = max(m_all, m);
+            }
+        }
+        m_all = __reduce_max_sync(0xFFFFFFFFu, m_all);
+        if (lane == 0) s_wmax[warp] = m_all;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPfSoftWarps; i++) m_all = max(m_all, s_wmax[i]);
+        e0 = m_all ? max((int)(m_all >> 7) - 127 - 14, -100) : 0;
+        wide = e0 > 0;                                      // some |q| >= 2^15
+    }
     if (tid < kPfRows) {
 #pragma unroll
         for (int i = 0; i < LPR; i++) {
             const int r = (i * kPfRows + tid) / LPR, c = tid % LPR;
             uint4 x = qv[i];
             if (IO_BF16) {
-                uint32_t m = i8_absmax8(x);
-#pragma unroll
-                for (int off = LPR / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
-                const int e = m ? max((int)(m >> 7) - 127 - 14, -100) : 0;      // the largest element becomes 2^14 .. 2^15
+                const int e = wide ? (row_max[i] ? max((int)(row_max[i] >> 7) - 127 - 14, -100) : 0) : e0;
                 const float down = pf_pow2i(-e);
                 uint32_t* w = &x.x;
 #pragma unroll
@@ -200,6 +251,15 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     bool alive = true;
     constexpr float kLazy = 8.0f;
 
+    // Registers: 512 threads x 128 at launch; 160 for the two softmax warpgroups, 88 for the others (2 x 128 x (160 + 88) = 63488 of
+    // the 65536 the block was launched with).
+    // A role other than softmax ends at the barrier that all threads of the CTA meet on, whatever became of it.
+    auto leave = [&]() {
+        tc_fence_before();
+        asm volatile("bar.sync 1, %0;" ::"n"(kPfThreads) : "memory");
+    };
+    if (warp >= kPfMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == kPfMmaWarp) {
         // ===== MMA warp: an elected lane feeds the tensor pipe =====
         constexpr uint32_t kIdescS = instr_desc(false, false, kPfBlock), kIdescO = instr_desc(false, true, D);
@@ -275,34 +335,40 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         // no copy of this CTA may be in flight when it returns, whatever became of the other roles
         for (int blk = max(0, issued - kPfRaw); blk < issued; blk++)
             (void)__all_sync(0xFFFFFFFFu, mbar_wait_bounded_idle(smem_u32(&rawfull[blk % kPfRaw]), (uint32_t)((blk / kPfRaw) & 1), status));
-    } else if (warp >= kPfSoftWarps) {
+    }
+    leave();
+    if (warp == kPfMmaWarp) tmem_dealloc(tmem, kPfTmemCols); // tensor memory goes back on every path
+    return;
+    }
+    if (warp >= kPfSoftWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         // ===== expander warps: codes -> fp16 slabs =====
         const int et = tid - kPfSoftWarps * 32;
-        const float sc2 = kLog2e / sqrtf((float)D);
-        constexpr int CPR = D / 16;                         // 16-code chunks per row
+        const float sc2E = kLog2e / sqrtf((float)D) * (IO_BF16 && !wide ? pf_pow2i(e0) : 1.0f);
+        // A thread expands the same 16 columns of every 16th (D = 64: 32nd) row: all its addresses are constants away from these.
+        constexpr int CPR = D / 16, ROWS = kPfExpThreads / CPR;     // 16-code chunks per row, rows per pass
+        const int er = et / CPR, ec = et % CPR;
+        const uint32_t from = (uint32_t)((er / kI8Page) * C::TILE + (er % kI8Page) * D + ec * 16);
+        // 16 codes = two 16-byte chunks of the fp16 row.  At D = 128 a quarter warp stores one row: lanes of the second dim half
+        // store their chunks in the other order, or both halves would meet in the same banks.
+        const bool swap = D == 128 && ec >= 4;
+        const uint32_t to = (uint32_t)((ec >> 2) * C::HALF + er * 128);
+        const uint32_t to_lo = to + (((2 * (ec & 3) + (swap ? 1 : 0)) ^ (er & 7)) << 4), to_hi = to_lo ^ 16u;
         auto expand = [&](const uint8_t* raw, int kv, uint8_t* slab) {
 #pragma unroll
-            for (int i = 0; i < kPfBlock * CPR / kPfExpThreads; i++) {
-                const int u = i * kPfExpThreads + et, r = u / CPR, c = u % CPR;
-                uint4 w = *reinterpret_cast<const uint4*>(raw + (r / kI8Page) * C::TILE + i8_row_off(D, kv, r % kI8Page) + c * 16);
-                // 16 codes = two 16-byte chunks 2c, 2c+1 of the fp16 row.  At D = 128 a quarter warp stores one row: lanes of the
-                // second dim half store their chunks in the other order, or both halves would meet in the same banks.
-                const int swap = D == 128 ? c >> 2 : 0;
-                if (swap) w = make_uint4(w.z, w.w, w.x, w.y);
-                const uint4 lo = make_uint4(pf_expand(w.x, 0x4140), pf_expand(w.x, 0x4342), pf_expand(w.y, 0x4140), pf_expand(w.y, 0x4342));
-                const uint4 hi = make_uint4(pf_expand(w.z, 0x4140), pf_expand(w.z, 0x4342), pf_expand(w.w, 0x4140), pf_expand(w.w, 0x4342));
-                uint8_t* row = slab + (c >> 2) * C::HALF + r * 128;
-                const int c2 = 2 * (c & 3);
-                *reinterpret_cast<uint4*>(row + (((c2 + swap) ^ (r & 7)) << 4)) = lo;
-                *reinterpret_cast<uint4*>(row + (((c2 + 1 - swap) ^ (r & 7)) << 4)) = hi;
+            for (int i = 0; i < kPfBlock / ROWS; i++) {
+                const uint4 w = *reinterpret_cast<const uint4*>(raw + from + i * (ROWS / kI8Page) * C::TILE + i8_row_off(D, kv, 0));
+                const uint32_t a0 = swap ? w.z : w.x, a1 = swap ? w.w : w.y, b0 = swap ? w.x : w.z, b1 = swap ? w.y : w.w;
+                *reinterpret_cast<uint4*>(slab + to_lo + i * ROWS * 128) = make_uint4(pf_expand(a0, 0x4140), pf_expand(a0, 0x4342), pf_expand(a1, 0x4140), pf_expand(a1, 0x4342));
+                *reinterpret_cast<uint4*>(slab + to_hi + i * ROWS * 128) = make_uint4(pf_expand(b0, 0x4140), pf_expand(b0, 0x4342), pf_expand(b1, 0x4140), pf_expand(b1, 0x4342));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };
         auto expand_k = [&](int blk) {
             const int s = blk & 1, rs = blk % kPfRaw;
             const uint8_t* raw = s_raw + rs * C::RAW;
-            if (!mbar_wait_bounded(smem_u32(&rawfull[rs]), (uint32_t)((blk / kPfRaw) & 1), status)) return false;
-            if (blk >= 2 && !mbar_wait_bounded(smem_u32(&kempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
+            if (!mbar_wait_bounded_idle(smem_u32(&rawfull[rs]), (uint32_t)((blk / kPfRaw) & 1), status)) return false;
+            if (blk >= 2 && !mbar_wait_bounded_idle(smem_u32(&kempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
             expand(raw, 0, s_k + s * C::SLAB);
             mbar_arrive(smem_u32(&kfull[s]));
             if (et < kPfBlock) {
@@ -313,7 +379,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                 const float ks = *reinterpret_cast<const float*>(t + i8_scale_off(D, 0, et % kI8Page));
                 const float vs = *reinterpret_cast<const float*>(t + i8_scale_off(D, 1, et % kI8Page));
                 float* o = s_sc + (blk & 3) * 3 * kPfBlock + et;
-                o[0] = in ? ks * sc2 : 0.0f;
+                o[0] = in ? ks * sc2E : 0.0f;
                 o[kPfBlock] = in ? pf_lg2(vs) : 0.0f;
                 o[2 * kPfBlock] = in ? __fdividef(1.0f, vs) : 0.0f;
                 mbar_arrive(smem_u32(&scfull[blk & 3]));
@@ -322,7 +388,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         };
         auto expand_v = [&](int blk) {
             const int s = blk & 1, rs = blk % kPfRaw;
-            if (blk >= 2 && !mbar_wait_bounded(smem_u32(&vempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
+            if (blk >= 2 && !mbar_wait_bounded_idle(smem_u32(&vempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
             expand(s_raw + rs * C::RAW, 1, s_v + s * C::SLAB);
             mbar_arrive(smem_u32(&vfull[s]));
             mbar_arrive(smem_u32(&rawempty[rs]));
@@ -331,21 +397,26 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         // W V of block i - 2 and S of block i end together: they hand back the slabs of V(i) and K(i + 2), needed in this order
         bool ok = expand_k(0) && (n_blocks < 2 || expand_k(1));
         for (int blk = 0; blk < n_blocks && ok; blk++) ok = expand_v(blk) && (blk + 2 >= n_blocks || expand_k(blk + 2));
-    } else if (warp < halves * (kTcRows / 32)) {
+        leave();
+        return;
+    }
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    if (warp < halves * (kTcRows / 32)) {
         // ===== softmax warps =====
         // A warp owns 32 rows (tensor-memory lanes), as fragments: thread t holds, of rows t/4, +8, +16, +24, the columns
         // 2 (t%4), +1 of every eight.  The numbers of a token are then read once for four rows (with a row per thread each
         // would be a broadcast of its own: 192 shared-memory wavefronts per warp and block instead of 24).
         const int half = warp >> 2, quad = lane & 3;
         const uint32_t base = tmem + half * kPfHalfCols + ((uint32_t)((warp & 3) * 32) << 16);    // this warp's 32 lanes
-        float E[4], m2[4], la[4], lb[4];                     // per row: query's power of two, reference (base 2), sums over this thread's columns
+        float E[4], m2[4];                                   // per row: query's power of two, reference (base 2)
+        f32x2 l2[4];                                         // ... sums over this thread's even and odd columns
         int lim[4];                                          // positions the row sees
 #pragma unroll
         for (int rr = 0; rr < 4; rr++) {
             const int row = warp * 32 + 8 * rr + (lane >> 2);
-            E[rr] = IO_BF16 ? s_e[row] : 1.0f;
+            E[rr] = IO_BF16 && wide ? s_e[row] : 1.0f;
             m2[rr] = -1e30f;
-            la[rr] = lb[rr] = 0.0f;
+            l2[rr] = 0ull;
             // (rows without a token: zero queries, nothing of theirs is written; unmasked, so that they cost no careful pass)
             lim[rr] = row / G < tok_cnt ? base_pos + tok_first + row / G + 1 : len;
         }
@@ -364,16 +435,23 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             bool rescale = false;
             float alpha[4] = {1.0f, 1.0f, 1.0f, 1.0f};
             if (!idle) {
-                const bool full = started && tok_base + kPfBlock <= t1 && __all_sync(0xFFFFFFFFu, lim_min >= tok_base + kPfBlock);
-                bool settled = false;
-                uint32_t pr[2][16];                          // W of rows (0, 8) and (16, 24) + t/4 as 16x128b fragments
-                if (full) {
-                    // One pass against the current references, 16 columns at a time, the next 16 on their way; S stays in
-                    // tensor memory until no row of the warp needs it again.
-                    uint32_t sr[2][2][8];
-                    float ta[4], tb[4], top = -1e30f;        // top: largest x - m of the block
+                const int end = min(t1, tok_base + kPfBlock);
+                // whole: every row of the warp sees all of the block and no power of two is due
+                const bool whole = !(IO_BF16 && wide) && end - tok_base == kPfBlock && __all_sync(0xFFFFFFFFu, lim_min >= tok_base + kPfBlock);
+                int nv[4];                                   // of a row: tokens of the block it sees, from this thread's first column on
 #pragma unroll
-                    for (int rr = 0; rr < 4; rr++) ta[rr] = tb[rr] = 0.0f;
+                for (int rr = 0; rr < 4; rr++) nv[rr] = min(lim[rr], end) - tok_base - 2 * quad;
+                uint32_t pr[2][16];                          // W of rows (0, 8) and (16, 24) + t/4 as 16x128b fragments
+                f32x2 tl[4];                                 // the block's share of the sums
+                // The weights of the block against the current references, 16 columns of S at a time, the next 16 on their way; S
+                // stays in tensor memory.  -> whether a score exceeds its row's reference by more than 2^kLazy.
+                auto weigh = [&](auto masked) -> bool {
+                    constexpr bool M = decltype(masked)::value;
+                    f32x2 nm[4];
+                    float top = -1e30f;
+#pragma unroll
+                    for (int rr = 0; rr < 4; rr++) { tl[rr] = 0ull; nm[rr] = pack_x2(-m2[rr], -m2[rr]); }
+                    uint32_t sr[2][2][8];
                     tmem_ld_frag16(col_s, sr[0][0]);
                     tmem_ld_frag16(col_s + (16u << 16), sr[0][1]);
 #pragma unroll
@@ -386,96 +464,79 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
 #pragma unroll
                         for (int k = 0; k < 2; k++) {        // tokens 16 qt + 8 k + 2 quad, +1
                             const int t = 16 * qt + 8 * k;
-                            const float2 ks = *reinterpret_cast<const float2*>(sc + t), lv = *reinterpret_cast<const float2*>(sc + kPfBlock + t),
-                                         iv = *reinterpret_cast<const float2*>(sc + 2 * kPfBlock + t);
+                            const f32x2 ks = *reinterpret_cast<const f32x2*>(sc + t), lv = *reinterpret_cast<const f32x2*>(sc + kPfBlock + t),
+                                        iv = *reinterpret_cast<const f32x2*>(sc + 2 * kPfBlock + t);
 #pragma unroll
                             for (int rr = 0; rr < 4; rr++) {
-                                const float a0 = __uint_as_float(sr[qt & 1][rr >> 1][4 * k + 2 * (rr & 1)]),
-                                            a1 = __uint_as_float(sr[qt & 1][rr >> 1][4 * k + 2 * (rr & 1) + 1]);
-                                float x0, x1;
-                                if (IO_BF16) {
-                                    float u0 = lv.x, u1 = lv.y;
-                                    mul2v(x0, x1, a0, a1, ks.x, ks.y);
-                                    add2(u0, u1, -m2[rr], -m2[rr]);
-                                    fma2v(x0, x1, x0, x1, E[rr], E[rr], u0, u1);
-                                } else {
-                                    fma2v(x0, x1, a0, a1, ks.x, ks.y, lv.x, lv.y);
-                                    add2(x0, x1, -m2[rr], -m2[rr]);
+                                const f32x2 a = pack_x2(sr[qt & 1][rr >> 1][4 * k + 2 * (rr & 1)], sr[qt & 1][rr >> 1][4 * k + 2 * (rr & 1) + 1]);
+                                const f32x2 u = add_x2(lv, nm[rr]);
+                                float2 x = unpack_x2(M ? fma_x2(mul_x2(a, ks), pack_x2(E[rr], E[rr]), u) : fma_x2(a, ks, u));
+                                if (M) {                     // (also where the scale of a token the row does not see is a NaN)
+                                    x.x = t < nv[rr] ? x.x : -INFINITY;
+                                    x.y = t + 1 < nv[rr] ? x.y : -INFINITY;
                                 }
-                                top = fmaxf(top, fmaxf(x0, x1));
-                                const float w0 = ex2(x0), w1 = ex2(x1);
-                                fma2v(ta[rr], tb[rr], w0, w1, iv.x, iv.y, ta[rr], tb[rr]);
+                                top = fmaxf(top, fmaxf(x.x, x.y));
+                                const float w0 = ex2(x.x), w1 = ex2(x.y);
+                                if (M) {
+                                    const float2 ivf = unpack_x2(iv);
+                                    tl[rr] = add_x2(tl[rr], pack_x2(t < nv[rr] ? w0 * ivf.x : 0.0f, t + 1 < nv[rr] ? w1 * ivf.y : 0.0f));
+                                } else {
+                                    tl[rr] = fma_x2(pack_x2(w0, w1), iv, tl[rr]);
+                                }
                                 pr[rr >> 1][4 * qt + 2 * k + (rr & 1)] = pack2<false>(w0, w1);
                             }
                         }
                     }
-                    if (!__any_sync(0xFFFFFFFFu, top > kLazy)) {
+                    return __any_sync(0xFFFFFFFFu, top > kLazy);
+                };
+                // speculating that the references stay; a row without one (its first block, or none of it seen so far) has to look first
+                bool look = !started;
+                if (!look) look = whole ? weigh(std::false_type{}) : weigh(std::true_type{});
+                if (look) {                                  // new references for the rows that need one, then the weights
+                    float mx[4];
 #pragma unroll
-                        for (int rr = 0; rr < 4; rr++) { la[rr] += ta[rr]; lb[rr] += tb[rr]; }
-                        settled = true;
-                    }
-                }
-                if (!settled) {
-                    // the careful pass: masks, the new reference of every row that moved, and its weights
-                    float mx[4], sum[4], m_new[4];
+                    for (int rr = 0; rr < 4; rr++) mx[rr] = -INFINITY;
 #pragma unroll
-                    for (int rr = 0; rr < 4; rr++) { mx[rr] = -INFINITY; sum[rr] = 0.0f; }
-                    for (int ph = 0; ph < 2; ph++) {         // 0: maxima, 1: weights
+                    for (int h = 0; h < 2; h++)
 #pragma unroll
-                        for (int h = 0; h < 2; h++)
+                        for (int gi = 0; gi < 2; gi++) {
+                            uint32_t sf[16];
+                            tmem_ld_frag32(col_s + 32 * h + ((uint32_t)(16 * gi) << 16), sf);
+                            tc_wait_ld16(sf);
 #pragma unroll
-                            for (int gi = 0; gi < 2; gi++) {
-                                uint32_t sf[16];
-                                tmem_ld_frag32(col_s + 32 * h + ((uint32_t)(16 * gi) << 16), sf);
-                                tc_wait_ld16(sf);
+                            for (int k = 0; k < 4; k++) {
+                                const int t = 32 * h + 8 * k;
+                                const f32x2 ks = *reinterpret_cast<const f32x2*>(sc + t), lv = *reinterpret_cast<const f32x2*>(sc + kPfBlock + t);
 #pragma unroll
-                                for (int k = 0; k < 4; k++) {
-                                    const int t = 32 * h + 8 * k;
-                                    const float2 ks = *reinterpret_cast<const float2*>(sc + t), lv = *reinterpret_cast<const float2*>(sc + kPfBlock + t),
-                                                 iv = *reinterpret_cast<const float2*>(sc + 2 * kPfBlock + t);
-                                    const int p0 = tok_base + t + 2 * quad;
-#pragma unroll
-                                    for (int hh = 0; hh < 2; hh++) {
-                                        const int rr = 2 * gi + hh;
-                                        const bool on0 = p0 < min(lim[rr], t1), on1 = p0 + 1 < min(lim[rr], t1);
-                                        const float x0 = fmaf(__uint_as_float(sf[4 * k + 2 * hh]) * ks.x, E[rr], lv.x),
-                                                    x1 = fmaf(__uint_as_float(sf[4 * k + 2 * hh + 1]) * ks.y, E[rr], lv.y);
-                                        if (ph == 0) {
-                                            if (on0) mx[rr] = fmaxf(mx[rr], x0);
-                                            if (on1) mx[rr] = fmaxf(mx[rr], x1);
-                                        } else {             // (masked: also where the scale of a token the row does not see is a NaN)
-                                            const float w0 = on0 ? ex2(x0 - m_new[rr]) : 0.0f, w1 = on1 ? ex2(x1 - m_new[rr]) : 0.0f;
-                                            if (on0) sum[rr] += w0 * iv.x;
-                                            if (on1) sum[rr] += w1 * iv.y;
-                                            pr[gi][8 * h + 2 * k + hh] = pack2<false>(w0, w1);
-                                        }
-                                    }
+                                for (int hh = 0; hh < 2; hh++) {
+                                    const int rr = 2 * gi + hh;
+                                    const float2 x = unpack_x2(fma_x2(mul_x2(pack_x2(sf[4 * k + 2 * hh], sf[4 * k + 2 * hh + 1]), ks), pack_x2(E[rr], E[rr]), lv));
+                                    mx[rr] = fmaxf(mx[rr], t < nv[rr] ? x.x : -INFINITY);
+                                    mx[rr] = fmaxf(mx[rr], t + 1 < nv[rr] ? x.y : -INFINITY);
                                 }
                             }
-                        if (ph == 0) {
-#pragma unroll
-                            for (int rr = 0; rr < 4; rr++) { // the four threads of a row agree
-                                mx[rr] = fmaxf(mx[rr], __shfl_xor_sync(0xFFFFFFFFu, mx[rr], 1));
-                                mx[rr] = fmaxf(mx[rr], __shfl_xor_sync(0xFFFFFFFFu, mx[rr], 2));
-                                const bool moved = mx[rr] > m2[rr] + kLazy;
-                                m_new[rr] = moved ? mx[rr] : m2[rr];
-                                alpha[rr] = moved ? ex2(m2[rr] - mx[rr]) : 1.0f;     // a row's first block: 0
-                                rescale = rescale || moved;
-                            }
                         }
-                    }
-#pragma unroll
-                    for (int rr = 0; rr < 4; rr++) {
-                        la[rr] = la[rr] * alpha[rr] + sum[rr];
-                        lb[rr] *= alpha[rr];
-                        m2[rr] = m_new[rr];
-                    }
                     started = true;
-                    if (blk == 0 || !full) started = __all_sync(0xFFFFFFFFu, fminf(fminf(m2[0], m2[1]), fminf(m2[2], m2[3])) > -1e29f);
+#pragma unroll
+                    for (int rr = 0; rr < 4; rr++) {         // the four threads of a row agree
+                        mx[rr] = fmaxf(mx[rr], __shfl_xor_sync(0xFFFFFFFFu, mx[rr], 1));
+                        mx[rr] = fmaxf(mx[rr], __shfl_xor_sync(0xFFFFFFFFu, mx[rr], 2));
+                        if (mx[rr] > m2[rr] + kLazy) {
+                            alpha[rr] = ex2(m2[rr] - mx[rr]);    // a row's first block: 0
+                            m2[rr] = mx[rr];
+                            rescale = true;
+                        }
+                        started = started && m2[rr] > -1e29f;
+                        l2[rr] = mul_x2(l2[rr], pack_x2(alpha[rr], alpha[rr]));
+                    }
+                    started = __all_sync(0xFFFFFFFFu, started);
+                    rescale = __any_sync(0xFFFFFFFFu, rescale);
+                    (void)weigh(std::true_type{});
                 }
+#pragma unroll
+                for (int rr = 0; rr < 4; rr++) l2[rr] = add_x2(l2[rr], tl[rr]);
                 tmem_st_half32(col_s, pr[0]);                // W over the columns S was read from
                 tmem_st_half32(col_s + (16u << 16), pr[1]);
-                rescale = __any_sync(0xFFFFFFFFu, rescale);
             }
             // O += W V of the previous block must be done before O is rescaled.  S of this block was committed behind W V of
             // block blk-2, so the barrier's phase is blk-1 or later; the last block waits in any case, so that the wait after
@@ -510,7 +571,8 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             // a row per thread from here on: (m, l) of row t through shared memory (each warp's own entries)
 #pragma unroll
             for (int rr = 0; rr < 4; rr++) {
-                float l = la[rr] + lb[rr];
+                const float2 lf = unpack_x2(l2[rr]);
+                float l = lf.x + lf.y;
                 l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
                 l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
                 if (quad == 0) {
@@ -563,10 +625,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         }
     }
 
-    // ---- tensor memory goes back on every path ----
-    tc_fence_before();
-    __syncthreads();
-    if (warp == kPfMmaWarp) tmem_dealloc(tmem, kPfTmemCols);
+    leave();
     if (n_chunks == 1) return;
     // the CTA that arrives last for the tile merges its chunks (nothing is written while the status word is set)
     if (tid == 0) {
@@ -577,11 +636,11 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         if (last) *c = 0;
         *s_flag = last;
     }
-    __syncthreads();
+    asm volatile("bar.sync 2, %0;" ::"n"(kPfRows) : "memory");
     if (*s_flag) {
         const MergeOut mo{nullptr, out, nullptr, out_dtype, nullptr, status};
         merge_rows(g, mo, b, kvh, G, 0, n_chunks, partials + (size_t)poff * g.H * (D + 2),
-                   MergeMap{G * tok_cnt, nq * g.H, q_base + tok_first, tok_first, 0});
+                   MergeMap{G * tok_cnt, nq * g.H, q_base + tok_first, tok_first, 0}, kPfSoftWarps);
     }
 }
 

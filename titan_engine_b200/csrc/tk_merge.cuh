@@ -33,12 +33,13 @@ struct MergeMap {
 };
 
 // The merge itself, by every thread of the CTA that arrived last for (b, kvh): rows r0 .. r0+n-1.
+// `warps`: how many warps call it, from warp 0 on.
 __device__ __forceinline__ void merge_rows(const Geometry& g, const MergeOut& mo, int b, int kvh, int G, int r0, int n,
-                                           const float* partials, const MergeMap& mm) {
+                                           const float* partials, const MergeMap& mm, int warps = 0) {
     __threadfence();                                   // see the other CTAs' rows
     if (mo.status && __ldcg(mo.status) != 0) return;   // fail closed: a wait timed out, leave `out` alone
     const int D = g.Dv;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_warps = blockDim.x >> 5;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_warps = warps ? warps : blockDim.x >> 5;
     const int epl = D >> 5;                            // dims per lane: 2 (D=64) or 4 (D=128)
     const PeerCtx* pc = mo.peer;
     const uint32_t epoch = pc ? __ldcg(pc->epoch) + 1u : 0u;
