@@ -34,8 +34,8 @@ constexpr int kPfRows = kPrefillRowsInt8;       // 256: two halves of kTcRows
 constexpr int kPfBlock = 64;                    // context tokens per block (4 pages)
 constexpr int kPfRaw = 4;                       // stages of raw tiles: K is expanded two blocks ahead of V
 constexpr int kPfSoftWarps = kPfRows / 32, kPfExpWarps = 4;
-constexpr int kPfMmaWarp = kPfSoftWarps + kPfExpWarps, kPfLoadWarp = kPfMmaWarp + 1;
-constexpr int kPfThreads = 512;                  // 4 warpgroups: softmax, softmax, expanders, (MMA, loader, two idle warps)
+constexpr int kPfMmaWarp = kPfSoftWarps + kPfExpWarps, kPfLoadWarp = kPfMmaWarp + 2;    // an MMA warp for each half
+constexpr int kPfThreads = 512;                  // 4 warpgroups: softmax, softmax, expanders, (two MMA warps, loader, an idle warp)
 constexpr int kPfExpThreads = kPfExpWarps * 32;
 constexpr uint32_t kPfTmemCols = 512, kPfHalfCols = 256, kPfColO = 128;   // half h: S at 256h and 256h + 64, O at 256h + 128
 
@@ -161,14 +161,14 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     }
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(smem_u32(&kfull[i]), kPfExpThreads); mbar_init(smem_u32(&vfull[i]), kPfExpThreads);
-            mbar_init(smem_u32(&kempty[i]), 1); mbar_init(smem_u32(&vempty[i]), 1);
+            mbar_init(smem_u32(&kfull[i]), kPfExpWarps); mbar_init(smem_u32(&vfull[i]), kPfExpWarps);
+            mbar_init(smem_u32(&kempty[i]), halves); mbar_init(smem_u32(&vempty[i]), halves);
             mbar_init(smem_u32(&bar_o[i]), 1);
         }
         for (int i = 0; i < 4; i++) {
-            mbar_init(smem_u32(&scfull[i]), kPfBlock);
+            mbar_init(smem_u32(&scfull[i]), kPfBlock / 32);
             mbar_init(smem_u32(&bar_s[i]), 1);
-            mbar_init(smem_u32(&p_ready[i]), kTcRows);
+            mbar_init(smem_u32(&p_ready[i]), kTcRows / 32);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -187,7 +187,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     };
     if (warp == kPfLoadWarp) {
         if (lane == 0) {
-            for (int i = 0; i < kPfRaw; i++) { mbar_init(smem_u32(&rawfull[i]), 1); mbar_init(smem_u32(&rawempty[i]), kPfExpThreads); }
+            for (int i = 0; i < kPfRaw; i++) { mbar_init(smem_u32(&rawfull[i]), 1); mbar_init(smem_u32(&rawempty[i]), kPfExpWarps); }
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
@@ -253,6 +253,11 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
 
     // Registers: 512 threads x 128 at launch; 160 for the two softmax warpgroups, 88 for the others (2 x 128 x (160 + 88) = 63488 of
     // the 65536 the block was launched with).
+    // One arrival per warp, after all its lanes' writes.
+    auto warp_arrive = [&](uint64_t* bar) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(bar));
+    };
     // A role other than softmax ends at the barrier that all threads of the CTA meet on, whatever became of it.
     auto leave = [&]() {
         tc_fence_before();
@@ -260,68 +265,59 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     };
     if (warp >= kPfMmaWarp) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == kPfMmaWarp) {
-        // ===== MMA warp: an elected lane feeds the tensor pipe =====
+    if (warp - kPfMmaWarp < halves) {
+        // ===== MMA warps, one per half of the tile: an elected lane feeds the tensor pipe =====
+        // (one warp for both halves made each wait for the other's barriers)
+        const int half = warp - kPfMmaWarp;
         constexpr uint32_t kIdescS = instr_desc(false, false, kPfBlock), kIdescO = instr_desc(false, true, D);
-        const uint64_t desc_q = smem_desc(smem_u32(s_q), 16), desc_k = smem_desc(smem_u32(s_k), 16),
+        const uint64_t dq = smem_desc(smem_u32(s_q + half * C::HALVES * kTcRows * 128), 16), desc_k = smem_desc(smem_u32(s_k), 16),
                        desc_v = smem_desc(smem_u32(s_v), C::HALF);
+        const uint32_t at = tmem + half * kPfHalfCols;
         auto await = [&](uint64_t* bar, uint32_t parity) {
             const bool done = __all_sync(0xFFFFFFFFu, mbar_wait_bounded_idle(smem_u32(bar), parity, status));
             tc_fence_after();
             return done;
         };
-        auto issue_s = [&](int half, int blk) {              // S = Q K^T of a half's rows
-            const uint64_t dq = desc_q + (uint64_t)((half * C::HALVES * kTcRows * 128) >> 4);
+        auto issue_s = [&](int blk) {                        // S = Q K^T
             const uint64_t dk = desc_k + (uint64_t)(((blk & 1) * C::SLAB) >> 4);
-            const uint32_t d_s = tmem + half * kPfHalfCols + 64u * (blk & 1);
             if (elect_one()) {
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ks++)
-                    tc_mma_ss(d_s, dq + (uint64_t)(((ks >> 2) * (kTcRows * 128) + (ks & 3) * 32) >> 4),
+                    tc_mma_ss(at + 64u * (blk & 1), dq + (uint64_t)(((ks >> 2) * (kTcRows * 128) + (ks & 3) * 32) >> 4),
                               dk + (uint64_t)(((ks >> 2) * C::HALF + (ks & 3) * 32) >> 4), kIdescS, ks > 0);
                 tc_commit(smem_u32(&bar_s[2 * half + (blk & 1)]));
-                if (half == halves - 1) tc_commit(smem_u32(&kempty[blk & 1]));       // (covers the other half's too)
+                tc_commit(smem_u32(&kempty[blk & 1]));
             }
             __syncwarp();
         };
-        auto issue_o = [&](int half, int blk) {              // O += W V, 16 tokens per MMA: 8 columns of W, 16 rows of the V slab
+        auto issue_o = [&](int blk) {                        // O += W V, 16 tokens per MMA: 8 columns of W, 16 rows of the V slab
             const uint64_t dv = desc_v + (uint64_t)(((blk & 1) * C::SLAB) >> 4);
-            const uint32_t at = tmem + half * kPfHalfCols;
             const uint32_t acc = blk > 0 ? 1u : 0u;
             if (elect_one()) {
 #pragma unroll
                 for (int ks = 0; ks < 4; ks++)
                     tc_mma_ts(at + kPfColO, at + 64u * (blk & 1) + 8 * ks, dv + (uint64_t)((ks * 2048) >> 4), kIdescO, ks > 0 ? 1u : acc);
                 tc_commit(smem_u32(&bar_o[half]));
-                if (half == halves - 1) tc_commit(smem_u32(&vempty[blk & 1]));
+                tc_commit(smem_u32(&vempty[blk & 1]));
             }
             __syncwarp();
         };
         bool ok = true;
         for (int blk = 0; blk < 2 && blk < n_blocks && ok; blk++) {
             ok = await(&kfull[blk], 0u);
-            if (!ok) break;
-            issue_s(0, blk);
-            if (halves == 2) issue_s(1, blk);
+            if (ok) issue_s(blk);
         }
         for (int blk = 0; blk < n_blocks && ok; blk++) {
             const int s = blk & 1;
             const uint32_t ph = (uint32_t)((blk >> 1) & 1);
-            // a half's W of this block is in tensor memory (and O rescaled): O += W V, then S of the block after next.  MMAs run
-            // in order: S(blk+2) overwrites the columns after W V has read them
-            ok = await(&vfull[s], ph) && await(&p_ready[s], ph);
+            // W of this block is in tensor memory (and O rescaled): O += W V, then S of the block after next.  The warp's MMAs run in
+            // order: S(blk+2) overwrites the columns after W V has read them
+            ok = await(&vfull[s], ph) && await(&p_ready[2 * half + s], ph);
             if (!ok) break;
-            issue_o(0, blk);
+            issue_o(blk);
             if (blk + 2 < n_blocks) {
                 ok = await(&kfull[s], ph ^ 1u);
-                if (!ok) break;
-                issue_s(0, blk + 2);
-            }
-            if (halves == 2) {
-                ok = await(&p_ready[2 + s], ph);
-                if (!ok) break;
-                issue_o(1, blk);
-                if (blk + 2 < n_blocks) issue_s(1, blk + 2);
+                if (ok) issue_s(blk + 2);
             }
         }
     } else if (warp == kPfLoadWarp) {
@@ -370,7 +366,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             if (!mbar_wait_bounded_idle(smem_u32(&rawfull[rs]), (uint32_t)((blk / kPfRaw) & 1), status)) return false;
             if (blk >= 2 && !mbar_wait_bounded_idle(smem_u32(&kempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
             expand(raw, 0, s_k + s * C::SLAB);
-            mbar_arrive(smem_u32(&kfull[s]));
+            warp_arrive(&kfull[s]);
             if (et < kPfBlock) {
                 // (the numbers of block blk - 4 are out of use: S of block blk - 2, whose slab was just handed back, was
                 // issued after every row's W of block blk - 4)
@@ -382,7 +378,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                 o[0] = in ? ks * sc2E : 0.0f;
                 o[kPfBlock] = in ? pf_lg2(vs) : 0.0f;
                 o[2 * kPfBlock] = in ? __fdividef(1.0f, vs) : 0.0f;
-                mbar_arrive(smem_u32(&scfull[blk & 3]));
+                warp_arrive(&scfull[blk & 3]);
             }
             return true;
         };
@@ -390,8 +386,8 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             const int s = blk & 1, rs = blk % kPfRaw;
             if (blk >= 2 && !mbar_wait_bounded_idle(smem_u32(&vempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
             expand(s_raw + rs * C::RAW, 1, s_v + s * C::SLAB);
-            mbar_arrive(smem_u32(&vfull[s]));
-            mbar_arrive(smem_u32(&rawempty[rs]));
+            warp_arrive(&vfull[s]);
+            if (lane == 0) mbar_arrive(smem_u32(&rawempty[rs]));
             return true;
         };
         // W V of block i - 2 and S of block i end together: they hand back the slabs of V(i) and K(i + 2), needed in this order
@@ -561,7 +557,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             }
             tc_wait_st();
             tc_fence_before();
-            mbar_arrive(smem_u32(&p_ready[2 * half + buf])); // these rows' W (and O) are ready for the tensor pipe
+            warp_arrive(&p_ready[2 * half + buf]);           // these rows' W (and O) are ready for the tensor pipe
         }
         if (alive && !__all_sync(0xFFFFFFFFu, mbar_wait_bounded(smem_u32(&bar_o[half]), (uint32_t)((n_blocks - 1) & 1), status))) alive = false;
         tc_fence_after();
