@@ -11,7 +11,7 @@
 //   4 expander warps codes -> fp16 into the 128-byte-swizzled slabs the MMAs read (2 K and 2 V stages), and the three
 //                    numbers per token the softmax needs: ks log2(e)/sqrt(D), log2 vs, 1/vs (4 stages)
 //   MMA thread       S = Q K^T (M 128, N 64) and O += W V (M 128, N D, W from tensor memory) for both halves
-//   8 softmax warps  32 rows each, as fragments: a speculative pass against the current reference, redone when a score exceeds it
+//   16 softmax warps 16 rows each, as fragments: a speculative pass against the current reference, redone when a score exceeds it
 //                    by 2^8 or the block is cut; only then O is rescaled (prefill_tc.cu describes the scheme)
 // The expansion is what an 8-bit cache costs over a 16-bit one: 2 D values per token, shared here by 256 rows - about an
 // eighth of the issue slots - where two CTAs of 128 rows would each do it.  Tensor memory: per half two S buffers of 64
@@ -33,9 +33,10 @@ namespace {
 constexpr int kPfRows = kPrefillRowsInt8;       // 256: two halves of kTcRows
 constexpr int kPfBlock = 64;                    // context tokens per block (4 pages)
 constexpr int kPfRaw = 4;                       // stages of raw tiles: K is expanded two blocks ahead of V
-constexpr int kPfSoftWarps = kPfRows / 32, kPfExpWarps = 4;
+constexpr int kPfSoftWarps = kPfRows / 16, kPfExpWarps = 4;
 constexpr int kPfMmaWarp = kPfSoftWarps + kPfExpWarps, kPfLoadWarp = kPfMmaWarp + 2;    // an MMA warp for each half
-constexpr int kPfThreads = 512;                  // 4 warpgroups: softmax, softmax, expanders, (two MMA warps, loader, an idle warp)
+constexpr int kPfThreads = 768;                  // 6 warpgroups: 4 of softmax, expanders, (two MMA warps, loader, an idle warp)
+constexpr int kPfSoftThreads = kPfSoftWarps * 32;
 constexpr int kPfExpThreads = kPfExpWarps * 32;
 constexpr uint32_t kPfTmemCols = 512, kPfHalfCols = 256, kPfColO = 128;   // half h: S at 256h and 256h + 64, O at 256h + 128
 
@@ -48,7 +49,7 @@ struct PfCfg {
     static constexpr int HALF = kPfBlock * 128;
     static constexpr int RAW = 4 * TILE;
     static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + 2 * SLAB, OFF_RAW = OFF_V + 2 * SLAB, OFF_SC = OFF_RAW + kPfRaw * RAW,
-                         OFF_E = OFF_SC + 4 * 3 * kPfBlock * 4, OFF_PAGES = OFF_E + 2 * kPfRows * 4, OFF_BARS = OFF_PAGES + kPrefillMaxPages * 4,
+                         OFF_E = OFF_SC + 4 * 3 * kPfBlock * 4, OFF_PAGES = OFF_E + kPfRows * 4, OFF_BARS = OFF_PAGES + kPrefillMaxPages * 4,
                          SMEM = OFF_BARS + 512 + 1024;
 };
 
@@ -115,15 +116,14 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t *s_q = smem, *s_k = smem + C::OFF_K, *s_v = smem + C::OFF_V, *s_raw = smem + C::OFF_RAW;
     float* s_sc = (float*)(smem + C::OFF_SC);               // [4][3][64]: ks log2(e)/sqrt(D), log2 vs, 1/vs
-    float* s_e = (float*)(smem + C::OFF_E);                 // [256] power of two of the row's query; at the end the row's reference
-    float* s_l = s_e + kPfRows;                             // [256] at the end the row's sum
+    float* s_e = (float*)(smem + C::OFF_E);                 // [256] power of two of the row's query
     int32_t* s_pages = (int32_t*)(smem + C::OFF_PAGES);
     uint64_t* bars = (uint64_t*)(smem + C::OFF_BARS);
     uint64_t *rawfull = bars, *rawempty = bars + 4, *kfull = bars + 8, *kempty = bars + 10, *vfull = bars + 12, *vempty = bars + 14,
              *scfull = bars + 16, *bar_s = bars + 20 /* [half][2] */, *p_ready = bars + 24 /* [half][2] */, *bar_o = bars + 28 /* [half] */;
     uint32_t* s_tmem = (uint32_t*)(bars + 30);
     int* s_flag = (int*)(s_tmem + 1);
-    uint32_t* s_wmax = (uint32_t*)(bars + 32);              // [warps] prologue: largest query magnitude
+    uint32_t* s_wmax = (uint32_t*)(bars + 32);              // [24 warps] prologue: largest query magnitude
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = g.H / g.Hkv;
@@ -143,18 +143,14 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     const int n_chunks = p_last / ct + 1;
     const int32_t* pt_row = page_table + (size_t)seq * g.max_pages_per_seq + t0 / kI8Page;
 
-    // this thread's row of the tile at the end (softmax warps): query token tid / G of the tile, head tid % G of the group
-    const bool valid = tid < kPfRows && tid / G < tok_cnt;
-    const size_t qo_row = (size_t)(q_base + tok_first + tid / G) * g.H + (size_t)kvh * G + tid % G;
-
     // ---- prologue ----
-    constexpr int LPR = D / 8;                              // lanes (16-byte vectors) per query row
-    uint4 qv[LPR];
-    if (tid < kPfRows) {
+    constexpr int LPR = D / 8, QV = kPfRows * LPR / kPfSoftThreads;      // 16-byte vectors per query row, per softmax thread
+    uint4 qv[QV];
+    if (tid < kPfSoftThreads) {
         const int sh = __ffs(G) - 1;                        // G divides 128: a power of two
 #pragma unroll
-        for (int i = 0; i < LPR; i++) {
-            const int r = (i * kPfRows + tid) / LPR, c = tid % LPR;
+        for (int i = 0; i < QV; i++) {
+            const int r = (i * kPfSoftThreads + tid) / LPR, c = tid % LPR;
             const size_t row = (size_t)(q_base + tok_first + (r >> sh)) * g.H + (size_t)kvh * G + (r & (G - 1));
             qv[i] = (r >> sh) < tok_cnt ? __ldg(reinterpret_cast<const uint4*>(q + row * D) + c) : make_uint4(0, 0, 0, 0);
         }
@@ -168,7 +164,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         for (int i = 0; i < 4; i++) {
             mbar_init(smem_u32(&scfull[i]), kPfBlock / 32);
             mbar_init(smem_u32(&bar_s[i]), 1);
-            mbar_init(smem_u32(&p_ready[i]), kTcRows / 32);
+            mbar_init(smem_u32(&p_ready[i]), kPfSoftWarps / 2);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -200,12 +196,12 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     // its own, and its scores are multiplied by it.
     int e0 = 0;
     bool wide = false;
-    uint32_t row_max[LPR];                                  // bf16 pattern of each of this thread's vectors' rows' largest magnitude
+    uint32_t row_max[QV];                                  // bf16 pattern of each of this thread's vectors' rows' largest magnitude
     if (IO_BF16) {
         uint32_t m_all = 0;
-        if (tid < kPfRows) {
+        if (tid < kPfSoftThreads) {
 #pragma unroll
-            for (int i = 0; i < LPR; i++) {
+            for (int i = 0; i < QV; i++) {
                 uint32_t m = i8_absmax8(qv[i]);
 #pragma unroll
                 for (int off = LPR / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
@@ -221,10 +217,10 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         e0 = m_all ? max((int)(m_all >> 7) - 127 - 14, -100) : 0;
         wide = e0 > 0;                                      // some |q| >= 2^15
     }
-    if (tid < kPfRows) {
+    if (tid < kPfSoftThreads) {
 #pragma unroll
-        for (int i = 0; i < LPR; i++) {
-            const int r = (i * kPfRows + tid) / LPR, c = tid % LPR;
+        for (int i = 0; i < QV; i++) {
+            const int r = (i * kPfSoftThreads + tid) / LPR, c = tid % LPR;
             uint4 x = qv[i];
             if (IO_BF16) {
                 const int e = wide ? (row_max[i] ? max((int)(row_max[i] >> 7) - 127 - 14, -100) : 0) : e0;
@@ -251,8 +247,8 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     bool alive = true;
     constexpr float kLazy = 8.0f;
 
-    // Registers: 512 threads x 128 at launch; 160 for the two softmax warpgroups, 88 for the others (2 x 128 x (160 + 88) = 63488 of
-    // the 65536 the block was launched with).
+    // Registers: 768 threads x 80 at launch; 88 for the four softmax warpgroups, 64 for the other two (512 x 88 + 256 x 64 = 61440,
+    // what the block was launched with).
     // One arrival per warp, after all its lanes' writes.
     auto warp_arrive = [&](uint64_t* bar) {
         __syncwarp();
@@ -264,7 +260,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         asm volatile("bar.sync 1, %0;" ::"n"(kPfThreads) : "memory");
     };
     if (warp >= kPfMmaWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp - kPfMmaWarp < halves) {
         // ===== MMA warps, one per half of the tile: an elected lane feeds the tensor pipe =====
         // (one warp for both halves made each wait for the other's barriers)
@@ -337,7 +333,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     return;
     }
     if (warp >= kPfSoftWarps) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         // ===== expander warps: codes -> fp16 slabs =====
         const int et = tid - kPfSoftWarps * 32;
         const float sc2E = kLog2e / sqrtf((float)D) * (IO_BF16 && !wide ? pf_pow2i(e0) : 1.0f);
@@ -396,28 +392,32 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         leave();
         return;
     }
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
-    if (warp < halves * (kTcRows / 32)) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+    if (warp < halves * (kPfSoftWarps / 2)) {
         // ===== softmax warps =====
-        // A warp owns 32 rows (tensor-memory lanes), as fragments: thread t holds, of rows t/4, +8, +16, +24, the columns
-        // 2 (t%4), +1 of every eight.  The numbers of a token are then read once for four rows (with a row per thread each
-        // would be a broadcast of its own: 192 shared-memory wavefronts per warp and block instead of 24).
-        const int half = warp >> 2, quad = lane & 3;
-        const uint32_t base = tmem + half * kPfHalfCols + ((uint32_t)((warp & 3) * 32) << 16);    // this warp's 32 lanes
-        float E[4], m2[4];                                   // per row: query's power of two, reference (base 2)
-        f32x2 l2[4];                                         // ... sums over this thread's even and odd columns
-        int lim[4];                                          // positions the row sees
+        // A warp owns 16 rows (tensor-memory lanes; the two that share a 32-lane window, and a scheduler, take a half of it each),
+        // as fragments: thread t holds, of rows t/4 and t/4 + 8, the columns 2 (t%4), +1 of every eight.  The numbers of a
+        // token are then read once for 16 rows (with a row per thread each would be a broadcast of its own: 192 shared-memory
+        // wavefronts per 32 rows and block instead of 48).  Four warps per scheduler, because the pass is a chain of TMEM load,
+        // multiply-add, exponential, conversion: with two, of 32 rows each, it took 2200 clocks a block of which the
+        // special-function unit worked 1024.
+        const int half = warp >> 3, quad = lane & 3;
+        const int row0 = half * kTcRows + (warp & 3) * 32 + ((warp >> 2) & 1) * 16 + (lane >> 2);    // + 8 rr
+        const uint32_t base = tmem + half * kPfHalfCols + ((uint32_t)((warp & 3) * 32 + ((warp >> 2) & 1) * 16) << 16);
+        float E[2], m2[2];                                   // per row: query's power of two, reference (base 2)
+        f32x2 l2[2];                                         // ... sums over this thread's even and odd columns
+        int lim[2];                                          // positions the row sees
 #pragma unroll
-        for (int rr = 0; rr < 4; rr++) {
-            const int row = warp * 32 + 8 * rr + (lane >> 2);
+        for (int rr = 0; rr < 2; rr++) {
+            const int row = row0 + 8 * rr;
             E[rr] = IO_BF16 && wide ? s_e[row] : 1.0f;
             m2[rr] = -1e30f;
             l2[rr] = 0ull;
             // (rows without a token: zero queries, nothing of theirs is written; unmasked, so that they cost no careful pass)
             lim[rr] = row / G < tok_cnt ? base_pos + tok_first + row / G + 1 : len;
         }
-        const bool idle = (warp * 32) / G >= tok_cnt;        // no row of this warp has a token: whatever W holds, nobody reads its O
-        const int lim_min = min(min(lim[0], lim[1]), min(lim[2], lim[3]));
+        const bool idle = (row0 - (lane >> 2)) / G >= tok_cnt;   // no row of this warp has a token: whatever W holds, nobody reads its O
+        const int lim_min = min(lim[0], lim[1]);
         bool started = false;
         for (int blk = 0; blk < n_blocks; blk++) {
             const int buf = blk & 1;
@@ -429,42 +429,38 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             if (!__all_sync(0xFFFFFFFFu, ok)) { alive = false; break; }
             tc_fence_after();
             bool rescale = false;
-            float alpha[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+            float alpha[2] = {1.0f, 1.0f};
             if (!idle) {
                 const int end = min(t1, tok_base + kPfBlock);
                 // whole: every row of the warp sees all of the block and no power of two is due
                 const bool whole = !(IO_BF16 && wide) && end - tok_base == kPfBlock && __all_sync(0xFFFFFFFFu, lim_min >= tok_base + kPfBlock);
-                int nv[4];                                   // of a row: tokens of the block it sees, from this thread's first column on
+                int nv[2];                                   // of a row: tokens of the block it sees, from this thread's first column on
 #pragma unroll
-                for (int rr = 0; rr < 4; rr++) nv[rr] = min(lim[rr], end) - tok_base - 2 * quad;
-                uint32_t pr[2][16];                          // W of rows (0, 8) and (16, 24) + t/4 as 16x128b fragments
-                f32x2 tl[4];                                 // the block's share of the sums
+                for (int rr = 0; rr < 2; rr++) nv[rr] = min(lim[rr], end) - tok_base - 2 * quad;
+                uint32_t pr[16];                             // W of the rows as a 16x128b fragment
+                f32x2 tl[2];                                 // the block's share of the sums
                 // The weights of the block against the current references, 16 columns of S at a time, the next 16 on their way; S
                 // stays in tensor memory.  -> whether a score exceeds its row's reference by more than 2^kLazy.
                 auto weigh = [&](auto masked) -> bool {
                     constexpr bool M = decltype(masked)::value;
-                    f32x2 nm[4];
+                    f32x2 nm[2];
                     float top = -1e30f;
 #pragma unroll
-                    for (int rr = 0; rr < 4; rr++) { tl[rr] = 0ull; nm[rr] = pack_x2(-m2[rr], -m2[rr]); }
-                    uint32_t sr[2][2][8];
-                    tmem_ld_frag16(col_s, sr[0][0]);
-                    tmem_ld_frag16(col_s + (16u << 16), sr[0][1]);
+                    for (int rr = 0; rr < 2; rr++) { tl[rr] = 0ull; nm[rr] = pack_x2(-m2[rr], -m2[rr]); }
+                    uint32_t sr[2][8];
+                    tmem_ld_frag16(col_s, sr[0]);
 #pragma unroll
                     for (int qt = 0; qt < 4; qt++) {
-                        tc_wait_ld_frag16(sr[qt & 1][0], sr[qt & 1][1]);
-                        if (qt < 3) {
-                            tmem_ld_frag16(col_s + 16 * (qt + 1), sr[(qt + 1) & 1][0]);
-                            tmem_ld_frag16(col_s + 16 * (qt + 1) + (16u << 16), sr[(qt + 1) & 1][1]);
-                        }
+                        tc_wait_ld_frag16(sr[qt & 1]);
+                        if (qt < 3) tmem_ld_frag16(col_s + 16 * (qt + 1), sr[(qt + 1) & 1]);
 #pragma unroll
                         for (int k = 0; k < 2; k++) {        // tokens 16 qt + 8 k + 2 quad, +1
                             const int t = 16 * qt + 8 * k;
                             const f32x2 ks = *reinterpret_cast<const f32x2*>(sc + t), lv = *reinterpret_cast<const f32x2*>(sc + kPfBlock + t),
                                         iv = *reinterpret_cast<const f32x2*>(sc + 2 * kPfBlock + t);
 #pragma unroll
-                            for (int rr = 0; rr < 4; rr++) {
-                                const f32x2 a = pack_x2(sr[qt & 1][rr >> 1][4 * k + 2 * (rr & 1)], sr[qt & 1][rr >> 1][4 * k + 2 * (rr & 1) + 1]);
+                            for (int rr = 0; rr < 2; rr++) {
+                                const f32x2 a = pack_x2(sr[qt & 1][4 * k + 2 * rr], sr[qt & 1][4 * k + 2 * rr + 1]);
                                 const f32x2 u = add_x2(lv, nm[rr]);
                                 float2 x = unpack_x2(M ? fma_x2(mul_x2(a, ks), pack_x2(E[rr], E[rr]), u) : fma_x2(a, ks, u));
                                 if (M) {                     // (also where the scale of a token the row does not see is a NaN)
@@ -479,7 +475,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                                 } else {
                                     tl[rr] = fma_x2(pack_x2(w0, w1), iv, tl[rr]);
                                 }
-                                pr[rr >> 1][4 * qt + 2 * k + (rr & 1)] = pack2<false>(w0, w1);
+                                pr[4 * qt + 2 * k + rr] = pack2<false>(w0, w1);
                             }
                         }
                     }
@@ -489,32 +485,27 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                 bool look = !started;
                 if (!look) look = whole ? weigh(std::false_type{}) : weigh(std::true_type{});
                 if (look) {                                  // new references for the rows that need one, then the weights
-                    float mx[4];
+                    float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int rr = 0; rr < 4; rr++) mx[rr] = -INFINITY;
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t sf[16];
+                        tmem_ld_frag32(col_s + 32 * h, sf);
+                        tc_wait_ld16(sf);
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                        for (int k = 0; k < 4; k++) {
+                            const int t = 32 * h + 8 * k;
+                            const f32x2 ks = *reinterpret_cast<const f32x2*>(sc + t), lv = *reinterpret_cast<const f32x2*>(sc + kPfBlock + t);
 #pragma unroll
-                        for (int gi = 0; gi < 2; gi++) {
-                            uint32_t sf[16];
-                            tmem_ld_frag32(col_s + 32 * h + ((uint32_t)(16 * gi) << 16), sf);
-                            tc_wait_ld16(sf);
-#pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                const int t = 32 * h + 8 * k;
-                                const f32x2 ks = *reinterpret_cast<const f32x2*>(sc + t), lv = *reinterpret_cast<const f32x2*>(sc + kPfBlock + t);
-#pragma unroll
-                                for (int hh = 0; hh < 2; hh++) {
-                                    const int rr = 2 * gi + hh;
-                                    const float2 x = unpack_x2(fma_x2(mul_x2(pack_x2(sf[4 * k + 2 * hh], sf[4 * k + 2 * hh + 1]), ks), pack_x2(E[rr], E[rr]), lv));
-                                    mx[rr] = fmaxf(mx[rr], t < nv[rr] ? x.x : -INFINITY);
-                                    mx[rr] = fmaxf(mx[rr], t + 1 < nv[rr] ? x.y : -INFINITY);
-                                }
+                            for (int rr = 0; rr < 2; rr++) {
+                                const float2 x = unpack_x2(fma_x2(mul_x2(pack_x2(sf[4 * k + 2 * rr], sf[4 * k + 2 * rr + 1]), ks), pack_x2(E[rr], E[rr]), lv));
+                                mx[rr] = fmaxf(mx[rr], t < nv[rr] ? x.x : -INFINITY);
+                                mx[rr] = fmaxf(mx[rr], t + 1 < nv[rr] ? x.y : -INFINITY);
                             }
                         }
+                    }
                     started = true;
 #pragma unroll
-                    for (int rr = 0; rr < 4; rr++) {         // the four threads of a row agree
+                    for (int rr = 0; rr < 2; rr++) {         // the four threads of a row agree
                         mx[rr] = fmaxf(mx[rr], __shfl_xor_sync(0xFFFFFFFFu, mx[rr], 1));
                         mx[rr] = fmaxf(mx[rr], __shfl_xor_sync(0xFFFFFFFFu, mx[rr], 2));
                         if (mx[rr] > m2[rr] + kLazy) {
@@ -530,9 +521,8 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                     (void)weigh(std::true_type{});
                 }
 #pragma unroll
-                for (int rr = 0; rr < 4; rr++) l2[rr] = add_x2(l2[rr], tl[rr]);
-                tmem_st_half32(col_s, pr[0]);                // W over the columns S was read from
-                tmem_st_half32(col_s + (16u << 16), pr[1]);
+                for (int rr = 0; rr < 2; rr++) l2[rr] = add_x2(l2[rr], tl[rr]);
+                tmem_st_half32(col_s, pr);                   // W over the columns S was read from
             }
             // O += W V of the previous block must be done before O is rescaled.  S of this block was committed behind W V of
             // block blk-2, so the barrier's phase is blk-1 or later; the last block waits in any case, so that the wait after
@@ -542,17 +532,14 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                 tc_fence_after();
                 if (rescale) {
 #pragma unroll
-                    for (int part = 0; part < D / 32; part++)
+                    for (int part = 0; part < D / 32; part++) {
+                        uint32_t of[16];
+                        tmem_ld_frag32(base + kPfColO + 32 * part, of);
+                        tc_wait_ld16(of);
 #pragma unroll
-                        for (int gi = 0; gi < 2; gi++) {
-                            uint32_t of[16];
-                            const uint32_t at = base + kPfColO + 32 * part + ((uint32_t)(16 * gi) << 16);
-                            tmem_ld_frag32(at, of);
-                            tc_wait_ld16(of);
-#pragma unroll
-                            for (int c = 0; c < 16; c++) of[c] = __float_as_uint(__uint_as_float(of[c]) * alpha[2 * gi + ((c >> 1) & 1)]);
-                            tmem_st_frag32(at, of);
-                        }
+                        for (int c = 0; c < 16; c++) of[c] = __float_as_uint(__uint_as_float(of[c]) * alpha[(c >> 1) & 1]);
+                        tmem_st_frag32(base + kPfColO + 32 * part, of);
+                    }
                 }
             }
             tc_wait_st();
@@ -564,60 +551,48 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
 
         const bool poisoned = __any_sync(0xFFFFFFFFu, !alive || __ldcg(status) != 0);   // fail closed, whole warps at a time
         if (!poisoned && !idle) {
-            // a row per thread from here on: (m, l) of row t through shared memory (each warp's own entries)
+            float f[2];
+            float* prow[2];
+            size_t qo[2];
+            bool valid[2];
 #pragma unroll
-            for (int rr = 0; rr < 4; rr++) {
+            for (int rr = 0; rr < 2; rr++) {
                 const float2 lf = unpack_x2(l2[rr]);
                 float l = lf.x + lf.y;
                 l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
                 l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-                if (quad == 0) {
-                    s_e[warp * 32 + 8 * rr + (lane >> 2)] = m2[rr];
-                    s_l[warp * 32 + 8 * rr + (lane >> 2)] = l;
+                const int row = row0 + 8 * rr, tok = tok_first + row / G, head = kvh * G + row % G;
+                valid[rr] = row / G < tok_cnt;
+                qo[rr] = ((size_t)(q_base + tok) * g.H + head) * D;
+                prow[rr] = nullptr;
+                f[rr] = l == 0.0f ? 0.0f : 1.0f / l;         // l counts weights over value scales: at least one term of any size
+                if (n_chunks > 1) {                          // (o, m, l) of this chunk, brought to l in [1, 2)
+                    prow[rr] = partials + (size_t)poff * g.H * (D + 2) + partial_off(chunk, tok * g.H + head, nq * g.H, D);
+                    const uint32_t ex = (__float_as_uint(l) >> 23) & 0xFFu;
+                    const int k = ex == 0 || ex >= 254 ? 0 : (int)ex - 127;
+                    f[rr] = pf_pow2i(-k);
+                    if (valid[rr] && quad == 0)
+                        *reinterpret_cast<float2*>(prow[rr] + D) = make_float2(l == 0.0f ? -1e30f : (m2[rr] + (float)k) * 0.6931471805599453f, l * f[rr]);
                 }
-            }
-            __syncwarp();
-            const float m_run = s_e[tid], l_run = s_l[tid];
-            float* prow = nullptr;
-            float f = l_run == 0.0f ? 0.0f : 1.0f / l_run;   // l counts weights over value scales: at least one term of any size
-            float m_row = m_run;
-            if (n_chunks > 1) {                              // (o, m, l) of this chunk, brought to l in [1, 2)
-                prow = partials + (size_t)poff * g.H * (D + 2) +
-                       partial_off(chunk, (tok_first + tid / G) * g.H + kvh * G + tid % G, nq * g.H, D);
-                const uint32_t ex = (__float_as_uint(l_run) >> 23) & 0xFFu;
-                const int k = ex == 0 || ex >= 254 ? 0 : (int)ex - 127;
-                f = pf_pow2i(-k);
-                m_row = l_run == 0.0f ? -1e30f : (m_run + (float)k) * 0.6931471805599453f;
             }
 #pragma unroll
             for (int part = 0; part < D / 32; part++) {
-                uint32_t orow[32];
-                tmem_ld32(base + kPfColO + 32 * part, orow);
-                tc_wait_ld(orow);
-                if (!valid) continue;
-                if (n_chunks > 1) {
+                uint32_t of[16];
+                tmem_ld_frag32(base + kPfColO + 32 * part, of);
+                tc_wait_ld16(of);
 #pragma unroll
-                    for (int c = 0; c < 32; c += 2)
-                        *reinterpret_cast<float2*>(prow + 32 * part + c) = make_float2(__uint_as_float(orow[c]) * f, __uint_as_float(orow[c + 1]) * f);
-                } else if (out_dtype == DT_FP32) {
+                for (int rr = 0; rr < 2; rr++) {
+                    if (!valid[rr]) continue;
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4)
-                        *reinterpret_cast<float4*>((float*)out + qo_row * D + 32 * part + c) =
-                            make_float4(__uint_as_float(orow[c]) * f, __uint_as_float(orow[c + 1]) * f, __uint_as_float(orow[c + 2]) * f,
-                                        __uint_as_float(orow[c + 3]) * f);
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 32; c += 8) {
-                        uint4 w;
-                        w.x = pack2<IO_BF16>(__uint_as_float(orow[c]) * f, __uint_as_float(orow[c + 1]) * f);
-                        w.y = pack2<IO_BF16>(__uint_as_float(orow[c + 2]) * f, __uint_as_float(orow[c + 3]) * f);
-                        w.z = pack2<IO_BF16>(__uint_as_float(orow[c + 4]) * f, __uint_as_float(orow[c + 5]) * f);
-                        w.w = pack2<IO_BF16>(__uint_as_float(orow[c + 6]) * f, __uint_as_float(orow[c + 7]) * f);
-                        *reinterpret_cast<uint4*>((uint16_t*)out + qo_row * D + 32 * part + c) = w;
+                    for (int k = 0; k < 4; k++) {
+                        const float o0 = __uint_as_float(of[4 * k + 2 * rr]) * f[rr], o1 = __uint_as_float(of[4 * k + 2 * rr + 1]) * f[rr];
+                        const int c = 32 * part + 8 * k + 2 * quad;
+                        if (n_chunks > 1)                *reinterpret_cast<float2*>(prow[rr] + c) = make_float2(o0, o1);
+                        else if (out_dtype == DT_FP32)   *reinterpret_cast<float2*>((float*)out + qo[rr] + c) = make_float2(o0, o1);
+                        else                             *reinterpret_cast<uint32_t*>((uint16_t*)out + qo[rr] + c) = pack2<IO_BF16>(o0, o1);
                     }
                 }
             }
-            if (n_chunks > 1 && valid) *reinterpret_cast<float2*>(prow + D) = make_float2(m_row, l_run * f);
         }
     }
 
@@ -632,7 +607,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         if (last) *c = 0;
         *s_flag = last;
     }
-    asm volatile("bar.sync 2, %0;" ::"n"(kPfRows) : "memory");
+    asm volatile("bar.sync 2, %0;" ::"n"(kPfSoftThreads) : "memory");
     if (*s_flag) {
         const MergeOut mo{nullptr, out, nullptr, out_dtype, nullptr, status};
         merge_rows(g, mo, b, kvh, G, 0, n_chunks, partials + (size_t)poff * g.H * (D + 2),
