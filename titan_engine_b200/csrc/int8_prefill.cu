@@ -247,7 +247,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     bool alive = true;
     constexpr float kLazy = 8.0f;
 
-    // Registers: 768 threads x 80 at launch; 88 for the four softmax warpgroups, 64 for the other two (512 x 88 + 256 x 64 = 61440,
+    // Registers: 768 threads x 80 at launch; 96 for the four softmax warpgroups, 48 for the other two (512 x 96 + 256 x 48 = 61440,
     // what the block was launched with).
     // One arrival per warp, after all its lanes' writes.
     auto warp_arrive = [&](uint64_t* bar) {
@@ -260,7 +260,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         asm volatile("bar.sync 1, %0;" ::"n"(kPfThreads) : "memory");
     };
     if (warp >= kPfMmaWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp - kPfMmaWarp < halves) {
         // ===== MMA warps, one per half of the tile: an elected lane feeds the tensor pipe =====
         // (one warp for both halves made each wait for the other's barriers)
@@ -270,7 +270,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                        desc_v = smem_desc(smem_u32(s_v), C::HALF);
         const uint32_t at = tmem + half * kPfHalfCols;
         auto await = [&](uint64_t* bar, uint32_t parity) {
-            const bool done = __all_sync(0xFFFFFFFFu, mbar_wait_bounded_idle(smem_u32(bar), parity, status));
+            const bool done = __all_sync(0xFFFFFFFFu, mbar_wait_bounded_tight(smem_u32(bar), parity, status));
             tc_fence_after();
             return done;
         };
@@ -320,20 +320,20 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         // ===== loader warp (the first kPfRaw blocks left in the prologue) =====
         int issued = min(kPfRaw, n_blocks);
         for (int blk = kPfRaw; blk < n_blocks; blk++) {
-            if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded_idle(smem_u32(&rawempty[blk % kPfRaw]), (uint32_t)((blk / kPfRaw - 1) & 1), status))) break;
+            if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded_tight(smem_u32(&rawempty[blk % kPfRaw]), (uint32_t)((blk / kPfRaw - 1) & 1), status))) break;
             load_block(blk, s_pages);
             issued = blk + 1;
         }
         // no copy of this CTA may be in flight when it returns, whatever became of the other roles
         for (int blk = max(0, issued - kPfRaw); blk < issued; blk++)
-            (void)__all_sync(0xFFFFFFFFu, mbar_wait_bounded_idle(smem_u32(&rawfull[blk % kPfRaw]), (uint32_t)((blk / kPfRaw) & 1), status));
+            (void)__all_sync(0xFFFFFFFFu, mbar_wait_bounded_tight(smem_u32(&rawfull[blk % kPfRaw]), (uint32_t)((blk / kPfRaw) & 1), status));
     }
     leave();
     if (warp == kPfMmaWarp) tmem_dealloc(tmem, kPfTmemCols); // tensor memory goes back on every path
     return;
     }
     if (warp >= kPfSoftWarps) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         // ===== expander warps: codes -> fp16 slabs =====
         const int et = tid - kPfSoftWarps * 32;
         const float sc2E = kLog2e / sqrtf((float)D) * (IO_BF16 && !wide ? pf_pow2i(e0) : 1.0f);
@@ -346,42 +346,42 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         const bool swap = D == 128 && ec >= 4;
         const uint32_t to = (uint32_t)((ec >> 2) * C::HALF + er * 128);
         const uint32_t to_lo = to + (((2 * (ec & 3) + (swap ? 1 : 0)) ^ (er & 7)) << 4), to_hi = to_lo ^ 16u;
-        auto expand = [&](const uint8_t* raw, int kv, uint8_t* slab) {
+        const uint32_t raw_u = smem_u32(s_raw), k_u = smem_u32(s_k), v_u = smem_u32(s_v), sc_u = smem_u32(s_sc);
+        auto expand = [&](uint32_t raw, int kv, uint32_t slab) {
 #pragma unroll
             for (int i = 0; i < kPfBlock / ROWS; i++) {
-                const uint4 w = *reinterpret_cast<const uint4*>(raw + from + i * (ROWS / kI8Page) * C::TILE + i8_row_off(D, kv, 0));
+                const uint4 w = lds128(raw + from + i * (ROWS / kI8Page) * C::TILE + i8_row_off(D, kv, 0));
                 const uint32_t a0 = swap ? w.z : w.x, a1 = swap ? w.w : w.y, b0 = swap ? w.x : w.z, b1 = swap ? w.y : w.w;
-                *reinterpret_cast<uint4*>(slab + to_lo + i * ROWS * 128) = make_uint4(pf_expand(a0, 0x4140), pf_expand(a0, 0x4342), pf_expand(a1, 0x4140), pf_expand(a1, 0x4342));
-                *reinterpret_cast<uint4*>(slab + to_hi + i * ROWS * 128) = make_uint4(pf_expand(b0, 0x4140), pf_expand(b0, 0x4342), pf_expand(b1, 0x4140), pf_expand(b1, 0x4342));
+                sts128(slab + to_lo + i * ROWS * 128, make_uint4(pf_expand(a0, 0x4140), pf_expand(a0, 0x4342), pf_expand(a1, 0x4140), pf_expand(a1, 0x4342)));
+                sts128(slab + to_hi + i * ROWS * 128, make_uint4(pf_expand(b0, 0x4140), pf_expand(b0, 0x4342), pf_expand(b1, 0x4140), pf_expand(b1, 0x4342)));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };
         auto expand_k = [&](int blk) {
             const int s = blk & 1, rs = blk % kPfRaw;
-            const uint8_t* raw = s_raw + rs * C::RAW;
-            if (!mbar_wait_bounded_idle(smem_u32(&rawfull[rs]), (uint32_t)((blk / kPfRaw) & 1), status)) return false;
-            if (blk >= 2 && !mbar_wait_bounded_idle(smem_u32(&kempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
-            expand(raw, 0, s_k + s * C::SLAB);
+            const uint32_t raw = raw_u + rs * C::RAW;
+            if (!mbar_wait_bounded_tight(smem_u32(&rawfull[rs]), (uint32_t)((blk / kPfRaw) & 1), status)) return false;
+            if (blk >= 2 && !mbar_wait_bounded_tight(smem_u32(&kempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
+            expand(raw, 0, k_u + s * C::SLAB);
             warp_arrive(&kfull[s]);
             if (et < kPfBlock) {
                 // (the numbers of block blk - 4 are out of use: S of block blk - 2, whose slab was just handed back, was
                 // issued after every row's W of block blk - 4)
-                const uint8_t* t = raw + (et / kI8Page) * C::TILE;
+                const uint32_t t = raw + (et / kI8Page) * C::TILE;
                 const bool in = t0 + blk * kPfBlock + et < t1;      // behind the range: whatever the page's last owner left
-                const float ks = *reinterpret_cast<const float*>(t + i8_scale_off(D, 0, et % kI8Page));
-                const float vs = *reinterpret_cast<const float*>(t + i8_scale_off(D, 1, et % kI8Page));
-                float* o = s_sc + (blk & 3) * 3 * kPfBlock + et;
-                o[0] = in ? ks * sc2E : 0.0f;
-                o[kPfBlock] = in ? pf_lg2(vs) : 0.0f;
-                o[2 * kPfBlock] = in ? __fdividef(1.0f, vs) : 0.0f;
+                const float ks = lds32(t + i8_scale_off(D, 0, et % kI8Page)), vs = lds32(t + i8_scale_off(D, 1, et % kI8Page));
+                const uint32_t o = sc_u + (((blk & 3) * 3 * kPfBlock + et) << 2);
+                sts32(o, in ? ks * sc2E : 0.0f);
+                sts32(o + 4 * kPfBlock, in ? pf_lg2(vs) : 0.0f);
+                sts32(o + 8 * kPfBlock, in ? __fdividef(1.0f, vs) : 0.0f);
                 warp_arrive(&scfull[blk & 3]);
             }
             return true;
         };
         auto expand_v = [&](int blk) {
             const int s = blk & 1, rs = blk % kPfRaw;
-            if (blk >= 2 && !mbar_wait_bounded_idle(smem_u32(&vempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
-            expand(s_raw + rs * C::RAW, 1, s_v + s * C::SLAB);
+            if (blk >= 2 && !mbar_wait_bounded_tight(smem_u32(&vempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
+            expand(raw_u + rs * C::RAW, 1, v_u + s * C::SLAB);
             warp_arrive(&vfull[s]);
             if (lane == 0) mbar_arrive(smem_u32(&rawempty[rs]));
             return true;
@@ -392,7 +392,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         leave();
         return;
     }
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
     if (warp < halves * (kPfSoftWarps / 2)) {
         // ===== softmax warps =====
         // A warp owns 16 rows (tensor-memory lanes; the two that share a 32-lane window, and a scheduler, take a half of it each),
@@ -423,9 +423,9 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             const int buf = blk & 1;
             const uint32_t col_s = base + 64u * buf;         // S of this block; its first 32 columns become W
             const int tok_base = t0 + blk * kPfBlock;
-            const float* sc = s_sc + (blk & 3) * 3 * kPfBlock + 2 * quad;
-            bool ok = mbar_wait_bounded(smem_u32(&scfull[blk & 3]), (uint32_t)((blk >> 2) & 1), status) &&
-                      mbar_wait_bounded(smem_u32(&bar_s[2 * half + buf]), (uint32_t)((blk >> 1) & 1), status);
+            const uint32_t sc = smem_u32(s_sc) + (((blk & 3) * 3 * kPfBlock + 2 * quad) << 2);
+            bool ok = mbar_wait_bounded_tight(smem_u32(&scfull[blk & 3]), (uint32_t)((blk >> 2) & 1), status) &&
+                      mbar_wait_bounded_tight(smem_u32(&bar_s[2 * half + buf]), (uint32_t)((blk >> 1) & 1), status);
             if (!__all_sync(0xFFFFFFFFu, ok)) { alive = false; break; }
             tc_fence_after();
             bool rescale = false;
@@ -437,17 +437,17 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                 int nv[2];                                   // of a row: tokens of the block it sees, from this thread's first column on
 #pragma unroll
                 for (int rr = 0; rr < 2; rr++) nv[rr] = min(lim[rr], end) - tok_base - 2 * quad;
-                uint32_t pr[16];                             // W of the rows as a 16x128b fragment
-                f32x2 tl[2];                                 // the block's share of the sums
                 // The weights of the block against the current references, 16 columns of S at a time, the next 16 on their way; S
-                // stays in tensor memory.  -> whether a score exceeds its row's reference by more than 2^kLazy.
-                auto weigh = [&](auto masked) -> bool {
+                // stays in tensor memory until W goes over it.  -> false, with nothing changed, where `check` is set and a score exceeds
+                // its row's reference by more than 2^kLazy.
+                auto weigh = [&](auto masked, bool check) -> bool {
                     constexpr bool M = decltype(masked)::value;
-                    f32x2 nm[2];
+                    uint32_t pr[16];                         // W of the rows as a 16x128b fragment
+                    f32x2 nm[2], tl[2];                      // tl: the block's share of the sums
                     float top = -1e30f;
 #pragma unroll
                     for (int rr = 0; rr < 2; rr++) { tl[rr] = 0ull; nm[rr] = pack_x2(-m2[rr], -m2[rr]); }
-                    uint32_t sr[2][8];
+                    f32x2 sr[2][4];
                     tmem_ld_frag16(col_s, sr[0]);
 #pragma unroll
                     for (int qt = 0; qt < 4; qt++) {
@@ -456,11 +456,10 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
 #pragma unroll
                         for (int k = 0; k < 2; k++) {        // tokens 16 qt + 8 k + 2 quad, +1
                             const int t = 16 * qt + 8 * k;
-                            const f32x2 ks = *reinterpret_cast<const f32x2*>(sc + t), lv = *reinterpret_cast<const f32x2*>(sc + kPfBlock + t),
-                                        iv = *reinterpret_cast<const f32x2*>(sc + 2 * kPfBlock + t);
+                            const f32x2 ks = lds64(sc + 4 * t), lv = lds64(sc + 4 * (kPfBlock + t)), iv = lds64(sc + 4 * (2 * kPfBlock + t));
 #pragma unroll
                             for (int rr = 0; rr < 2; rr++) {
-                                const f32x2 a = pack_x2(sr[qt & 1][4 * k + 2 * rr], sr[qt & 1][4 * k + 2 * rr + 1]);
+                                const f32x2 a = sr[qt & 1][2 * k + rr];
                                 const f32x2 u = add_x2(lv, nm[rr]);
                                 float2 x = unpack_x2(M ? fma_x2(mul_x2(a, ks), pack_x2(E[rr], E[rr]), u) : fma_x2(a, ks, u));
                                 if (M) {                     // (also where the scale of a token the row does not see is a NaN)
@@ -479,11 +478,15 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                             }
                         }
                     }
-                    return __any_sync(0xFFFFFFFFu, top > kLazy);
+                    if (__any_sync(0xFFFFFFFFu, top > kLazy) && check) return false;
+#pragma unroll
+                    for (int rr = 0; rr < 2; rr++) l2[rr] = add_x2(l2[rr], tl[rr]);
+                    tmem_st_half32(col_s, pr);               // W over the columns S was read from
+                    return true;
                 };
                 // speculating that the references stay; a row without one (its first block, or none of it seen so far) has to look first
                 bool look = !started;
-                if (!look) look = whole ? weigh(std::false_type{}) : weigh(std::true_type{});
+                if (!look) look = !(whole ? weigh(std::false_type{}, true) : weigh(std::true_type{}, true));
                 if (look) {                                  // new references for the rows that need one, then the weights
                     float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -494,7 +497,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             const int t = 32 * h + 8 * k;
-                            const f32x2 ks = *reinterpret_cast<const f32x2*>(sc + t), lv = *reinterpret_cast<const f32x2*>(sc + kPfBlock + t);
+                            const f32x2 ks = lds64(sc + 4 * t), lv = lds64(sc + 4 * (kPfBlock + t));
 #pragma unroll
                             for (int rr = 0; rr < 2; rr++) {
                                 const float2 x = unpack_x2(fma_x2(mul_x2(pack_x2(sf[4 * k + 2 * rr], sf[4 * k + 2 * rr + 1]), ks), pack_x2(E[rr], E[rr]), lv));
@@ -518,17 +521,14 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                     }
                     started = __all_sync(0xFFFFFFFFu, started);
                     rescale = __any_sync(0xFFFFFFFFu, rescale);
-                    (void)weigh(std::true_type{});
+                    (void)weigh(std::true_type{}, false);
                 }
-#pragma unroll
-                for (int rr = 0; rr < 2; rr++) l2[rr] = add_x2(l2[rr], tl[rr]);
-                tmem_st_half32(col_s, pr);                   // W over the columns S was read from
             }
             // O += W V of the previous block must be done before O is rescaled.  S of this block was committed behind W V of
             // block blk-2, so the barrier's phase is blk-1 or later; the last block waits in any case, so that the wait after
             // the loop cannot meet a barrier that is two phases away
             if (blk > 0 && (rescale || blk == n_blocks - 1)) {
-                if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(smem_u32(&bar_o[half]), (uint32_t)((blk - 1) & 1), status))) { alive = false; break; }
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded_tight(smem_u32(&bar_o[half]), (uint32_t)((blk - 1) & 1), status))) { alive = false; break; }
                 tc_fence_after();
                 if (rescale) {
 #pragma unroll
@@ -546,7 +546,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             tc_fence_before();
             warp_arrive(&p_ready[2 * half + buf]);           // these rows' W (and O) are ready for the tensor pipe
         }
-        if (alive && !__all_sync(0xFFFFFFFFu, mbar_wait_bounded(smem_u32(&bar_o[half]), (uint32_t)((n_blocks - 1) & 1), status))) alive = false;
+        if (alive && !__all_sync(0xFFFFFFFFu, mbar_wait_bounded_tight(smem_u32(&bar_o[half]), (uint32_t)((n_blocks - 1) & 1), status))) alive = false;
         tc_fence_after();
 
         const bool poisoned = __any_sync(0xFFFFFFFFu, !alive || __ldcg(status) != 0);   // fail closed, whole warps at a time

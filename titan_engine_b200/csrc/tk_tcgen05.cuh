@@ -101,9 +101,12 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 // Fragment shapes: 16 lanes (the address names the first: 0 or 16 of the warp's 32), a thread holds rows lane/4 and lane/4 + 8.
 //   16x256b, repeat k (8 columns): r[4k], r[4k+1] = columns 8k + 2 (lane%4), +1 of row lane/4; r[4k+2], r[4k+3] = the same of row + 8
 //   16x128b, repeat k (4 columns): r[2k] = column 4k + lane%4 of row lane/4; r[2k+1] = the same of row + 8
-__device__ __forceinline__ void tmem_ld_frag16(uint32_t taddr, uint32_t (&r)[8]) {          // 16 columns
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+// (16 columns as pairs: r[2k] = columns 8k + 2 (lane%4), +1 of row lane/4, r[2k+1] = the same of row + 8)
+__device__ __forceinline__ void tmem_ld_frag16(uint32_t taddr, unsigned long long (&r)[4]) {
+    asm volatile("{\n\t.reg .b32 t<8>;\n\t"
+        "tcgen05.ld.sync.aligned.16x256b.x2.b32 {t0, t1, t2, t3, t4, t5, t6, t7}, [%4];\n\t"
+        "mov.b64 %0, {t0, t1};\n\tmov.b64 %1, {t2, t3};\n\tmov.b64 %2, {t4, t5};\n\tmov.b64 %3, {t6, t7};\n\t}"
+        : "=l"(r[0]), "=l"(r[1]), "=l"(r[2]), "=l"(r[3])
         : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_ld_frag32(uint32_t taddr, uint32_t (&r)[16]) {         // 32 columns
@@ -119,9 +122,8 @@ __device__ __forceinline__ void tmem_st_half32(uint32_t taddr, const uint32_t (&
     asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
-__device__ __forceinline__ void tc_wait_ld_frag16(uint32_t (&r)[8]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]) :: "memory");
+__device__ __forceinline__ void tc_wait_ld_frag16(unsigned long long (&r)[4]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+l"(r[0]), "+l"(r[1]), "+l"(r[2]), "+l"(r[3]) :: "memory");
 }
 
 // Two FP32 lanes per instruction (sm_100): (a0, a1) * b + c and (s0, s1) += (p0, p1)
