@@ -120,10 +120,10 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     int32_t* s_pages = (int32_t*)(smem + C::OFF_PAGES);
     uint64_t* bars = (uint64_t*)(smem + C::OFF_BARS);
     uint64_t *rawfull = bars, *rawempty = bars + 4, *kfull = bars + 8, *kempty = bars + 10, *vfull = bars + 12, *vempty = bars + 14,
-             *scfull = bars + 16, *bar_s = bars + 20 /* [half][2] */, *p_ready = bars + 24 /* [half][2] */, *bar_o = bars + 28 /* [half] */;
-    uint32_t* s_tmem = (uint32_t*)(bars + 30);
+             *bar_s = bars + 16 /* [half][2] */, *p_ready = bars + 20 /* [half][2] */, *bar_o = bars + 24 /* [half] */;
+    uint32_t* s_tmem = (uint32_t*)(bars + 26);
     int* s_flag = (int*)(s_tmem + 1);
-    uint32_t* s_wmax = (uint32_t*)(bars + 32);              // [24 warps] prologue: largest query magnitude
+    uint32_t* s_wmax = (uint32_t*)(bars + 28);              // [24 warps] prologue: largest query magnitude
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = g.H / g.Hkv;
@@ -162,8 +162,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             mbar_init(smem_u32(&bar_o[i]), 1);
         }
         for (int i = 0; i < 4; i++) {
-            mbar_init(smem_u32(&scfull[i]), kPfBlock / 32);
-            mbar_init(smem_u32(&bar_s[i]), 1);
+            mbar_init(smem_u32(&bar_s[i]), 2);              // the commit of S and a plain arrival of its MMA warp
             mbar_init(smem_u32(&p_ready[i]), kPfSoftWarps / 2);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -282,6 +281,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                     tc_mma_ss(at + 64u * (blk & 1), dq + (uint64_t)(((ks >> 2) * (kTcRows * 128) + (ks & 3) * 32) >> 4),
                               dk + (uint64_t)(((ks >> 2) * C::HALF + (ks & 3) * 32) >> 4), kIdescS, ks > 0);
                 tc_commit(smem_u32(&bar_s[2 * half + (blk & 1)]));
+                mbar_arrive(smem_u32(&bar_s[2 * half + (blk & 1)]));     // passes on what kfull said: the numbers of the block's tokens are there
                 tc_commit(smem_u32(&kempty[blk & 1]));
             }
             __syncwarp();
@@ -362,8 +362,6 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             const uint32_t raw = raw_u + rs * C::RAW;
             if (!mbar_wait_bounded_tight(smem_u32(&rawfull[rs]), (uint32_t)((blk / kPfRaw) & 1), status)) return false;
             if (blk >= 2 && !mbar_wait_bounded_tight(smem_u32(&kempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
-            expand(raw, 0, k_u + s * C::SLAB);
-            warp_arrive(&kfull[s]);
             if (et < kPfBlock) {
                 // (the numbers of block blk - 4 are out of use: S of block blk - 2, whose slab was just handed back, was
                 // issued after every row's W of block blk - 4)
@@ -374,8 +372,9 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                 sts32(o, in ? ks * sc2E : 0.0f);
                 sts32(o + 4 * kPfBlock, in ? pf_lg2(vs) : 0.0f);
                 sts32(o + 8 * kPfBlock, in ? __fdividef(1.0f, vs) : 0.0f);
-                warp_arrive(&scfull[blk & 3]);
             }
+            expand(raw, 0, k_u + s * C::SLAB);
+            warp_arrive(&kfull[s]);
             return true;
         };
         auto expand_v = [&](int blk) {
@@ -404,18 +403,19 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         const int half = warp >> 3, quad = lane & 3;
         const int row0 = half * kTcRows + (warp & 3) * 32 + ((warp >> 2) & 1) * 16 + (lane >> 2);    // + 8 rr
         const uint32_t base = tmem + half * kPfHalfCols + ((uint32_t)((warp & 3) * 32 + ((warp >> 2) & 1) * 16) << 16);
-        float E[2], m2[2];                                   // per row: query's power of two, reference (base 2)
+        float m2[2];                                         // per row: reference (base 2)
         f32x2 l2[2];                                         // ... sums over this thread's even and odd columns
         int lim[2];                                          // positions the row sees
 #pragma unroll
         for (int rr = 0; rr < 2; rr++) {
             const int row = row0 + 8 * rr;
-            E[rr] = IO_BF16 && wide ? s_e[row] : 1.0f;
             m2[rr] = -1e30f;
             l2[rr] = 0ull;
             // (rows without a token: zero queries, nothing of theirs is written; unmasked, so that they cost no careful pass)
             lim[rr] = row / G < tok_cnt ? base_pos + tok_first + row / G + 1 : len;
         }
+        const uint32_t e_u = smem_u32(s_e) + 4 * row0;       // the rows' powers of two, 8 rows apart
+        auto power = [&](int rr) { const float e = IO_BF16 && wide ? lds32(e_u + 32 * rr) : 1.0f; return pack_x2(e, e); };
         const bool idle = (row0 - (lane >> 2)) / G >= tok_cnt;   // no row of this warp has a token: whatever W holds, nobody reads its O
         const int lim_min = min(lim[0], lim[1]);
         bool started = false;
@@ -424,8 +424,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             const uint32_t col_s = base + 64u * buf;         // S of this block; its first 32 columns become W
             const int tok_base = t0 + blk * kPfBlock;
             const uint32_t sc = smem_u32(s_sc) + (((blk & 3) * 3 * kPfBlock + 2 * quad) << 2);
-            bool ok = mbar_wait_bounded_tight(smem_u32(&scfull[blk & 3]), (uint32_t)((blk >> 2) & 1), status) &&
-                      mbar_wait_bounded_tight(smem_u32(&bar_s[2 * half + buf]), (uint32_t)((blk >> 1) & 1), status);
+            const bool ok = mbar_wait_bounded_tight(smem_u32(&bar_s[2 * half + buf]), (uint32_t)((blk >> 1) & 1), status);
             if (!__all_sync(0xFFFFFFFFu, ok)) { alive = false; break; }
             tc_fence_after();
             bool rescale = false;
@@ -447,6 +446,8 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                     float top = -1e30f;
 #pragma unroll
                     for (int rr = 0; rr < 2; rr++) { tl[rr] = 0ull; nm[rr] = pack_x2(-m2[rr], -m2[rr]); }
+                    f32x2 E[2];
+                    if (M) { E[0] = power(0); E[1] = power(1); }
                     f32x2 sr[2][4];
                     tmem_ld_frag16(col_s, sr[0]);
 #pragma unroll
@@ -461,7 +462,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                             for (int rr = 0; rr < 2; rr++) {
                                 const f32x2 a = sr[qt & 1][2 * k + rr];
                                 const f32x2 u = add_x2(lv, nm[rr]);
-                                float2 x = unpack_x2(M ? fma_x2(mul_x2(a, ks), pack_x2(E[rr], E[rr]), u) : fma_x2(a, ks, u));
+                                float2 x = unpack_x2(M ? fma_x2(mul_x2(a, ks), E[rr], u) : fma_x2(a, ks, u));
                                 if (M) {                     // (also where the scale of a token the row does not see is a NaN)
                                     x.x = t < nv[rr] ? x.x : -INFINITY;
                                     x.y = t + 1 < nv[rr] ? x.y : -INFINITY;
@@ -489,6 +490,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                 if (!look) look = !(whole ? weigh(std::false_type{}, true) : weigh(std::true_type{}, true));
                 if (look) {                                  // new references for the rows that need one, then the weights
                     float mx[2] = {-INFINITY, -INFINITY};
+                    const f32x2 E[2] = {power(0), power(1)};
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         uint32_t sf[16];
@@ -500,7 +502,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                             const f32x2 ks = lds64(sc + 4 * t), lv = lds64(sc + 4 * (kPfBlock + t));
 #pragma unroll
                             for (int rr = 0; rr < 2; rr++) {
-                                const float2 x = unpack_x2(fma_x2(mul_x2(pack_x2(sf[4 * k + 2 * rr], sf[4 * k + 2 * rr + 1]), ks), pack_x2(E[rr], E[rr]), lv));
+                                const float2 x = unpack_x2(fma_x2(mul_x2(pack_x2(sf[4 * k + 2 * rr], sf[4 * k + 2 * rr + 1]), ks), E[rr], lv));
                                 mx[rr] = fmaxf(mx[rr], t < nv[rr] ? x.x : -INFINITY);
                                 mx[rr] = fmaxf(mx[rr], t + 1 < nv[rr] ? x.y : -INFINITY);
                             }
