@@ -83,7 +83,7 @@ SIGNATURES = {
     "tk_kv_step_chunk_tokens": (C.c_int, [_P]),
     "tk_kv_step_prefill_plan": (C.c_int, [_P, C.c_int32, _I32P, _I32P, _I32P, _I32P]),
     "tk_kv_append": (C.c_int, [_P, C.c_int32, _P, _P, _P, _P]),
-    "tk_kv_read": (C.c_int, [_P, C.c_int32, C.c_int32, _I32P, _I32P, _I32P, _P, _P, C.c_int32, _P]),
+    "tk_kv_read": (C.c_int, [_P, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, C.c_int32, _P]),
     "tk_kv_decode": (C.c_int, [_P, C.c_int32, _P, _P, _P]),
     "tk_kv_append_decode": (C.c_int, [_P, C.c_int32, _P, _P, _P, _P, _P]),
     "tk_kv_rope_append_decode": (C.c_int, [_P, C.c_int32, _P, _P, _P, _P, C.c_float, C.c_float, _P]),

@@ -43,6 +43,16 @@ __device__ __forceinline__ uint32_t i8_code(float x, float to_code) {
     return __float_as_uint(__fadd_rn(snapped, 12582912.0f + 128.0f)) & 0xFFu;
 }
 
+// Two bytes of `w`, picked by SEL, -> two codes as fp16, exact: 1024 + u, minus 1152.
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t i8_expand(uint32_t w) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0x64646464u), "n"(SEL));
+    const uint32_t bias = 0x64806480u;
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&bias));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // Shared-memory accesses by 32-bit address (a pointer that went through a lambda or a conditional may be taken for a generic one)
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     uint4 v;

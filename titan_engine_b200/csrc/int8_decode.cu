@@ -24,14 +24,17 @@ namespace tk {
 
 namespace {
 
-constexpr int kI8Stages = 3, kI8MinCtas = 3;
 
-template <int D>
+// One column block (128 registers) leaves room for 4 CTAs per SM, two (168) for 3; the stages share out the shared memory.  Measured
+// at D = 128, one block: 2 stages x 4 CTAs 364 us, 3 x 3 377, 4 x 2 438 (32 sequences of 32768 tokens, 64 heads); two blocks: 3 x 3 168 us, 2 x 4 (spilling) 175 (64 sequences, 4 tokens each).
+template <int D, int NB>
 struct I8Cfg {
+    static constexpr int CTAS = NB == 1 ? 4 : 3;
+    static constexpr int STAGES = D == 64 ? 4 : NB == 1 ? 2 : 3;
     static constexpr int TILE = i8_tile_bytes(D);
     static constexpr int LINES = TILE / 128;                // the tile as lines of 128 bytes: one TMA box
     static constexpr int STAGE = (TILE + 1023) / 1024 * 1024;   // the 128-byte swizzle repeats every 1024 bytes
-    static constexpr int SMEM = kWarps * kI8Stages * STAGE + 1024 + 128;
+    static constexpr int SMEM = kWarps * STAGES * STAGE + 1024 + 256;
     static constexpr int SCALES = 2 * kI8Page * D;          // byte offset of the scale line; its line number is a multiple of 8: not swizzled
 };
 
@@ -42,14 +45,6 @@ __device__ __forceinline__ uint32_t i8_swz(int r, int c) {
     return (uint32_t)((r >> 1) * 128 + (((((r & 1) << 2) + c) ^ ((r >> 1) & 7)) << 4));
 }
 
-// bytes of `w` selected by `sel` (as the low bytes of two 16-bit lanes) -> two codes as fp16, exact: 1024 + u, minus 1152
-__device__ __forceinline__ uint32_t i8_expand(uint32_t w, uint32_t sel) {
-    uint32_t r;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0x64646464u), "r"(sel));
-    const uint32_t bias = 0x64806480u;
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&bias));
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ float lg2(float x) {
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -58,12 +53,12 @@ __device__ __forceinline__ float lg2(float x) {
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 template <int D, bool IO_BF16, int NB>
-__global__ void __launch_bounds__(kWarps * 32, kI8MinCtas)
+__global__ void __launch_bounds__(kWarps * 32, I8Cfg<D, NB>::CTAS)
 decode_int8_kernel(const __grid_constant__ CUtensorMap tmap, Geometry g, uint8_t* __restrict__ pool, StepDev st,
                    const int32_t* __restrict__ page_table, const uint16_t* __restrict__ q, float* __restrict__ partials,
                    int* __restrict__ status, MergeOut mo, FuseAppend fa, int multi) {
-    using C = I8Cfg<D>;
-    constexpr int KS = D / 16;
+    using C = I8Cfg<D, NB>;
+    constexpr int KS = D / 16, kI8Stages = C::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t* bars = (uint64_t*)(smem + kWarps * kI8Stages * C::STAGE);
@@ -222,8 +217,8 @@ decode_int8_kernel(const __grid_constant__ CUtensorMap tmap, Geometry g, uint8_t
             for (int cp = 0; cp < D / 32; cp++) {
                 uint32_t r0, r1, r2, r3;
                 ldsm_x4(stg_u + i8_swz<D>(row, 2 * cp + (mi >> 1)), r0, r1, r2, r3);
-                const uint32_t a0[4] = {i8_expand(r0, 0x4140), i8_expand(r1, 0x4140), i8_expand(r0, 0x4342), i8_expand(r1, 0x4342)};
-                const uint32_t a1[4] = {i8_expand(r2, 0x4140), i8_expand(r3, 0x4140), i8_expand(r2, 0x4342), i8_expand(r3, 0x4342)};
+                const uint32_t a0[4] = {i8_expand<0x4140>(r0), i8_expand<0x4140>(r1), i8_expand<0x4342>(r0), i8_expand<0x4342>(r1)};
+                const uint32_t a1[4] = {i8_expand<0x4140>(r2), i8_expand<0x4140>(r3), i8_expand<0x4342>(r2), i8_expand<0x4342>(r3)};
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++) {
                     mma16816<false>(sT[nb], a0, qb[nb][2 * cp][0], qb[nb][2 * cp][1]);
@@ -239,46 +234,51 @@ decode_int8_kernel(const __grid_constant__ CUtensorMap tmap, Geometry g, uint8_t
         }
         const float lv0 = lg2(vs0), lv1 = lg2(vs1), iv0 = __fdividef(1.0f, vs0), iv1 = __fdividef(1.0f, vs1);
         uint32_t bfr[NB][2];
+        float x[NB][4], xa[NB], xb[NB];
+        bool over = false;
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
-            float a0 = fmaf(sT[nb][0] + uT[nb][0], ks0 * f0[nb], lv0), a1 = fmaf(sT[nb][1] + uT[nb][1], ks0 * f1[nb], lv0);
-            float a2 = fmaf(sT[nb][2] + uT[nb][2], ks1 * f0[nb], lv1), a3 = fmaf(sT[nb][3] + uT[nb][3], ks1 * f1[nb], lv1);
+            x[nb][0] = fmaf(sT[nb][0] + uT[nb][0], ks0 * f0[nb], lv0); x[nb][1] = fmaf(sT[nb][1] + uT[nb][1], ks0 * f1[nb], lv0);
+            x[nb][2] = fmaf(sT[nb][2] + uT[nb][2], ks1 * f0[nb], lv1); x[nb][3] = fmaf(sT[nb][3] + uT[nb][3], ks1 * f1[nb], lv1);
             if (cut) {
                 const int p0 = tok_base + gr, p1 = p0 + 8;
-                if (p0 >= min(lim0[nb], t1)) a0 = -INFINITY;
-                if (p0 >= min(lim1[nb], t1)) a1 = -INFINITY;
-                if (p1 >= min(lim0[nb], t1)) a2 = -INFINITY;
-                if (p1 >= min(lim1[nb], t1)) a3 = -INFINITY;
+                if (p0 >= min(lim0[nb], t1)) x[nb][0] = -INFINITY;
+                if (p0 >= min(lim1[nb], t1)) x[nb][1] = -INFINITY;
+                if (p1 >= min(lim0[nb], t1)) x[nb][2] = -INFINITY;
+                if (p1 >= min(lim1[nb], t1)) x[nb][3] = -INFINITY;
             }
-            float xa = fmaxf(a0, a2), xb = fmaxf(a1, a3);
-            if (__any_sync(0xFFFFFFFFu, xa > m0[nb] + 4.0f || xb > m1[nb] + 4.0f)) {
+            xa[nb] = fmaxf(x[nb][0], x[nb][2]); xb[nb] = fmaxf(x[nb][1], x[nb][3]);
+            over = over || xa[nb] > m0[nb] + 4.0f || xb[nb] > m1[nb] + 4.0f;
+        }
+        if (__any_sync(0xFFFFFFFFu, over)) {                // new references, in all column blocks at once
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
                 for (int off = 4; off < 32; off <<= 1) {
-                    xa = fmaxf(xa, __shfl_xor_sync(0xFFFFFFFFu, xa, off));
-                    xb = fmaxf(xb, __shfl_xor_sync(0xFFFFFFFFu, xb, off));
+                    xa[nb] = fmaxf(xa[nb], __shfl_xor_sync(0xFFFFFFFFu, xa[nb], off));
+                    xb[nb] = fmaxf(xb[nb], __shfl_xor_sync(0xFFFFFFFFu, xb[nb], off));
                 }
-                const float na = fmaxf(m0[nb], xa), nc = fmaxf(m1[nb], xb);
+                const float na = fmaxf(m0[nb], xa[nb]), nc = fmaxf(m1[nb], xb[nb]);
                 const float al0 = ex2(m0[nb] - na), al1 = ex2(m1[nb] - nc);
                 l0[nb] *= al0; l1[nb] *= al1;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) { o[nb][nt][0] *= al0; o[nb][nt][2] *= al0; o[nb][nt][1] *= al1; o[nb][nt][3] *= al1; }
                 m0[nb] = na; m1[nb] = nc;
             }
-            float w0 = ex2(a0 - m0[nb]), w1 = ex2(a1 - m1[nb]), w2 = ex2(a2 - m0[nb]), w3 = ex2(a3 - m1[nb]);
-            if (cut) {                                      // a masked score's weight is 0 also where its token's scale is a NaN
-                if (a0 == -INFINITY) w0 = 0.0f;
-                if (a1 == -INFINITY) w1 = 0.0f;
-                if (a2 == -INFINITY) w2 = 0.0f;
-                if (a3 == -INFINITY) w3 = 0.0f;
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            const float w0 = ex2(x[nb][0] - m0[nb]), w1 = ex2(x[nb][1] - m1[nb]), w2 = ex2(x[nb][2] - m0[nb]), w3 = ex2(x[nb][3] - m1[nb]);
+            if (cut) {                                      // a masked weight counts nothing also where its token's scale is a NaN
                 l0[nb] += (w0 == 0.0f ? 0.0f : w0 * iv0) + (w2 == 0.0f ? 0.0f : w2 * iv1);
                 l1[nb] += (w1 == 0.0f ? 0.0f : w1 * iv0) + (w3 == 0.0f ? 0.0f : w3 * iv1);
             } else {
                 l0[nb] = fmaf(w0, iv0, fmaf(w2, iv1, l0[nb]));
                 l1[nb] = fmaf(w1, iv0, fmaf(w3, iv1, l1[nb]));
             }
-            const uint32_t x0 = pack2<false>(w0, w1), x1 = pack2<false>(w2, w3);     // W^T as the B operand: transposed below
-            asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(bfr[nb][0]) : "r"(x0));
-            asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(bfr[nb][1]) : "r"(x1));
+            const uint32_t c0 = pack2<false>(w0, w1), c1 = pack2<false>(w2, w3);     // W^T as the B operand: transposed below
+            asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(bfr[nb][0]) : "r"(c0));
+            asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(bfr[nb][1]) : "r"(c1));
         }
         // ---- O^T += V^T W^T ----
         {
@@ -287,8 +287,8 @@ decode_int8_kernel(const __grid_constant__ CUtensorMap tmap, Geometry g, uint8_t
             for (int cp = 0; cp < D / 32; cp++) {
                 uint32_t r0, r1, r2, r3;                    // bytes: (even dim, odd dim) of token 2j, the same of token 2j+1
                 ldsm_x4_t(stg_u + i8_swz<D>(row, 2 * cp + (mi >> 1)), r0, r1, r2, r3);
-                const uint32_t ae[4] = {i8_expand(r0, 0x4240), i8_expand(r2, 0x4240), i8_expand(r1, 0x4240), i8_expand(r3, 0x4240)};
-                const uint32_t ao[4] = {i8_expand(r0, 0x4341), i8_expand(r2, 0x4341), i8_expand(r1, 0x4341), i8_expand(r3, 0x4341)};
+                const uint32_t ae[4] = {i8_expand<0x4240>(r0), i8_expand<0x4240>(r2), i8_expand<0x4240>(r1), i8_expand<0x4240>(r3)};
+                const uint32_t ao[4] = {i8_expand<0x4341>(r0), i8_expand<0x4341>(r2), i8_expand<0x4341>(r1), i8_expand<0x4341>(r3)};
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++) {
                     mma16816<false>(o[nb][2 * cp], ae, bfr[nb][0], bfr[nb][1]);
@@ -334,34 +334,53 @@ decode_int8_kernel(const __grid_constant__ CUtensorMap tmap, Geometry g, uint8_t
             }
         }
     __syncthreads();
-    pdl_wait();
-    const int prow = st.chunk_base[b] + chunk;
-    const int heads_per_row = multi ? g.H * st.nq_max : g.H;
-    for (int idx = threadIdx.x; idx < rows * (D + 2); idx += blockDim.x) {
-        const int row = idx / (D + 2), d = idx % (D + 2);
+    // per row: the largest reference M, the factor 2^(m_w - M - k) of each warp's sums, and (m, l) of the row; l counts weights over
+    // value scales, which may be of any size: 2^-k brings it to [1, 2)
+    float* fac = red + kWarps * rows * (D + 2);             // [rows][kWarps + 2]
+    if (threadIdx.x < rows) {
+        const int row = threadIdx.x;
         float M = -1e30f, l = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWarps; w++) M = fmaxf(M, red_at(w, row, D));
 #pragma unroll
         for (int w = 0; w < kWarps; w++) l += red_at(w, row, D + 1) * ex2(red_at(w, row, D) - M);
-        // the row times 2^-k with l 2^-k in [1, 2): l counts weights over value scales, which may be of any size
         const uint32_t ex = (__float_as_uint(l) >> 23) & 0xFFu;
         const int k = ex == 0 || ex >= 254 ? 0 : (int)ex - 127;
-        float val;
-        if (d == D) {
-            val = l == 0.0f ? -1e30f : (M + (float)k) * 0.6931471805599453f;      // natural-log units, as split-KV rows carry it
-        } else {
-            val = l;
-            if (d < D) {
-                val = 0.0f;
 #pragma unroll
-                for (int w = 0; w < kWarps; w++) val += red_at(w, row, d) * ex2(red_at(w, row, D) - M);
-            }
-            val *= pow2i(-k);
-        }
-        partials[partial_off(prow, multi ? (row / G) * g.H + kvh * G + row % G : kvh * G + row, heads_per_row, D) + d] = val;
+        for (int w = 0; w < kWarps; w++) fac[row * (kWarps + 2) + w] = ex2(red_at(w, row, D) - M) * pow2i(-k);
+        fac[row * (kWarps + 2) + kWarps] = l == 0.0f ? -1e30f : (M + (float)k) * 0.6931471805599453f;    // natural-log units, as split-KV rows carry it
+        fac[row * (kWarps + 2) + kWarps + 1] = l * pow2i(-k);
     }
-    merge_if_last(g, st, mo, b, kvh, G, partials, s_flag, MergeMap{rows, heads_per_row, q_row0, 0, 0});
+    __syncthreads();
+    pdl_wait();
+    const int prow = st.chunk_base[b] + chunk;
+    const int heads_per_row = multi ? g.H * st.nq_max : g.H;
+    // the only chunk of its sequence: the result goes straight out (nothing is written while the status word is set)
+    const bool direct = mo.counters && mo.out && !mo.partial_out && !mo.peer && st.chunk_base[b + 1] - st.chunk_base[b] == 1;
+    if (direct && __ldcg(status) != 0) return;
+    for (int idx = threadIdx.x; idx < rows * (D / 2); idx += blockDim.x) {
+        const int row = idx / (D / 2), d = 2 * (idx % (D / 2));
+        const float* f = fac + row * (kWarps + 2);
+        float v0 = 0.0f, v1 = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            const float2 x = *reinterpret_cast<const float2*>(&red_at(w, row, d));
+            v0 += x.x * f[w];
+            v1 += x.y * f[w];
+        }
+        const int tok = multi ? row / G : 0, head = kvh * G + (multi ? row % G : row);
+        if (direct) {
+            const float inv = 1.0f / (f[kWarps + 1] + 1e-8f);
+            const size_t at = ((size_t)(q_row0 + tok) * g.H + head) * D + d;
+            if (mo.out_dtype == DT_FP32) *reinterpret_cast<float2*>((float*)mo.out + at) = make_float2(v0 * inv, v1 * inv);
+            else                         *reinterpret_cast<uint32_t*>((uint16_t*)mo.out + at) = pack2<IO_BF16>(v0 * inv, v1 * inv);
+        } else {
+            float* o_row = partials + partial_off(prow, tok * g.H + head, heads_per_row, D);
+            *reinterpret_cast<float2*>(o_row + d) = make_float2(v0, v1);
+            if (d == 0) *reinterpret_cast<float2*>(o_row + D) = make_float2(f[kWarps], f[kWarps + 1]);
+        }
+    }
+    if (!direct) merge_if_last(g, st, mo, b, kvh, G, partials, s_flag, MergeMap{rows, heads_per_row, q_row0, 0, 0});
 }
 
 template <int D, bool IO_BF16, int NB>
@@ -373,12 +392,12 @@ cudaError_t launch_one(const CUtensorMap* map, const Geometry& g, const LayerPtr
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, I8Cfg<D>::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (I8Cfg<D, NB>::SMEM));
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(st.n_items); cfg.blockDim = dim3(kWarps * 32); cfg.dynamicSmemBytes = I8Cfg<D>::SMEM; cfg.stream = s;
+    cfg.gridDim = dim3(st.n_items); cfg.blockDim = dim3(kWarps * 32); cfg.dynamicSmemBytes = (I8Cfg<D, NB>::SMEM); cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -53,13 +53,6 @@ struct PfCfg {
                          SMEM = OFF_BARS + 512 + 1024;
 };
 
-__device__ __forceinline__ uint32_t pf_expand(uint32_t w, uint32_t sel) {      // two codes as fp16, exact: 1024 + u, minus 1152
-    uint32_t r;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0x64646464u), "r"(sel));
-    const uint32_t bias = 0x64806480u;
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&bias));
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
 // two FP32 values in one 64-bit register
 typedef unsigned long long f32x2;
 __device__ __forceinline__ f32x2 pack_x2(float lo, float hi) {
@@ -347,13 +340,13 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         const uint32_t to = (uint32_t)((ec >> 2) * C::HALF + er * 128);
         const uint32_t to_lo = to + (((2 * (ec & 3) + (swap ? 1 : 0)) ^ (er & 7)) << 4), to_hi = to_lo ^ 16u;
         const uint32_t raw_u = smem_u32(s_raw), k_u = smem_u32(s_k), v_u = smem_u32(s_v), sc_u = smem_u32(s_sc);
-        auto expand = [&](uint32_t raw, int kv, uint32_t slab) {
+            auto expand = [&](uint32_t raw, int kv, uint32_t slab) {
 #pragma unroll
             for (int i = 0; i < kPfBlock / ROWS; i++) {
                 const uint4 w = lds128(raw + from + i * (ROWS / kI8Page) * C::TILE + i8_row_off(D, kv, 0));
                 const uint32_t a0 = swap ? w.z : w.x, a1 = swap ? w.w : w.y, b0 = swap ? w.x : w.z, b1 = swap ? w.y : w.w;
-                sts128(slab + to_lo + i * ROWS * 128, make_uint4(pf_expand(a0, 0x4140), pf_expand(a0, 0x4342), pf_expand(a1, 0x4140), pf_expand(a1, 0x4342)));
-                sts128(slab + to_hi + i * ROWS * 128, make_uint4(pf_expand(b0, 0x4140), pf_expand(b0, 0x4342), pf_expand(b1, 0x4140), pf_expand(b1, 0x4342)));
+                sts128(slab + to_lo + i * ROWS * 128, make_uint4(i8_expand<0x4140>(a0), i8_expand<0x4342>(a0), i8_expand<0x4140>(a1), i8_expand<0x4342>(a1)));
+                sts128(slab + to_hi + i * ROWS * 128, make_uint4(i8_expand<0x4140>(b0), i8_expand<0x4342>(b0), i8_expand<0x4140>(b1), i8_expand<0x4342>(b1)));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         };

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import weakref
+from array import array
 from typing import Optional, Sequence
 
 import numpy as np
@@ -35,6 +36,15 @@ def _i32(a) -> np.ndarray:
 
 def _ptr(a: Optional[np.ndarray]):
     return None if a is None else a.ctypes.data_as(C.POINTER(C.c_int32))
+
+
+def _ints(a):
+    """Sequence of integers -> (int32 buffer, its address): what the C calls on a step's path are handed."""
+    if isinstance(a, np.ndarray):
+        a = np.ascontiguousarray(a, dtype=np.int32)
+        return a, a.ctypes.data
+    a = array("i", a)
+    return a, a.buffer_info()[0]
 
 
 class PagedKVCache:
@@ -99,7 +109,7 @@ class PagedKVCache:
             raise KvError(st, self._lib.tk_kv_last_error(self._h).decode())
 
     def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
 
     def close(self) -> None:
         if getattr(self, "_h", None) and self._h.value:
@@ -243,28 +253,26 @@ class PagedKVCache:
         """K and V rows of tokens start[i] .. start[i] + count[i] - 1 of seq_ids[i], one range after the other:
         -> (k [rows, Hkv, D], v [rows, Hkv, Dv]) in the io dtype or torch.float32, 8-bit storage dequantised.
         start None: from 0; count None: up to each sequence's length."""
-        s = _i32(seq_ids)
-        a = np.zeros(len(s), dtype=np.int32) if start is None else _i32(start)
-        if count is None:
-            n = np.array([self.seq_len(int(x)) for x in s], dtype=np.int32)
-            n = n - a if len(a) == len(s) else n
-        else:
-            n = _i32(count)
-        if len(a) != len(s) or len(n) != len(s):
-            raise KvError(L.TK_INVALID_ARG, "read: start and count need one entry for each sequence")
-        if out_dtype is None:
-            out_dtype = self.io_torch_dtype
-        if out_dtype not in (self.io_torch_dtype, torch.float32):
-            raise KvError(L.TK_INVALID_ARG, f"read: out dtype must be {self.io_torch_dtype} or torch.float32")
         if self.host_only:
             raise KvError(L.TK_CUDA_ERROR, "read: handle has no device (bookkeeping only)")
-        if n.size and (n.min() < 0 or n.max() > self.cfg.num_pages * self.cfg.page_size):
+        if out_dtype is None:
+            out_dtype = self.io_torch_dtype
+        elif out_dtype not in (self.io_torch_dtype, torch.float32):
+            raise KvError(L.TK_INVALID_ARG, f"read: out dtype must be {self.io_torch_dtype} or torch.float32")
+        if start is None:
+            start = [0] * len(seq_ids)
+        if count is None:
+            count = [self.seq_len(int(s)) - int(a) for s, a in zip(seq_ids, start)]
+        if not len(seq_ids) == len(start) == len(count):
+            raise KvError(L.TK_INVALID_ARG, "read: start and count need one entry for each sequence")
+        rows, cfg = int(sum(count)), self.cfg
+        if rows and not 0 <= min(count) <= max(count) <= cfg.num_pages * cfg.page_size:
             raise KvError(L.TK_INVALID_ARG, "read: ranges must lie inside live sequences' tokens")
-        rows = int(n.sum(dtype=np.int64))
-        k = torch.empty(rows, self.cfg.num_kv_heads, self.cfg.head_dim, dtype=out_dtype, device=self.device)
-        v = torch.empty(rows, self.cfg.num_kv_heads, self.cfg.v_head_dim, dtype=out_dtype, device=self.device)
-        self._check(self._lib.tk_kv_read(self._h, layer, len(s), _ptr(s), _ptr(a), _ptr(n), k.data_ptr(), v.data_ptr(),
-                                         L.TK_FP32 if out_dtype == torch.float32 else self.cfg.io_dtype, self._stream()))
+        (s, s_at), (a, a_at), (n, n_at) = _ints(seq_ids), _ints(start), _ints(count)
+        k = torch.empty(rows, cfg.num_kv_heads, cfg.head_dim, dtype=out_dtype, device=self.device)
+        v = torch.empty(rows, cfg.num_kv_heads, cfg.v_head_dim, dtype=out_dtype, device=self.device)
+        self._check(self._lib.tk_kv_read(self._h, layer, len(s), s_at, a_at, n_at, k.data_ptr(), v.data_ptr(),
+                                         L.TK_FP32 if out_dtype == torch.float32 else cfg.io_dtype, self._stream()))
         return k, v
 
     def decode(self, layer: int, q: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
