@@ -38,6 +38,8 @@ struct I8Cfg {
     static constexpr int SCALES = 2 * kI8Page * D;          // byte offset of the scale line; its line number is a multiple of 8: not swizzled
 };
 
+constexpr int kMergeCells = 3000;           // (row, chunk) pairs whose (m, l) fit the shared memory of the smallest configuration
+
 // byte offset inside a stage of 16-byte chunk c of code row r (K rows 0-15, V rows 16-31), under the swizzle
 template <int D>
 __device__ __forceinline__ uint32_t i8_swz(int r, int c) {
@@ -322,10 +324,8 @@ decode_int8_kernel(const __grid_constant__ CUtensorMap tmap, Geometry g, uint8_t
             if (row < rows) {
 #pragma unroll
                 for (int c = 0; c < D / 32; c++) {
-                    red_at(warp, row, 32 * c + 2 * gr + 0) = o[nb][2 * c][hh];
-                    red_at(warp, row, 32 * c + 2 * gr + 1) = o[nb][2 * c + 1][hh];
-                    red_at(warp, row, 32 * c + 16 + 2 * gr + 0) = o[nb][2 * c][2 + hh];
-                    red_at(warp, row, 32 * c + 16 + 2 * gr + 1) = o[nb][2 * c + 1][2 + hh];
+                    *reinterpret_cast<float2*>(&red_at(warp, row, 32 * c + 2 * gr)) = make_float2(o[nb][2 * c][hh], o[nb][2 * c + 1][hh]);
+                    *reinterpret_cast<float2*>(&red_at(warp, row, 32 * c + 16 + 2 * gr)) = make_float2(o[nb][2 * c][2 + hh], o[nb][2 * c + 1][2 + hh]);
                 }
                 if (gr == 0) {
                     red_at(warp, row, D) = hh ? m1[nb] : m0[nb];
@@ -380,7 +380,96 @@ decode_int8_kernel(const __grid_constant__ CUtensorMap tmap, Geometry g, uint8_t
             if (d == 0) *reinterpret_cast<float2*>(o_row + D) = make_float2(f[kWarps], f[kWarps + 1]);
         }
     }
-    if (!direct) merge_if_last(g, st, mo, b, kvh, G, partials, s_flag, MergeMap{rows, heads_per_row, q_row0, 0, 0});
+    if (direct || !mo.counters) return;
+
+    // The CTA that arrives last for (b, kvh) merges the sequence's chunks.
+    const int r0 = st.chunk_base[b], n = st.chunk_base[b + 1] - r0;
+    if (mo.partial_out || mo.peer || rows * n > kMergeCells) {
+        merge_if_last(g, st, mo, b, kvh, G, partials, s_flag, MergeMap{rows, heads_per_row, q_row0, 0, 0});
+        return;
+    }
+    // The same merge (tk_merge.cuh) for all rows of the group at once, the first chunks' rows on their way while the weights are
+    // computed: a row after the other, 16 rows were four rounds of a chain of L2 loads per warp - 11 us at the end of the
+    // launch, where nothing else runs.
+    __syncthreads();                                        // the CTA's partial rows are complete ...
+    if (threadIdx.x == 0) {
+        __threadfence();                                    // ... and ordered before the ticket, device-wide
+        int* c = mo.counters + (size_t)b * g.Hkv + kvh;
+        const int last = atomicAdd(c, 1) == n - 1;
+        if (last) *c = 0;
+        *s_flag = last;
+    }
+    __syncthreads();
+    if (!*s_flag) return;
+    __threadfence();
+    if (__ldcg(status) != 0) return;
+    constexpr int U = 8 * NB * (D / 2) / (kWarps * 32), R = 32 / U;     // pairs of columns per thread, chunks in flight together
+    const float* col[U];                                    // this thread's columns in the first chunk's row
+    const size_t chunk_stride = (size_t)heads_per_row * (D + 2);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int idx = u * kWarps * 32 + threadIdx.x, row = min(idx / (D / 2), rows - 1);
+        col[u] = partials + partial_off(r0, (multi ? (row / G) * g.H + row % G : row) + kvh * G, heads_per_row, D) + 2 * (idx % (D / 2));
+    }
+    float2 x[R][U];
+    auto fetch = [&](int rb) {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                x[r][u] = rb + r < n ? __ldcg(reinterpret_cast<const float2*>(col[u] + (rb + r) * chunk_stride)) : make_float2(0.0f, 0.0f);
+    };
+    fetch(0);
+    float2* ml = reinterpret_cast<float2*>(smem);           // [rows][n] (m, l), then (weight, l)
+    float* s_inv = reinterpret_cast<float*>(ml + rows * n);
+    {
+        const int row = threadIdx.x >> 3, t = threadIdx.x & 7;      // eight threads per row
+        const bool on = row < rows;
+        const float* at = partials + partial_off(r0, (multi ? (min(row, rows - 1) / G) * g.H + min(row, rows - 1) % G : min(row, rows - 1)) + kvh * G, heads_per_row, D) + D;
+        float M = -1e30f, L = 0.0f;
+        for (int r = t; on && r < n; r += 8) {
+            const float2 c = __ldcg(reinterpret_cast<const float2*>(at + r * chunk_stride));
+            ml[row * n + r] = c;
+            M = fmaxf(M, c.x);
+        }
+#pragma unroll
+        for (int off = 4; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, off));
+        for (int r = t; on && r < n; r += 8) {              // (this thread's own entries)
+            float2& c = ml[row * n + r];
+            c.x = expf(c.x - M);
+            L += c.y * c.x;
+        }
+#pragma unroll
+        for (int off = 4; off > 0; off >>= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, off);
+        if (on && t == 0) s_inv[row] = 1.0f / (L + 1e-8f);
+    }
+    __syncthreads();
+    float2 acc[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) acc[u] = make_float2(0.0f, 0.0f);
+    for (int rb = 0; rb < n; rb += R) {
+        if (rb > 0) fetch(rb);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            if (rb + r >= n) break;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int row = min((u * kWarps * 32 + (int)threadIdx.x) / (D / 2), rows - 1);
+                const float w = ml[row * n + rb + r].x;
+                acc[u].x += x[r][u].x * w;
+                acc[u].y += x[r][u].y * w;
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int idx = u * kWarps * 32 + threadIdx.x, row = idx / (D / 2), d = 2 * (idx % (D / 2));
+        if (row >= rows) break;
+        const float inv = s_inv[row];
+        const size_t at = ((size_t)(q_row0 + (multi ? row / G : 0)) * g.H + kvh * G + (multi ? row % G : row)) * D + d;
+        if (mo.out_dtype == DT_FP32) *reinterpret_cast<float2*>((float*)mo.out + at) = make_float2(acc[u].x * inv, acc[u].y * inv);
+        else                         *reinterpret_cast<uint32_t*>((uint16_t*)mo.out + at) = pack2<IO_BF16>(acc[u].x * inv, acc[u].y * inv);
+    }
 }
 
 template <int D, bool IO_BF16, int NB>
