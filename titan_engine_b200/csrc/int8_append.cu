@@ -11,6 +11,7 @@ namespace tk {
 namespace {
 
 constexpr int kI8AppendThreads = 256;
+constexpr int kI8InFlight = 4;         // rows a thread has in flight
 
 // D / 8 lanes hold a row (8 values each); a row's K and V are separate rows here: unit u = (token, K|V, kv head).
 template <bool BF16, int D>
@@ -19,26 +20,38 @@ append_int8_kernel(Geometry g, uint8_t* __restrict__ pool, StepDev st, const int
                    const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int64_t* __restrict__ slots_out) {
     constexpr int LANES = D / 8, ROWS = kI8AppendThreads / LANES;
     const int c = threadIdx.x % LANES;
-    const long long u = (long long)blockIdx.x * ROWS + threadIdx.x / LANES;
-    const int per_tok = 2 * g.Hkv;
-    const bool live = u < (long long)st.n_tokens * per_tok;
-    const int t = live ? (int)(u / per_tok) : 0, rem = live ? (int)(u % per_tok) : 0;
-    const int kv = rem >= g.Hkv, h = kv ? rem - g.Hkv : rem;
-    const uint4 x = live ? *reinterpret_cast<const uint4*>((kv ? v : k) + ((size_t)t * g.Hkv + h) * D + c * 8) : make_uint4(0, 0, 0, 0);
-    uint32_t m = i8_absmax8(x);
+    const uint32_t per_tok = 2 * g.Hkv, n = (uint32_t)st.n_tokens * per_tok;     // (rows of a step fit the GPU's memory: below 2^31)
+    const uint32_t u0 = blockIdx.x * (ROWS * kI8InFlight) + threadIdx.x / LANES;
+    uint4 x[kI8InFlight];
+    int slot[kI8InFlight];
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    if (!live) return;
-    const I8Row row = i8_row(i8_amax_value<BF16>(m));
-    const int slot = st.tok_dst[t];
-    uint8_t* tile = pool + ((size_t)(slot / kI8Page) * g.Hkv + h) * i8_tile_bytes(D);
-    const int r = slot % kI8Page;
-    *reinterpret_cast<uint2*>(tile + i8_row_off(D, kv, r) + c * 8) = i8_codes8<BF16>(x, row.to_code);
-    if (c == 0) {
-        *reinterpret_cast<float*>(tile + i8_scale_off(D, kv, r)) = row.scale;
-        if (slots_out && rem == 0) {
-            const int pos = st.tok_pos[t];
-            slots_out[t] = (int64_t)page_table[(size_t)st.seq[st.tok_b[t]] * g.max_pages_per_seq + pos / kI8Page] * kI8Page + pos % kI8Page;
+    for (int i = 0; i < kI8InFlight; i++) {
+        const uint32_t u = u0 + i * ROWS;
+        x[i] = make_uint4(0, 0, 0, 0);
+        slot[i] = -1;
+        if (u < n) {
+            const uint32_t t = u / per_tok, rem = u % per_tok, kv = rem >= (uint32_t)g.Hkv, h = kv ? rem - g.Hkv : rem;
+            x[i] = *reinterpret_cast<const uint4*>((kv ? v : k) + ((size_t)t * g.Hkv + h) * D + c * 8);
+            slot[i] = st.tok_dst[t];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kI8InFlight; i++) {
+        uint32_t m = i8_absmax8(x[i]);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        if (slot[i] < 0) continue;
+        const uint32_t u = u0 + i * ROWS, t = u / per_tok, rem = u % per_tok, kv = rem >= (uint32_t)g.Hkv, h = kv ? rem - g.Hkv : rem;
+        const I8Row row = i8_row(i8_amax_value<BF16>(m));
+        uint8_t* tile = pool + ((size_t)(slot[i] / kI8Page) * g.Hkv + h) * i8_tile_bytes(D);
+        const int r = slot[i] % kI8Page;
+        *reinterpret_cast<uint2*>(tile + i8_row_off(D, kv, r) + c * 8) = i8_codes8<BF16>(x[i], row.to_code);
+        if (c == 0) {
+            *reinterpret_cast<float*>(tile + i8_scale_off(D, kv, r)) = row.scale;
+            if (slots_out && rem == 0) {
+                const int pos = st.tok_pos[t];
+                slots_out[t] = (int64_t)page_table[(size_t)st.seq[st.tok_b[t]] * g.max_pages_per_seq + pos / kI8Page] * kI8Page + pos % kI8Page;
+            }
         }
     }
 }
@@ -46,7 +59,7 @@ append_int8_kernel(Geometry g, uint8_t* __restrict__ pool, StepDev st, const int
 template <bool BF16, int D>
 cudaError_t launch_d(const Geometry& g, const LayerPtrs& lp, const StepDev& st, const int32_t* page_table, const void* k,
                      const void* v, int64_t* slots_out, cudaStream_t s) {
-    constexpr int ROWS = kI8AppendThreads / (D / 8);
+    constexpr int ROWS = kI8AppendThreads / (D / 8) * kI8InFlight;
     const long long units = (long long)st.n_tokens * 2 * g.Hkv;
     append_int8_kernel<BF16, D><<<(unsigned)((units + ROWS - 1) / ROWS), kI8AppendThreads, 0, s>>>(
         g, (uint8_t*)lp.pool, st, page_table, (const uint16_t*)k, (const uint16_t*)v, slots_out);
