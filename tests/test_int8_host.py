@@ -15,23 +15,45 @@ def _cache(**kw):
     return PagedKVCache(**args)
 
 
-def test_code_rounding_is_exact_for_every_pair_of_significands():
-    """The kernel's float32 steps (one product with the rounded 127/amax, the snap to 22 significant bits, one addition of a constant) against integer
-    arithmetic, for every value / amax of 11-bit significands and every exponent gap at which a code is not 0."""
+@pytest.mark.parametrize("off", [-1, 0, 1])
+def test_code_rounding_is_exact_for_every_pair_of_significands(off):
+    """The kernel's float32 steps (a product with 127 times a reciprocal that may be one unit in the last place off, the snap to
+    20 significant bits, one addition of a constant) against integer arithmetic, for every value / amax of 11-bit significands
+    and every exponent gap at which a code is not 0."""
     f32 = np.float32
     b = np.arange(1024, 2048, dtype=np.int64)[:, None]                     # amax = b
-    to_code = (f32(127.0) / b.astype(f32)).astype(f32)
+    inv = ((f32(1.0) / b.astype(f32)).view(np.int32) + off).view(f32)
+    to_code = f32(127.0) * inv
     for gap in range(0, 10):
         a = np.arange(1024, 2048, dtype=np.int64)[None, :]                 # x = a / 2^gap <= amax
-        x = a.astype(f32) / f32(2.0 ** gap)
-        y = np.clip((x * to_code).astype(f32), f32(-127), f32(127))
-        snapped = ((y.view(np.uint32) + np.uint32(2)) & np.uint32(0xFFFFFFFC)).view(f32)
+        y = (a.astype(f32) / f32(2.0 ** gap)) * to_code
+        snapped = ((y.view(np.uint32) + np.uint32(8)) & np.uint32(0xFFFFFFF0)).view(f32)
         got = (snapped + f32(12582912.0 + 128.0)).astype(f32).view(np.uint32).astype(np.int64) & 0xFF
         num, den = 2 * 127 * a, 2 * b * 2 ** gap                            # 127 x / amax = num / den
         q, rem = (num + den // 2) // den, (num + den // 2) % den
         want = np.where((rem == 0) & (q % 2 == 1), q - 1, q)                # a tie went up: take the even neighbour
-        ok = (x <= b)
+        ok = a <= b * 2 ** gap
         assert (np.broadcast_to(got - 128, ok.shape)[ok] == want[ok]).all(), gap
+
+
+def test_scale_is_the_rounded_quotient_for_every_significand():
+    """amax * fl(1/127) and one residual step, in exact arithmetic rounded as the fused operations round, = fl(amax / 127)."""
+    from fractions import Fraction
+
+    def rn(x):                                                              # nearest float32 of a positive fraction
+        e = 0
+        while x >= 2 ** 24: x /= 2; e += 1
+        while x < 2 ** 23: x *= 2; e -= 1
+        n = x.numerator // x.denominator
+        r = x - n
+        n += r > Fraction(1, 2) or (r == Fraction(1, 2) and n % 2 == 1)
+        return Fraction(n) * Fraction(2) ** e
+
+    k127 = rn(Fraction(1, 127))
+    for a in range(1024, 2049):
+        q = rn(a * k127)
+        r = a - q * 127                                                     # exact: far fewer than 24 significant bits
+        assert rn(r * k127 + q) == rn(Fraction(a, 127))
 
 
 def test_plain_rounding_of_ties_zeros_and_extremes():

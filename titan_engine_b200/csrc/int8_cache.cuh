@@ -22,25 +22,34 @@ __host__ __device__ constexpr int i8_tile_bytes(int D) { return 2 * kI8Page * D 
 __host__ __device__ constexpr int i8_row_off(int D, int kv, int r) { return (kv * kI8Page + r) * D; }
 __host__ __device__ constexpr int i8_scale_off(int D, int kv, int r) { return 2 * kI8Page * D + (kv * kI8Page + r) * (int)sizeof(float); }
 
-// What a row's largest magnitude makes of it: `to_code` = 127 / amax and the scale amax / 127, both single IEEE divisions.
-// A NaN among the values makes the scale NaN, so that the row reads as NaN; infinities saturate like any large value.
+// What a row's largest magnitude makes of it: `to_code`, 127 / amax to four parts in 2^24, and the scale, amax / 127 rounded to
+// nearest (amax has at most 11 significant bits: a product with the rounded 1/127 and one residual step give the
+// quotient's nearest float, checked for every significand).  A NaN among the values makes the scale NaN, so that the row reads
+// as NaN; infinities saturate like any large value.
 struct I8Row { float to_code, scale; };
 __device__ __forceinline__ I8Row i8_row(float amax) {
     const float a = fminf(fmaxf(amax, kI8AmaxMin), kI8AmaxMax);           // (a NaN becomes the minimum here)
-    return I8Row{__fdiv_rn(127.0f, a), amax != amax ? amax : __fdiv_rn(a, 127.0f)};
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(a));               // within one unit in the last place
+    constexpr float k127 = 1.0f / 127.0f;
+    const float q = a * k127;
+    return I8Row{127.0f * inv, amax != amax ? amax : fmaf(fmaf(-q, 127.0f, a), k127, q)};
 }
 
-// code + 128 in the low byte: the integer nearest to 127 x / amax, ties to even, EXACTLY.
+// code + 128 in the low byte of the result: the integer nearest to 127 x / amax, ties to even, EXACTLY.
 // x and amax have at most 11 significant bits, A and B: the quotient Q = 127 x / amax is 127 A 2^-n / B for some n, so it is a
-// half-integer or at least 1 / (2 B 2^n) = Q / (254 A) > Q 2^-19 away from every one.  y = x * fl(127 / amax) has two
-// roundings of 2^-24 relative: less than two units in the last place (ulp) from Q.  Snapped to a multiple of 4 ulps (22
-// significant bits, half-integers among them) y is the half-integer itself where Q is one, and otherwise within 4 ulps
-// of a Q that is at least 16 ulps from it: on the right side.  The addition of a constant whose neighbours are 1 apart then
-// rounds to the nearest integer, ties to even.  Checked against exact arithmetic for every pair of significands.
+// half-integer or at least 1 / (2 B 2^n) = Q / (254 A) > Q 2^-19 away from every one: 16 units in the last place (ulp) of Q.
+// y = x to_code has relative errors of 2^-23 (the reciprocal) and twice 2^-24 (two products): less than 4 ulps.  Snapped
+// to a multiple of 16 ulps (20 significant bits, half-integers among them) y is the half-integer itself where Q is one, and
+// otherwise within 12 ulps of a Q that is at least 16 ulps from it: on the right side.  The addition of a constant whose
+// neighbours are 1 apart then rounds to the nearest integer, ties to even.  Checked against exact arithmetic for every pair of
+// significands.  CLAMP: amax may have been cut to 2^64.
+template <bool CLAMP>
 __device__ __forceinline__ uint32_t i8_code(float x, float to_code) {
-    const float y = fminf(fmaxf(x * to_code, -127.0f), 127.0f);
-    const float snapped = __uint_as_float((__float_as_uint(y) + 2u) & ~3u);
-    return __float_as_uint(__fadd_rn(snapped, 12582912.0f + 128.0f)) & 0xFFu;
+    float y = x * to_code;
+    if (CLAMP) y = fminf(fmaxf(y, -127.0f), 127.0f);
+    const float snapped = __uint_as_float((__float_as_uint(y) + 8u) & ~15u);
+    return __float_as_uint(__fadd_rn(snapped, 12582912.0f + 128.0f));
 }
 
 // Two bytes of `w`, picked by SEL, -> two codes as fp16, exact: 1024 + u, minus 1152.
@@ -85,17 +94,16 @@ __device__ __forceinline__ float2 i8_unpack2(uint32_t w) {
 }
 
 // Eight 16-bit values (16 bytes) -> eight codes (8 bytes).
-template <bool BF16>
+template <bool BF16, bool CLAMP>
 __device__ __forceinline__ uint2 i8_codes8(const uint4& x, float to_code) {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    uint32_t c[8];
+    uint32_t c[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float2 f = i8_unpack2<BF16>(w[i]);
-        c[2 * i] = i8_code(f.x, to_code);
-        c[2 * i + 1] = i8_code(f.y, to_code);
+        c[i] = __byte_perm(i8_code<CLAMP>(f.x, to_code), i8_code<CLAMP>(f.y, to_code), 0x0040);
     }
-    return make_uint2(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24, c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24);
+    return make_uint2(__byte_perm(c[0], c[1], 0x5410), __byte_perm(c[2], c[3], 0x5410));
 }
 
 // Largest magnitude of eight 16-bit values, as the 16-bit pattern without its sign: patterns order like the magnitudes, and

@@ -191,7 +191,7 @@ decode_int8_kernel(const __grid_constant__ CUtensorMap tmap, Geometry g, uint8_t
 #pragma unroll
             for (int off = L8 / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
             const I8Row row = i8_row(i8_amax_value<IO_BF16>(m));
-            const uint2 codes = i8_codes8<IO_BF16>(x, row.to_code);
+            const uint2 codes = i8_codes8<IO_BF16, true>(x, row.to_code);
             if (lane < 2 * L8) {
                 uint8_t* tile = pool + ((size_t)page * g.Hkv + kvh) * C::TILE;
                 *reinterpret_cast<uint2*>(stg + i8_swz<D>(kv * kPage + r, c >> 1) + 8 * (c & 1)) = codes;
