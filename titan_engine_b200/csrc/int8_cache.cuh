@@ -23,8 +23,8 @@ __host__ __device__ constexpr int i8_row_off(int D, int kv, int r) { return (kv 
 __host__ __device__ constexpr int i8_scale_off(int D, int kv, int r) { return 2 * kI8Page * D + (kv * kI8Page + r) * (int)sizeof(float); }
 
 // What a row's largest magnitude makes of it: `to_code`, 127 / amax to four parts in 2^24, and the scale, amax / 127 rounded to
-// nearest (amax has at most 11 significant bits: a product with the rounded 1/127 and one residual step give the
-// quotient's nearest float, checked for every significand).  A NaN among the values makes the scale NaN, so that the row reads
+// nearest (amax has at most 11 significant bits: a product with the rounded 1/127 and one residual step, Markstein's
+// correction, give the quotient's nearest float, checked for every significand).  A NaN among the values makes the scale NaN, so that the row reads
 // as NaN; infinities saturate like any large value.
 struct I8Row { float to_code, scale; };
 __device__ __forceinline__ I8Row i8_row(float amax) {
