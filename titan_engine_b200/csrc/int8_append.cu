@@ -11,10 +11,9 @@ namespace tk {
 namespace {
 
 constexpr int kI8AppendThreads = 256;
-constexpr int kI8InFlight = 2;         // rows a thread has in flight
+constexpr int kI8Vec = 4;              // 16-byte vectors of a row per lane
 
-// u / d for u < 2^31 as a product (Granlund and Montgomery's division by invariant integers): (mul_hi(u, m) + u) >> s.  (A division per row of eight values a thread would be a tenth of the
-// kernel's instructions.)
+// u / d for u < 2^31 as a product (Granlund and Montgomery's division by invariant integers): (mul_hi(u, m) + u) >> s.
 struct Divisor {
     uint32_t d, m;
     int s;
@@ -26,53 +25,50 @@ Divisor divisor(uint32_t d) {
     return Divisor{d, (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
 }
 
-// D / 16 lanes hold a row, a lane eight values of each half of it; a row's K and V are separate rows here: unit u = (token,
+// D / 32 lanes hold a row, a lane eight values of each quarter of it; a row's K and V are separate rows here: unit u = (token,
 // K|V, kv head).  The kernel is bound by issue slots as much as by HBM: what is done once per row and lane (addresses, the
-// reduction, the reciprocal) costs as many instructions as ten values, hence two vectors per lane and not one (64 prompts of
-// 512 tokens, 8 kv heads, D = 128: one vector 53 us, 156 instructions per warp and vector).
+// reduction, the reciprocal) costs as many instructions as ten values, hence several vectors per lane.  Measured, 64 prompts of
+// 512 tokens, 8 kv heads, D = 128 (201 MB read and written): one vector per lane 53 us, two 43, four 39 = 5.2 TB/s; two rows in
+// flight per thread with four vectors each 41.
 template <bool BF16, int D>
 __global__ void __launch_bounds__(kI8AppendThreads)
 append_int8_kernel(Geometry g, uint8_t* __restrict__ pool, StepDev st, Divisor per_tok, const int32_t* __restrict__ page_table,
                    const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int64_t* __restrict__ slots_out) {
-    constexpr int LANES = D / 16, ROWS = kI8AppendThreads / LANES;
+    constexpr int LANES = D / (8 * kI8Vec);
     const int c = threadIdx.x % LANES;
-    const uint32_t n = (uint32_t)st.n_tokens * per_tok.d;    // (rows of a step fit the GPU's memory: below 2^31)
-    const uint32_t u0 = blockIdx.x * (ROWS * kI8InFlight) + threadIdx.x / LANES;
-    uint4 x[kI8InFlight][2];
-    int slot[kI8InFlight];
+    const uint32_t u = (blockIdx.x * kI8AppendThreads + threadIdx.x) / LANES;
+    const bool live = u < (uint32_t)st.n_tokens * per_tok.d;         // (rows of a step fit the GPU's memory: below 2^31)
+    const uint32_t t = per_tok.of(u), rem = u - t * per_tok.d, kv = rem >= (uint32_t)g.Hkv, h = kv ? rem - g.Hkv : rem;
+    uint4 x[kI8Vec];
+    int slot = 0;
+    if (live) {
+        const uint16_t* src = (kv ? v : k) + ((size_t)t * g.Hkv + h) * D + c * 8;
 #pragma unroll
-    for (int i = 0; i < kI8InFlight; i++) {
-        const uint32_t u = u0 + i * ROWS;
-        x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);
-        slot[i] = -1;
-        if (u < n) {
-            const uint32_t t = per_tok.of(u), rem = u - t * per_tok.d, kv = rem >= (uint32_t)g.Hkv, h = kv ? rem - g.Hkv : rem;
-            const uint16_t* src = (kv ? v : k) + ((size_t)t * g.Hkv + h) * D + c * 8;
-            x[i][0] = *reinterpret_cast<const uint4*>(src);
-            x[i][1] = *reinterpret_cast<const uint4*>(src + D / 2);
-            slot[i] = st.tok_dst[t];
-        }
+        for (int e = 0; e < kI8Vec; e++) x[e] = *reinterpret_cast<const uint4*>(src + e * (D / kI8Vec));
+        slot = st.tok_dst[t];
+    } else {
+#pragma unroll
+        for (int e = 0; e < kI8Vec; e++) x[e] = make_uint4(0, 0, 0, 0);
     }
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < kI8InFlight; i++) {
-        uint32_t m = max(i8_absmax8(x[i][0]), i8_absmax8(x[i][1]));
+    for (int e = 0; e < kI8Vec; e++) m = max(m, i8_absmax8(x[e]));
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        const bool huge = __any_sync(0xFFFFFFFFu, !(i8_amax_value<BF16>(m) <= kI8AmaxMax));    // values that saturate, or a NaN
-        if (slot[i] < 0) continue;
-        const uint32_t u = u0 + i * ROWS, t = per_tok.of(u), rem = u - t * per_tok.d, kv = rem >= (uint32_t)g.Hkv, h = kv ? rem - g.Hkv : rem;
-        const I8Row row = i8_row(i8_amax_value<BF16>(m));
-        uint8_t* tile = pool + ((size_t)(slot[i] / kI8Page) * g.Hkv + h) * i8_tile_bytes(D);
-        const int r = slot[i] % kI8Page;
-        uint2* to = reinterpret_cast<uint2*>(tile + i8_row_off(D, kv, r) + c * 8);
-        to[0]      = huge ? i8_codes8<BF16, true>(x[i][0], row.to_code) : i8_codes8<BF16, false>(x[i][0], row.to_code);
-        to[D / 16] = huge ? i8_codes8<BF16, true>(x[i][1], row.to_code) : i8_codes8<BF16, false>(x[i][1], row.to_code);
-        if (c == 0) {
-            *reinterpret_cast<float*>(tile + i8_scale_off(D, kv, r)) = row.scale;
-            if (slots_out && rem == 0) {
-                const int pos = st.tok_pos[t];
-                slots_out[t] = (int64_t)page_table[(size_t)st.seq[st.tok_b[t]] * g.max_pages_per_seq + pos / kI8Page] * kI8Page + pos % kI8Page;
-            }
+    for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    const bool huge = __any_sync(0xFFFFFFFFu, !(i8_amax_value<BF16>(m) <= kI8AmaxMax));    // values that saturate, or a NaN
+    if (!live) return;
+    const I8Row row = i8_row(i8_amax_value<BF16>(m));
+    uint8_t* tile = pool + ((size_t)(slot / kI8Page) * g.Hkv + h) * i8_tile_bytes(D);
+    const int r = slot % kI8Page;
+    uint2* to = reinterpret_cast<uint2*>(tile + i8_row_off(D, kv, r) + c * 8);
+#pragma unroll
+    for (int e = 0; e < kI8Vec; e++)
+        to[e * LANES] = huge ? i8_codes8<BF16, true>(x[e], row.to_code) : i8_codes8<BF16, false>(x[e], row.to_code);
+    if (c == 0) {
+        *reinterpret_cast<float*>(tile + i8_scale_off(D, kv, r)) = row.scale;
+        if (slots_out && rem == 0) {
+            const int pos = st.tok_pos[t];
+            slots_out[t] = (int64_t)page_table[(size_t)st.seq[st.tok_b[t]] * g.max_pages_per_seq + pos / kI8Page] * kI8Page + pos % kI8Page;
         }
     }
 }
@@ -80,7 +76,7 @@ append_int8_kernel(Geometry g, uint8_t* __restrict__ pool, StepDev st, Divisor p
 template <bool BF16, int D>
 cudaError_t launch_d(const Geometry& g, const LayerPtrs& lp, const StepDev& st, const int32_t* page_table, const void* k,
                      const void* v, int64_t* slots_out, cudaStream_t s) {
-    constexpr int ROWS = kI8AppendThreads / (D / 16) * kI8InFlight;
+    constexpr int ROWS = kI8AppendThreads / (D / (8 * kI8Vec));
     const long long units = (long long)st.n_tokens * 2 * g.Hkv;
     append_int8_kernel<BF16, D><<<(unsigned)((units + ROWS - 1) / ROWS), kI8AppendThreads, 0, s>>>(
         g, (uint8_t*)lp.pool, st, divisor(2 * (uint32_t)g.Hkv), page_table, (const uint16_t*)k, (const uint16_t*)v, slots_out);

@@ -169,7 +169,12 @@ decode_int8_kernel(const __grid_constant__ CUtensorMap tmap, Geometry g, uint8_t
     for (int i = 0; i < n_w; i++) {
         const int s = i % kI8Stages;
         // warp-uniform verdict; a wait that gave up has set the status word and no output is written
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(smem_u32(&bars[warp * kI8Stages + s]), (uint32_t)((i / kI8Stages) & 1), status))) break;
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait_bounded(smem_u32(&bars[warp * kI8Stages + s]), (uint32_t)((i / kI8Stages) & 1), status))) {
+            // (no copy of this warp may land after the CTA is gone: wait, with the same limit, for those behind the one that is late)
+            for (int f = i; f < min(i + kI8Stages, n_w); f++)
+                (void)mbar_wait_bounded(smem_u32(&bars[warp * kI8Stages + f % kI8Stages]), (uint32_t)((f / kI8Stages) & 1), status);
+            break;
+        }
         uint8_t* stg = wstage + (size_t)s * C::STAGE;
         const uint32_t stg_u = smem_u32(stg);
         const int tok_base = (lp0 + warp + kWarps * i) * kPage;
