@@ -33,10 +33,12 @@ namespace {
 constexpr int kPfRows = kPrefillRowsInt8;       // 256: two halves of kTcRows
 constexpr int kPfBlock = 64;                    // context tokens per block (4 pages)
 constexpr int kPfRaw = 4;                       // stages of raw tiles: K is expanded two blocks ahead of V
-constexpr int kPfSoftWarps = kPfRows / 16, kPfExpWarps = 4;
+constexpr int kPfGroups = 1;                     // 16-row groups per softmax warp
+constexpr int kPfSoftWarps = kPfRows / (16 * kPfGroups), kPfExpWarps = 4;
 constexpr int kPfMmaWarp = kPfSoftWarps + kPfExpWarps, kPfLoadWarp = kPfMmaWarp + 2;    // an MMA warp for each half
-constexpr int kPfThreads = 768;                  // 6 warpgroups: 4 of softmax, expanders, (two MMA warps, loader, an idle warp)
+constexpr int kPfThreads = (kPfSoftWarps + 8) * 32;                  // 6 warpgroups: 4 of softmax, expanders, (two MMA warps, loader, an idle warp)
 constexpr int kPfSoftThreads = kPfSoftWarps * 32;
+constexpr int kPfRegsSoft = 96, kPfRegsOther = 48;
 constexpr int kPfExpThreads = kPfExpWarps * 32;
 constexpr uint32_t kPfTmemCols = 512, kPfHalfCols = 256, kPfColO = 128;   // half h: S at 256h and 256h + 64, O at 256h + 128
 
@@ -252,7 +254,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         asm volatile("bar.sync 1, %0;" ::"n"(kPfThreads) : "memory");
     };
     if (warp >= kPfMmaWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfRegsOther));
     if (warp - kPfMmaWarp < halves) {
         // ===== MMA warps, one per half of the tile: an elected lane feeds the tensor pipe =====
         // (one warp for both halves made each wait for the other's barriers)
@@ -326,7 +328,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     return;
     }
     if (warp >= kPfSoftWarps) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfRegsOther));
         // ===== expander warps: codes -> fp16 slabs =====
         const int et = tid - kPfSoftWarps * 32;
         const float sc2E = kLog2e / sqrtf((float)D) * (IO_BF16 && !wide ? pf_pow2i(e0) : 1.0f);
@@ -384,7 +386,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         leave();
         return;
     }
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPfRegsSoft));
     if (warp < halves * (kPfSoftWarps / 2)) {
         // ===== softmax warps =====
         // A warp owns 16 rows (tensor-memory lanes; the two that share a 32-lane window, and a scheduler, take a half of it each),
@@ -393,14 +395,16 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         // wavefronts per 32 rows and block instead of 48).  Four warps per scheduler, because the pass is a chain of TMEM load,
         // multiply-add, exponential, conversion: with two, of 32 rows each, it took 2200 clocks a block of which the
         // special-function unit worked 1024.
-        const int half = warp >> 3, quad = lane & 3;
-        const int row0 = half * kTcRows + (warp & 3) * 32 + ((warp >> 2) & 1) * 16 + (lane >> 2);    // + 8 rr
-        const uint32_t base = tmem + half * kPfHalfCols + ((uint32_t)((warp & 3) * 32 + ((warp >> 2) & 1) * 16) << 16);
-        float m2[2];                                         // per row: reference (base 2)
-        f32x2 l2[2];                                         // ... sums over this thread's even and odd columns
-        int lim[2];                                          // positions the row sees
+        constexpr int NR = 2 * kPfGroups, WPH = kPfSoftWarps / 2;    // rows per thread, warps per half
+        const int half = warp / WPH, quad = lane & 3;
+        const int lane0 = (warp & 3) * 32 + (warp % WPH >> 2) * 16;  // first tensor-memory lane of the warp
+        const int row0 = half * kTcRows + lane0 + (lane >> 2);       // + 8 rr
+        const uint32_t base = tmem + half * kPfHalfCols + ((uint32_t)lane0 << 16);
+        float m2[NR];                                        // per row: reference (base 2)
+        f32x2 l2[NR];                                        // ... sums over this thread's even and odd columns
+        int lim[NR];                                         // positions the row sees
 #pragma unroll
-        for (int rr = 0; rr < 2; rr++) {
+        for (int rr = 0; rr < NR; rr++) {
             const int row = row0 + 8 * rr;
             m2[rr] = -1e30f;
             l2[rr] = 0ull;
@@ -410,7 +414,11 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         const uint32_t e_u = smem_u32(s_e) + 4 * row0;       // the rows' powers of two, 8 rows apart
         auto power = [&](int rr) { const float e = IO_BF16 && wide ? lds32(e_u + 32 * rr) : 1.0f; return pack_x2(e, e); };
         const bool idle = (row0 - (lane >> 2)) / G >= tok_cnt;   // no row of this warp has a token: whatever W holds, nobody reads its O
-        const int lim_min = min(lim[0], lim[1]);
+        int lim_min = lim[0];
+#pragma unroll
+        for (int rr = 1; rr < NR; rr++) lim_min = min(lim_min, lim[rr]);
+        // blocks that every row of the warp sees whole (none where the rows have powers of two of their own)
+        const int n_whole = IO_BF16 && wide ? 0 : (min(__reduce_min_sync(0xFFFFFFFFu, lim_min), t1) - t0) / kPfBlock;
         bool started = false;
         for (int blk = 0; blk < n_blocks; blk++) {
             const int buf = blk & 1;
@@ -421,39 +429,41 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             if (!__all_sync(0xFFFFFFFFu, ok)) { alive = false; break; }
             tc_fence_after();
             bool rescale = false;
-            float alpha[2] = {1.0f, 1.0f};
+            float alpha[NR];
             if (!idle) {
-                const int end = min(t1, tok_base + kPfBlock);
-                // whole: every row of the warp sees all of the block and no power of two is due
-                const bool whole = !(IO_BF16 && wide) && end - tok_base == kPfBlock && __all_sync(0xFFFFFFFFu, lim_min >= tok_base + kPfBlock);
-                int nv[2];                                   // of a row: tokens of the block it sees, from this thread's first column on
-#pragma unroll
-                for (int rr = 0; rr < 2; rr++) nv[rr] = min(lim[rr], end) - tok_base - 2 * quad;
                 // The weights of the block against the current references, 16 columns of S at a time, the next 16 on their way; S
                 // stays in tensor memory until W goes over it.  -> false, with nothing changed, where `check` is set and a score exceeds
                 // its row's reference by more than 2^kLazy.
                 auto weigh = [&](auto masked, bool check) -> bool {
                     constexpr bool M = decltype(masked)::value;
-                    uint32_t pr[16];                         // W of the rows as a 16x128b fragment
-                    f32x2 nm[2], tl[2];                      // tl: the block's share of the sums
+                    uint32_t pr[kPfGroups][16];              // W of the rows as 16x128b fragments
+                    f32x2 nm[NR], tl[NR];                    // tl: the block's share of the sums
                     float top = -1e30f;
 #pragma unroll
-                    for (int rr = 0; rr < 2; rr++) { tl[rr] = 0ull; nm[rr] = pack_x2(-m2[rr], -m2[rr]); }
-                    f32x2 E[2];
-                    if (M) { E[0] = power(0); E[1] = power(1); }
-                    f32x2 sr[2][4];
-                    tmem_ld_frag16(col_s, sr[0]);
+                    for (int rr = 0; rr < NR; rr++) { tl[rr] = 0ull; nm[rr] = pack_x2(-m2[rr], -m2[rr]); }
+                    f32x2 E[NR];
+                    int nv[NR];                              // of a row: tokens of the block it sees, from this thread's first column on
+#pragma unroll
+                    for (int rr = 0; rr < NR; rr++)
+                        if (M) { E[rr] = power(rr); nv[rr] = min(lim[rr], t1) - tok_base - 2 * quad; }
+                    f32x2 sr[2][kPfGroups][4];
+#pragma unroll
+                    for (int gi = 0; gi < kPfGroups; gi++) tmem_ld_frag16(col_s + ((uint32_t)(16 * gi) << 16), sr[0][gi]);
 #pragma unroll
                     for (int qt = 0; qt < 4; qt++) {
-                        tc_wait_ld_frag16(sr[qt & 1]);
-                        if (qt < 3) tmem_ld_frag16(col_s + 16 * (qt + 1), sr[(qt + 1) & 1]);
+#pragma unroll
+                        for (int gi = 0; gi < kPfGroups; gi++) tc_wait_ld_frag16(sr[qt & 1][gi]);
+                        if (qt < 3) {
+#pragma unroll
+                            for (int gi = 0; gi < kPfGroups; gi++) tmem_ld_frag16(col_s + 16 * (qt + 1) + ((uint32_t)(16 * gi) << 16), sr[(qt + 1) & 1][gi]);
+                        }
 #pragma unroll
                         for (int k = 0; k < 2; k++) {        // tokens 16 qt + 8 k + 2 quad, +1
                             const int t = 16 * qt + 8 * k;
                             const f32x2 ks = lds64(sc + 4 * t), lv = lds64(sc + 4 * (kPfBlock + t)), iv = lds64(sc + 4 * (2 * kPfBlock + t));
 #pragma unroll
-                            for (int rr = 0; rr < 2; rr++) {
-                                const f32x2 a = sr[qt & 1][2 * k + rr];
+                            for (int rr = 0; rr < NR; rr++) {
+                                const f32x2 a = sr[qt & 1][rr >> 1][2 * k + (rr & 1)];
                                 const f32x2 u = add_x2(lv, nm[rr]);
                                 float2 x = unpack_x2(M ? fma_x2(mul_x2(a, ks), E[rr], u) : fma_x2(a, ks, u));
                                 if (M) {                     // (also where the scale of a token the row does not see is a NaN)
@@ -468,42 +478,49 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                                 } else {
                                     tl[rr] = fma_x2(pack_x2(w0, w1), iv, tl[rr]);
                                 }
-                                pr[4 * qt + 2 * k + rr] = pack2<false>(w0, w1);
+                                pr[rr >> 1][4 * qt + 2 * k + (rr & 1)] = pack2<false>(w0, w1);
                             }
                         }
                     }
                     if (__any_sync(0xFFFFFFFFu, top > kLazy) && check) return false;
 #pragma unroll
-                    for (int rr = 0; rr < 2; rr++) l2[rr] = add_x2(l2[rr], tl[rr]);
-                    tmem_st_half32(col_s, pr);               // W over the columns S was read from
+                    for (int rr = 0; rr < NR; rr++) l2[rr] = add_x2(l2[rr], tl[rr]);
+#pragma unroll
+                    for (int gi = 0; gi < kPfGroups; gi++) tmem_st_half32(col_s + ((uint32_t)(16 * gi) << 16), pr[gi]);     // W over the columns S was read from
                     return true;
                 };
                 // speculating that the references stay; a row without one (its first block, or none of it seen so far) has to look first
                 bool look = !started;
-                if (!look) look = !(whole ? weigh(std::false_type{}, true) : weigh(std::true_type{}, true));
+                if (!look) look = !(blk < n_whole ? weigh(std::false_type{}, true) : weigh(std::true_type{}, true));
                 if (look) {                                  // new references for the rows that need one, then the weights
-                    float mx[2] = {-INFINITY, -INFINITY};
-                    const f32x2 E[2] = {power(0), power(1)};
+                    float mx[NR];
+                    f32x2 E[NR];
+                    int nv[NR];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        uint32_t sf[16];
-                        tmem_ld_frag32(col_s + 32 * h, sf);
-                        tc_wait_ld16(sf);
+                    for (int rr = 0; rr < NR; rr++) { mx[rr] = -INFINITY; E[rr] = power(rr); alpha[rr] = 1.0f; nv[rr] = min(lim[rr], t1) - tok_base - 2 * quad; }
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const int t = 32 * h + 8 * k;
-                            const f32x2 ks = lds64(sc + 4 * t), lv = lds64(sc + 4 * (kPfBlock + t));
+                    for (int h = 0; h < 2; h++)
 #pragma unroll
-                            for (int rr = 0; rr < 2; rr++) {
-                                const float2 x = unpack_x2(fma_x2(mul_x2(pack_x2(sf[4 * k + 2 * rr], sf[4 * k + 2 * rr + 1]), ks), E[rr], lv));
-                                mx[rr] = fmaxf(mx[rr], t < nv[rr] ? x.x : -INFINITY);
-                                mx[rr] = fmaxf(mx[rr], t + 1 < nv[rr] ? x.y : -INFINITY);
+                        for (int gi = 0; gi < kPfGroups; gi++) {
+                            uint32_t sf[16];
+                            tmem_ld_frag32(col_s + 32 * h + ((uint32_t)(16 * gi) << 16), sf);
+                            tc_wait_ld16(sf);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const int t = 32 * h + 8 * k;
+                                const f32x2 ks = lds64(sc + 4 * t), lv = lds64(sc + 4 * (kPfBlock + t));
+#pragma unroll
+                                for (int hh = 0; hh < 2; hh++) {
+                                    const int rr = 2 * gi + hh;
+                                    const float2 x = unpack_x2(fma_x2(mul_x2(pack_x2(sf[4 * k + 2 * hh], sf[4 * k + 2 * hh + 1]), ks), E[rr], lv));
+                                    mx[rr] = fmaxf(mx[rr], t < nv[rr] ? x.x : -INFINITY);
+                                    mx[rr] = fmaxf(mx[rr], t + 1 < nv[rr] ? x.y : -INFINITY);
+                                }
                             }
                         }
-                    }
                     started = true;
 #pragma unroll
-                    for (int rr = 0; rr < 2; rr++) {         // the four threads of a row agree
+                    for (int rr = 0; rr < NR; rr++) {         // the four threads of a row agree
                         mx[rr] = fmaxf(mx[rr], __shfl_xor_sync(0xFFFFFFFFu, mx[rr], 1));
                         mx[rr] = fmaxf(mx[rr], __shfl_xor_sync(0xFFFFFFFFu, mx[rr], 2));
                         if (mx[rr] > m2[rr] + kLazy) {
@@ -527,14 +544,17 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                 tc_fence_after();
                 if (rescale) {
 #pragma unroll
-                    for (int part = 0; part < D / 32; part++) {
-                        uint32_t of[16];
-                        tmem_ld_frag32(base + kPfColO + 32 * part, of);
-                        tc_wait_ld16(of);
+                    for (int part = 0; part < D / 32; part++)
 #pragma unroll
-                        for (int c = 0; c < 16; c++) of[c] = __float_as_uint(__uint_as_float(of[c]) * alpha[(c >> 1) & 1]);
-                        tmem_st_frag32(base + kPfColO + 32 * part, of);
-                    }
+                        for (int gi = 0; gi < kPfGroups; gi++) {
+                            uint32_t of[16];
+                            const uint32_t at = base + kPfColO + 32 * part + ((uint32_t)(16 * gi) << 16);
+                            tmem_ld_frag32(at, of);
+                            tc_wait_ld16(of);
+#pragma unroll
+                            for (int c = 0; c < 16; c++) of[c] = __float_as_uint(__uint_as_float(of[c]) * alpha[2 * gi + ((c >> 1) & 1)]);
+                            tmem_st_frag32(at, of);
+                        }
                 }
             }
             tc_wait_st();
@@ -546,12 +566,12 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
 
         const bool poisoned = __any_sync(0xFFFFFFFFu, !alive || __ldcg(status) != 0);   // fail closed, whole warps at a time
         if (!poisoned && !idle) {
-            float f[2];
-            float* prow[2];
-            size_t qo[2];
-            bool valid[2];
+            float f[NR];
+            float* prow[NR];
+            size_t qo[NR];
+            bool valid[NR];
 #pragma unroll
-            for (int rr = 0; rr < 2; rr++) {
+            for (int rr = 0; rr < NR; rr++) {
                 const float2 lf = unpack_x2(l2[rr]);
                 float l = lf.x + lf.y;
                 l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
@@ -571,23 +591,26 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                 }
             }
 #pragma unroll
-            for (int part = 0; part < D / 32; part++) {
-                uint32_t of[16];
-                tmem_ld_frag32(base + kPfColO + 32 * part, of);
-                tc_wait_ld16(of);
+            for (int part = 0; part < D / 32; part++)
 #pragma unroll
-                for (int rr = 0; rr < 2; rr++) {
-                    if (!valid[rr]) continue;
+                for (int gi = 0; gi < kPfGroups; gi++) {
+                    uint32_t of[16];
+                    tmem_ld_frag32(base + kPfColO + 32 * part + ((uint32_t)(16 * gi) << 16), of);
+                    tc_wait_ld16(of);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const float o0 = __uint_as_float(of[4 * k + 2 * rr]) * f[rr], o1 = __uint_as_float(of[4 * k + 2 * rr + 1]) * f[rr];
-                        const int c = 32 * part + 8 * k + 2 * quad;
-                        if (n_chunks > 1)                *reinterpret_cast<float2*>(prow[rr] + c) = make_float2(o0, o1);
-                        else if (out_dtype == DT_FP32)   *reinterpret_cast<float2*>((float*)out + qo[rr] + c) = make_float2(o0, o1);
-                        else                             *reinterpret_cast<uint32_t*>((uint16_t*)out + qo[rr] + c) = pack2<IO_BF16>(o0, o1);
+                    for (int hh = 0; hh < 2; hh++) {
+                        const int rr = 2 * gi + hh;
+                        if (!valid[rr]) continue;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const float o0 = __uint_as_float(of[4 * k + 2 * hh]) * f[rr], o1 = __uint_as_float(of[4 * k + 2 * hh + 1]) * f[rr];
+                            const int c = 32 * part + 8 * k + 2 * quad;
+                            if (n_chunks > 1)                *reinterpret_cast<float2*>(prow[rr] + c) = make_float2(o0, o1);
+                            else if (out_dtype == DT_FP32)   *reinterpret_cast<float2*>((float*)out + qo[rr] + c) = make_float2(o0, o1);
+                            else                             *reinterpret_cast<uint32_t*>((uint16_t*)out + qo[rr] + c) = pack2<IO_BF16>(o0, o1);
+                        }
                     }
                 }
-            }
         }
     }
 
