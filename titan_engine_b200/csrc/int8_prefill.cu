@@ -626,10 +626,68 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         *s_flag = last;
     }
     asm volatile("bar.sync 2, %0;" ::"n"(kPfSoftThreads) : "memory");
-    if (*s_flag) {
+    if (!*s_flag) return;
+    __threadfence();                                        // see the other CTAs' rows
+    if (__ldcg(status) != 0) return;
+    const int rows = G * tok_cnt;
+    const size_t chunk_stride = (size_t)nq * g.H * (D + 2);
+    const float* region = partials + (size_t)poff * g.H * (D + 2);
+    auto column = [&](int row) { return (size_t)(tok_first + row / G) * g.H + kvh * G + row % G; };
+    if (rows * n_chunks * 4 > C::OFF_BARS) {                // (more weights than shared memory)
         const MergeOut mo{nullptr, out, nullptr, out_dtype, nullptr, status};
-        merge_rows(g, mo, b, kvh, G, 0, n_chunks, partials + (size_t)poff * g.H * (D + 2),
-                   MergeMap{G * tok_cnt, nq * g.H, q_base + tok_first, tok_first, 0}, kPfSoftWarps);
+        merge_rows(g, mo, b, kvh, G, 0, n_chunks, region, MergeMap{rows, nq * g.H, q_base + tok_first, tok_first, 0}, kPfSoftWarps);
+        return;
+    }
+    // The merge of tk_merge.cuh for all rows at once (row after row its chain of L2 loads took 22 us for 256 rows): a thread per row
+    // for the weights, then every thread its columns of eight rows with the loads of four chunks in flight.
+    float* s_w = reinterpret_cast<float*>(smem);            // [rows][n_chunks] weight times the row's normaliser
+    if (tid < rows) {
+        const float* ml = region + column(tid) * (D + 2) + D;
+        float M = -1e30f, L = 0.0f;
+        for (int r = 0; r < n_chunks; r++) {
+            const float2 c = __ldcg(reinterpret_cast<const float2*>(ml + r * chunk_stride));
+            const float mn = fmaxf(M, c.x);
+            L = L * expf(M - mn) + c.y * expf(c.x - mn);
+            M = mn;
+            s_w[tid * n_chunks + r] = c.x;
+        }
+        const float inv = 1.0f / (L + 1e-8f);
+        for (int r = 0; r < n_chunks; r++) s_w[tid * n_chunks + r] = expf(s_w[tid * n_chunks + r] - M) * inv;
+    }
+    asm volatile("bar.sync 2, %0;" ::"n"(kPfSoftThreads) : "memory");
+    constexpr int U = 8, R = 4, PER = kPfSoftThreads / (D / 2);     // rows a pass of all threads covers
+    const int d = 2 * (tid % (D / 2));
+    for (int row_a = tid / (D / 2); row_a < rows; row_a += U * PER) {
+        float2 acc[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) acc[u] = make_float2(0.0f, 0.0f);
+        for (int rb = 0; rb < n_chunks; rb += R) {
+            float2 x[R][U];
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    x[r][u] = rb + r < n_chunks && row_a + u * PER < rows
+                                  ? __ldcg(reinterpret_cast<const float2*>(region + column(row_a + u * PER) * (D + 2) + d + (rb + r) * chunk_stride))
+                                  : make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (rb + r < n_chunks && row_a + u * PER < rows) {
+                        const float w = s_w[(row_a + u * PER) * n_chunks + rb + r];
+                        acc[u].x += x[r][u].x * w;
+                        acc[u].y += x[r][u].y * w;
+                    }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int row = row_a + u * PER;
+            if (row >= rows) break;
+            const size_t at = ((size_t)(q_base + tok_first + row / G) * g.H + kvh * G + row % G) * D + d;
+            if (out_dtype == DT_FP32) *reinterpret_cast<float2*>((float*)out + at) = acc[u];
+            else                      *reinterpret_cast<uint32_t*>((uint16_t*)out + at) = pack2<IO_BF16>(acc[u].x, acc[u].y);
+        }
     }
 }
 

@@ -4,6 +4,7 @@
 #include <cstdint>
 
 #include <algorithm>
+#include <functional>
 #include <cstring>
 
 namespace tk {
@@ -287,6 +288,48 @@ void radix_pass(const std::vector<uint32_t>& key, std::vector<int32_t>& idx, std
     for (int32_t i : idx) tmp[count[(key[(size_t)i] >> shift) & 2047u]++] = i;
     idx.swap(tmp);
 }
+// Split-KV chunk (tokens) of the INT8 chunk kernel's items.  One CTA fills an SM there; an item's start and end cost as much as
+// kItemBlocks blocks of 64 tokens, a part of a split tile kSplitBlocks more (its rows go out in FP32 and are merged).  A small
+// step is as long as its longest SM, so the items are dealt out, longest first, for whole tiles and for a few chunk sizes around
+// an SM's fair share of the blocks, and the shortest schedule is taken.  (9 prompt chunks of up to 517 tokens on contexts of up
+// to 1500: 47 us whole, 57 us in parts of 8 to 24 blocks; 5 tokens on a context of 65536: parts of 56 blocks or less.)
+constexpr int kItemBlocks = 6, kSplitBlocks = 10;
+template <typename Small>
+int64_t fair_chunk(const StepPlan& p, int tpt, int num_kv_heads, int sms, const Small& is_small) {
+    std::vector<int64_t> tiles;                            // blocks each (sequence, tile) sees
+    int64_t blocks = 0;
+    for (size_t i = 0; i < p.nq.size(); i++) {
+        if (is_small((int)i)) continue;
+        const int nq = p.nq[i], base = p.len[i] - nq;
+        for (int t = 0; t * tpt < nq; t++) {
+            tiles.push_back((base + std::min(nq, (t + 1) * tpt) + 63) / 64);
+            blocks += tiles.back() * num_kv_heads;
+        }
+    }
+    const int64_t share = std::max<int64_t>(4, (blocks + sms - 1) / sms);
+    if ((int64_t)tiles.size() * num_kv_heads > 8 * (int64_t)sms) return share * 64;     // many items balance themselves
+    const int64_t whole = tiles.empty() ? share : *std::max_element(tiles.begin(), tiles.end());
+    int64_t best = share, best_end = INT64_MAX;
+    std::vector<int64_t> cost, load;
+    for (int64_t cap : {whole, share, share * 3 / 4, share / 2, share / 3, share / 4}) {
+        cap = std::max<int64_t>(4, cap);
+        cost.clear();
+        for (int64_t b : tiles)
+            for (int64_t at = 0; at < b; at += cap)
+                for (int h = 0; h < num_kv_heads; h++) cost.push_back(std::min(cap, b - at) + kItemBlocks + (b > cap ? kSplitBlocks : 0));
+        std::sort(cost.begin(), cost.end(), std::greater<int64_t>());
+        load.assign((size_t)sms, 0);                       // a heap, the least loaded SM on top
+        for (int64_t c : cost) {
+            std::pop_heap(load.begin(), load.end(), std::greater<int64_t>());
+            load.back() += c;
+            std::push_heap(load.begin(), load.end(), std::greater<int64_t>());
+        }
+        const int64_t end = *std::max_element(load.begin(), load.end());
+        if (end < best_end) { best_end = end; best = cap; }
+    }
+    return best * 64;
+}
+
 }  // namespace
 
 int PageManager::plan_step(int n_seqs, const int32_t* seqs, const int32_t* n_new, int num_kv_heads,
@@ -481,6 +524,7 @@ int PageManager::plan_step(int n_seqs, const int32_t* seqs, const int32_t* n_new
             if (is_small(i)) plan->pf_small_nq_max = std::max(plan->pf_small_nq_max, plan->nq[i]);
         // rows of the workspace the decode kernel's share of the step uses; the split regions lie behind them
         const int64_t small_rows = (int64_t)plan->chunk_base[n_seqs] * plan->pf_small_nq_max;
+        const int64_t fair = prefill_rows == kPrefillRowsInt8 ? fair_chunk(*plan, tpt, num_kv_heads, std::max(1, target_items / 8), is_small) : 0;
         // split-KV chunk per sequence: about 48 items per sequence where its tiles alone give fewer; halve
         // the number of chunks (shrink) until the split regions fit the workspace
         for (int shrink = 0;; shrink++) {
@@ -494,6 +538,7 @@ int PageManager::plan_step(int n_seqs, const int32_t* seqs, const int32_t* n_new
                 int64_t ct = ((int64_t)len + want - 1) / want;
                 ct = (ct + 511) / 512 * 512;
                 ct = std::min<int64_t>(std::max<int64_t>(ct, 1024), max_ct);
+                if (fair) ct = std::min<int64_t>({((int64_t)len + 63) / 64 * 64, fair << shrink, (int64_t)max_ct});   // (tokens)
                 plan->pf_ct[i] = (int32_t)ct;
                 const int n_chunks = (int)((len + ct - 1) / ct);
                 plan->pf_poff[i] = (int32_t)rows;
@@ -501,7 +546,8 @@ int PageManager::plan_step(int n_seqs, const int32_t* seqs, const int32_t* n_new
             }
             // (past the last shrink every sequence has as few chunks as 32768-token items allow: the caller
             // then finds room for the rows elsewhere)
-            if (small_rows + rows <= max_partial_rows || shrink > 8) { plan->pf_partial_rows = (int32_t)std::min<int64_t>(rows, INT32_MAX); break; }
+            // (INT8: the caller's own workspace holds as many rows as a few hundred items of a small step write)
+            if (small_rows + rows <= std::max(max_partial_rows, fair ? kInt8SplitRows : 0) || shrink > 8) { plan->pf_partial_rows = (int32_t)std::min<int64_t>(rows, INT32_MAX); break; }
         }
         std::vector<int64_t> weight;
         weight.reserve(plan->pf_items.capacity());
@@ -542,7 +588,8 @@ int PageManager::plan_step(int n_seqs, const int32_t* seqs, const int32_t* n_new
             int64_t bytes_in = 0;
             int32_t set = 0;
             for (int32_t gi : gord) {
-                const int64_t kv_bytes = (int64_t)plan->len[gi / num_kv_heads] * 512;   // K and V rows of 128 16-bit dims
+                // K and V rows of 128 16-bit dims; of 128 codes and their scales
+                const int64_t kv_bytes = (int64_t)plan->len[gi / num_kv_heads] * (prefill_rows == kPrefillRowsInt8 ? 264 : 512);
                 if (bytes_in > 0 && bytes_in + kv_bytes > kSetBytes) { set++; bytes_in = 0; }
                 group_set[gi] = set;
                 bytes_in += kv_bytes;

@@ -79,6 +79,7 @@ struct StepPlan {
 constexpr int kPrefillRows = 64;           // (token, head) rows per tile of the mma.sync prefill kernel
 constexpr int kPrefillRowsTc = 128;        // ... of the tcgen05 prefill kernel
 constexpr int kPrefillRowsInt8 = 256;     // ... of the kernel over INT8 pools (two halves of 128)
+constexpr int kInt8SplitRows = 4096;       // token rows a step's split regions may take there whatever the handle's workspace holds
 constexpr int kPrefillMaxPages = 2048;     // pages per item: a split-KV chunk holds at most 32768 tokens
 constexpr int kDecodeTileRows = 16;        // rows of the decode kernel's tile
 constexpr int kDecodeMaxTokenGroups = 8;   // token groups per sequence the decode kernel's multi-token form takes
