@@ -107,3 +107,42 @@ def test_compute_calls_need_a_device():
     assert c._lib.tk_kv_read(c._h, 1, 0, None, None, None, None, None, L.TK_BF16, None) == L.TK_INVALID_ARG
     assert c._lib.tk_kv_read(None, 0, 0, None, None, None, None, None, L.TK_BF16, None) == L.TK_INVALID_ARG
     assert c._lib.tk_kv_decode_multi(c._h, 0, None, None, None) == L.TK_CUDA_ERROR
+
+
+@pytest.mark.parametrize("shape", [(32, 8), (64, 8), (16, 1), (6, 3), (4, 4)])
+@pytest.mark.parametrize("lens", [
+    ([0, 5000, 33, 0, 40000, 700, 17], [300, 1, 4096, 70, 37, 3, 129]),
+    ([1100, 518, 1240], [24, 334, 440]),
+    ([65536], [20]), ([0], [8192]), ([3] * 40, [17] * 40),
+])
+def test_chunk_work_list_covers_every_row_once(shape, lens):
+    """The 256-row tiles and their split-KV parts cover every (query token, head) and every position it sees exactly once; rows
+    that fit one 16-row tile stay with the decode kernel; the list fits the step's buffers."""
+    H, Hkv = shape
+    G = H // Hkv
+    ctx, new = lens
+    c = _cache(num_heads=H, num_kv_heads=Hkv, num_pages=sum((a + b + 15) // 16 for a, b in zip(ctx, new)) + 1, max_seqs=len(ctx),
+               max_pages_per_seq=max((a + b + 15) // 16 for a, b in zip(ctx, new)), max_step_tokens=sum(new))
+    seqs = [c.seq_alloc() for _ in ctx]
+    for s, n in zip(seqs, ctx):
+        c.reserve(s, n)
+    c.step_begin(seqs, new)
+    items, ct, n_decode = c.step_prefill_plan()
+    tpt = 256 // G
+    small = [i for i, n in enumerate(new) if n * G <= 16]
+    assert len(items) == 0 or n_decode == sum(-(-(a + b) // c.step_chunk_tokens) * Hkv for i, (a, b) in enumerate(zip(ctx, new)) if i in small)
+    seen = {}
+    for b, chunk, kvh, tile in items.tolist():
+        assert b not in small and 0 <= kvh < Hkv and ct[b] % 64 == 0 and ct[b] <= 32768
+        p_last = ctx[b] + min(new[b], (tile + 1) * tpt) - 1
+        t0, t1 = chunk * ct[b], min((chunk + 1) * ct[b], p_last + 1)
+        assert tile * tpt < new[b] and t1 > t0
+        seen.setdefault((b, kvh, tile), []).append((t0, t1))
+    for b, n in enumerate(new):
+        for kvh in range(Hkv if b not in small else 0):
+            for tile in range(-(-n // tpt)):
+                spans = sorted(seen.pop((b, kvh, tile)))
+                p_last = ctx[b] + min(n, (tile + 1) * tpt) - 1
+                assert spans[0][0] == 0 and spans[-1][1] == p_last + 1 and all(x[1] == y[0] for x, y in zip(spans, spans[1:]))
+                assert len(spans) == p_last // ct[b] + 1
+    assert not seen

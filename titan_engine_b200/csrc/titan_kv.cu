@@ -305,7 +305,7 @@ int create_impl(const tk_kv_config* cfg_in, void* arena, size_t arena_bytes, boo
         const int64_t tiles = (int64_t)c.max_step_tokens * G / tk::kPrefillRows + c.max_seqs;      // the smaller tile: the upper bound
         const int64_t long_chunks = ((int64_t)c.max_pages_per_seq + tk::kPrefillMaxPages - 1) / tk::kPrefillMaxPages;
         h->max_pf_groups = (int)std::min<int64_t>(tiles * c.num_kv_heads, 1 << 24);
-        h->max_pf_items = (int)std::min<int64_t>(tiles * c.num_kv_heads * long_chunks + 128 * (int64_t)c.max_seqs + (c.dtype == TK_INT8 ? 256 : 0), 1 << 24);
+        h->max_pf_items = (int)std::min<int64_t>(tiles * c.num_kv_heads * long_chunks + 128 * (int64_t)c.max_seqs + (c.dtype == TK_INT8 ? 1024 : 0), 1 << 24);   // INT8: parts of a quarter of an SM's share
     }
 
     // one buffer holds every per-step array; sections are 16-byte aligned

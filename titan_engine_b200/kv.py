@@ -98,6 +98,11 @@ class PagedKVCache:
         self.cfg = L.KvConfig()
         self._lib.tk_kv_get_config(self._h, C.byref(self.cfg))
         self.io_torch_dtype = _TORCH16[self.cfg.io_dtype]
+        # what every call checks its tensors against, as plain Python values (a field of a ctypes structure costs ten times as much)
+        self._dev_index = -1 if host_only else self.device.index
+        self._heads, self._kv_heads, self._out_dim = self.cfg.num_heads, self.cfg.num_kv_heads, self.cfg.v_head_dim
+        self._pool_tokens = self.cfg.num_pages * self.cfg.page_size
+        self._dims = {"k": self.cfg.head_dim, "q": self.cfg.head_dim, "v": self.cfg.v_head_dim, "out": self.cfg.v_head_dim}
         self._n_seqs = 0
         self._n_tokens = 0
         if not host_only:
@@ -109,7 +114,7 @@ class PagedKVCache:
             raise KvError(st, self._lib.tk_kv_last_error(self._h).decode())
 
     def _stream(self) -> int:
-        return torch._C._cuda_getCurrentRawStream(self.device.index)
+        return torch._C._cuda_getCurrentRawStream(self._dev_index)
 
     def close(self) -> None:
         if getattr(self, "_h", None) and self._h.value:
@@ -231,17 +236,16 @@ class PagedKVCache:
         return items, ct[:self._n_seqs], nd.value
 
     def _check_io(self, t: torch.Tensor, rows: int, heads: int, what: str) -> None:
-        dim = self.cfg.v_head_dim if what in ("v", "out") else self.cfg.head_dim
-        if t.device != self.device or t.dtype != self.io_torch_dtype or not t.is_contiguous():
+        if t.get_device() != self._dev_index or t.dtype != self.io_torch_dtype or not t.is_contiguous():
             raise KvError(L.TK_INVALID_ARG, f"{what}: need a contiguous {self.io_torch_dtype} tensor on {self.device}")
-        if t.numel() != rows * heads * dim:
-            raise KvError(L.TK_INVALID_ARG, f"{what}: expected [{rows}, {heads}, {dim}]")
+        if t.numel() != rows * heads * self._dims[what]:
+            raise KvError(L.TK_INVALID_ARG, f"{what}: expected [{rows}, {heads}, {self._dims[what]}]")
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor,
                slots_out: Optional[torch.Tensor] = None) -> None:
         """k, v: [n_tokens, Hkv, D] on the device, io dtype; the step's tokens in order."""
-        self._check_io(k, self._n_tokens, self.cfg.num_kv_heads, "k")
-        self._check_io(v, self._n_tokens, self.cfg.num_kv_heads, "v")
+        self._check_io(k, self._n_tokens, self._kv_heads, "k")
+        self._check_io(v, self._n_tokens, self._kv_heads, "v")
         sp = None
         if slots_out is not None:
             assert slots_out.dtype == torch.int64 and slots_out.numel() >= self._n_tokens
@@ -265,48 +269,50 @@ class PagedKVCache:
             count = [self.seq_len(int(s)) - int(a) for s, a in zip(seq_ids, start)]
         if not len(seq_ids) == len(start) == len(count):
             raise KvError(L.TK_INVALID_ARG, "read: start and count need one entry for each sequence")
-        rows, cfg = int(sum(count)), self.cfg
-        if rows and not 0 <= min(count) <= max(count) <= cfg.num_pages * cfg.page_size:
+        rows = int(sum(count))
+        if rows and not 0 <= min(count) <= max(count) <= self._pool_tokens:
             raise KvError(L.TK_INVALID_ARG, "read: ranges must lie inside live sequences' tokens")
         (s, s_at), (a, a_at), (n, n_at) = _ints(seq_ids), _ints(start), _ints(count)
-        k = torch.empty(rows, cfg.num_kv_heads, cfg.head_dim, dtype=out_dtype, device=self.device)
-        v = torch.empty(rows, cfg.num_kv_heads, cfg.v_head_dim, dtype=out_dtype, device=self.device)
+        k = torch.empty((rows, self._kv_heads, self._dims["k"]), dtype=out_dtype, device=self.device)
+        v = torch.empty((rows, self._kv_heads, self._dims["v"]), dtype=out_dtype, device=self.device)
         self._check(self._lib.tk_kv_read(self._h, layer, len(s), s_at, a_at, n_at, k.data_ptr(), v.data_ptr(),
-                                         L.TK_FP32 if out_dtype == torch.float32 else cfg.io_dtype, self._stream()))
+                                         L.TK_FP32 if out_dtype == torch.float32 else self.cfg.io_dtype, self._stream()))
         return k, v
 
     def decode(self, layer: int, q: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """q: [n_seqs, H, D] -> out [n_seqs, H, D], io dtype."""
-        self._check_io(q, self._n_seqs, self.cfg.num_heads, "q")
+        self._check_io(q, self._n_seqs, self._heads, "q")
         if out is None:
-            out = torch.empty(q.shape[0], self.cfg.num_heads, self.cfg.v_head_dim, dtype=q.dtype, device=q.device)
-        self._check_io(out, self._n_seqs, self.cfg.num_heads, "out")
+            out = torch.empty(q.shape[0], self._heads, self._out_dim, dtype=q.dtype, device=q.device)
+        self._check_io(out, self._n_seqs, self._heads, "out")
         self._check(self._lib.tk_kv_decode(self._h, layer, q.data_ptr(), out.data_ptr(), self._stream()))
         return out
 
     def decode_f32(self, layer: int, q: torch.Tensor) -> torch.Tensor:
         """decode() with the result left in FP32 (tk_kv_decode_ex): q [n_seqs, H, D] io dtype -> [n_seqs, H, Dv] f32."""
-        self._check_io(q, self._n_seqs, self.cfg.num_heads, "q")
-        out = torch.empty(q.shape[0], self.cfg.num_heads, self.cfg.v_head_dim, dtype=torch.float32, device=q.device)
+        self._check_io(q, self._n_seqs, self._heads, "q")
+        out = torch.empty(q.shape[0], self._heads, self._out_dim, dtype=torch.float32, device=q.device)
         self._check(self._lib.tk_kv_decode_ex(self._h, layer, q.data_ptr(), self.cfg.io_dtype, out.data_ptr(),
                                               L.TK_FP32, self._stream()))
         return out
 
     def decode_multi_f32(self, layer: int, q: torch.Tensor) -> torch.Tensor:
         """decode_multi() with the result left in FP32 (tk_kv_decode_multi_ex)."""
-        self._check_io(q, self._n_tokens, self.cfg.num_heads, "q")
-        out = torch.empty(self._n_tokens, self.cfg.num_heads, self.cfg.v_head_dim, dtype=torch.float32, device=self.device)
+        self._check_io(q, self._n_tokens, self._heads, "q")
+        out = torch.empty(self._n_tokens, self._heads, self._out_dim, dtype=torch.float32, device=self.device)
         self._check(self._lib.tk_kv_decode_multi_ex(self._h, layer, q.data_ptr(), out.data_ptr(), L.TK_FP32, self._stream()))
         return out
 
     def append_decode(self, layer: int, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor,
                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """append + decode of one layer; a single fused kernel on 16-bit decode steps."""
-        self._check_io(k, self._n_tokens, self.cfg.num_kv_heads, "k")
-        self._check_io(v, self._n_tokens, self.cfg.num_kv_heads, "v")
-        self._check_io(q, self._n_seqs, self.cfg.num_heads, "q")
+        self._check_io(k, self._n_tokens, self._kv_heads, "k")
+        self._check_io(v, self._n_tokens, self._kv_heads, "v")
+        self._check_io(q, self._n_seqs, self._heads, "q")
         if out is None:
-            out = torch.empty(q.shape[0], self.cfg.num_heads, self.cfg.v_head_dim, dtype=q.dtype, device=q.device)
+            out = torch.empty((self._n_seqs, self._heads, self._out_dim), dtype=self.io_torch_dtype, device=self.device)
+        else:
+            self._check_io(out, self._n_seqs, self._heads, "out")
         self._check(self._lib.tk_kv_append_decode(self._h, layer, k.data_ptr(), v.data_ptr(), q.data_ptr(),
                                                   out.data_ptr(), self._stream()))
         return out
@@ -314,42 +320,46 @@ class PagedKVCache:
     def rope_append_decode(self, layer: int, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor,
                            theta: float, scaling: float = 1.0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """RoPE(q, k) + append + decode of one layer; q and k are given before rotation."""
-        self._check_io(k, self._n_tokens, self.cfg.num_kv_heads, "k")
-        self._check_io(v, self._n_tokens, self.cfg.num_kv_heads, "v")
-        self._check_io(q, self._n_seqs, self.cfg.num_heads, "q")
+        self._check_io(k, self._n_tokens, self._kv_heads, "k")
+        self._check_io(v, self._n_tokens, self._kv_heads, "v")
+        self._check_io(q, self._n_seqs, self._heads, "q")
         if out is None:
-            out = torch.empty(q.shape[0], self.cfg.num_heads, self.cfg.v_head_dim, dtype=q.dtype, device=q.device)
+            out = torch.empty((self._n_seqs, self._heads, self._out_dim), dtype=self.io_torch_dtype, device=self.device)
+        else:
+            self._check_io(out, self._n_seqs, self._heads, "out")
         self._check(self._lib.tk_kv_rope_append_decode(self._h, layer, k.data_ptr(), v.data_ptr(), q.data_ptr(),
                                                        out.data_ptr(), theta, scaling, self._stream()))
         return out
 
     def decode_partial(self, layer: int, q: torch.Tensor, partial: Optional[torch.Tensor] = None) -> torch.Tensor:
         """-> [n_seqs, H, D+2] f32: unnormalised o, then m, then l."""
-        self._check_io(q, self._n_seqs, self.cfg.num_heads, "q")
+        self._check_io(q, self._n_seqs, self._heads, "q")
         if partial is None:
-            partial = torch.empty(self._n_seqs, self.cfg.num_heads, self.cfg.v_head_dim + 2,
+            partial = torch.empty(self._n_seqs, self._heads, self._out_dim + 2,
                                   dtype=torch.float32, device=self.device)
         self._check(self._lib.tk_kv_decode_partial(self._h, layer, q.data_ptr(), partial.data_ptr(), self._stream()))
         return partial
 
     def decode_multi(self, layer: int, q: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal attention for every token the step appended: q, out [n_tokens, H, D] (rows as in append)."""
-        self._check_io(q, self._n_tokens, self.cfg.num_heads, "q")
+        self._check_io(q, self._n_tokens, self._heads, "q")
         if out is None:
-            out = torch.empty(self._n_tokens, self.cfg.num_heads, self.cfg.v_head_dim, dtype=self.io_torch_dtype,
-                              device=self.device)
+            out = torch.empty((self._n_tokens, self._heads, self._out_dim), dtype=self.io_torch_dtype, device=self.device)
+        else:
+            self._check_io(out, self._n_tokens, self._heads, "out")
         self._check(self._lib.tk_kv_decode_multi(self._h, layer, q.data_ptr(), out.data_ptr(), self._stream()))
         return out
 
     def append_decode_multi(self, layer: int, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor,
                             out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """append(k, v) of the step's tokens, then decode_multi(q): one library call per layer."""
-        self._check_io(k, self._n_tokens, self.cfg.num_kv_heads, "k")
-        self._check_io(v, self._n_tokens, self.cfg.num_kv_heads, "v")
-        self._check_io(q, self._n_tokens, self.cfg.num_heads, "q")
+        self._check_io(k, self._n_tokens, self._kv_heads, "k")
+        self._check_io(v, self._n_tokens, self._kv_heads, "v")
+        self._check_io(q, self._n_tokens, self._heads, "q")
         if out is None:
-            out = torch.empty(self._n_tokens, self.cfg.num_heads, self.cfg.v_head_dim, dtype=self.io_torch_dtype,
-                              device=self.device)
+            out = torch.empty((self._n_tokens, self._heads, self._out_dim), dtype=self.io_torch_dtype, device=self.device)
+        else:
+            self._check_io(out, self._n_tokens, self._heads, "out")
         self._check(self._lib.tk_kv_append_decode_multi(self._h, layer, k.data_ptr(), v.data_ptr(), q.data_ptr(),
                                                         out.data_ptr(), self._stream()))
         return out
@@ -357,9 +367,9 @@ class PagedKVCache:
     def decode_exchange(self, layer: int, q: torch.Tensor, exchange, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention over the tokens of EVERY rank of `exchange` (a dist.PeerExchange): this rank's
         partial rows, then one kernel that swaps rows with the peers over NVLink and combines."""
-        self._check_io(q, self._n_seqs, self.cfg.num_heads, "q")
+        self._check_io(q, self._n_seqs, self._heads, "q")
         if out is None:
-            out = torch.empty(self._n_seqs, self.cfg.num_heads, self.cfg.v_head_dim, dtype=self.io_torch_dtype,
+            out = torch.empty(self._n_seqs, self._heads, self._out_dim, dtype=self.io_torch_dtype,
                               device=self.device)
         self._check(self._lib.tk_kv_decode_exchange(self._h, layer, q.data_ptr(), exchange._h, out.data_ptr(),
                                                     self._stream()))
