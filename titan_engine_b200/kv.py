@@ -241,6 +241,12 @@ class PagedKVCache:
         if t.numel() != rows * heads * self._dims[what]:
             raise KvError(L.TK_INVALID_ARG, f"{what}: expected [{rows}, {heads}, {self._dims[what]}]")
 
+    def _new_out(self, q: torch.Tensor, rows: int) -> torch.Tensor:
+        """Output rows for queries that _check_io has seen."""
+        if q.dim() == 3 and self._out_dim == self._dims["q"]:
+            return torch.empty_like(q)                      # (half the host time of naming shape, type and device)
+        return q.new_empty((rows, self._heads, self._out_dim))
+
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor,
                slots_out: Optional[torch.Tensor] = None) -> None:
         """k, v: [n_tokens, Hkv, D] on the device, io dtype; the step's tokens in order."""
@@ -263,19 +269,24 @@ class PagedKVCache:
             out_dtype = self.io_torch_dtype
         elif out_dtype not in (self.io_torch_dtype, torch.float32):
             raise KvError(L.TK_INVALID_ARG, f"read: out dtype must be {self.io_torch_dtype} or torch.float32")
+        n = len(seq_ids)
         if start is None:
-            start = [0] * len(seq_ids)
+            start = [0] * n
         if count is None:
-            count = [self.seq_len(int(s)) - int(a) for s, a in zip(seq_ids, start)]
-        if not len(seq_ids) == len(start) == len(count):
+            count = [self.seq_len(int(q)) - int(a) for q, a in zip(seq_ids, start)]
+        if not n == len(start) == len(count):
             raise KvError(L.TK_INVALID_ARG, "read: start and count need one entry for each sequence")
         rows = int(sum(count))
-        if rows and not 0 <= min(count) <= max(count) <= self._pool_tokens:
+        if not 0 <= rows <= n * self._pool_tokens:          # (the library checks each range)
             raise KvError(L.TK_INVALID_ARG, "read: ranges must lie inside live sequences' tokens")
-        (s, s_at), (a, a_at), (n, n_at) = _ints(seq_ids), _ints(start), _ints(count)
-        k = torch.empty((rows, self._kv_heads, self._dims["k"]), dtype=out_dtype, device=self.device)
-        v = torch.empty((rows, self._kv_heads, self._dims["v"]), dtype=out_dtype, device=self.device)
-        self._check(self._lib.tk_kv_read(self._h, layer, len(s), s_at, a_at, n_at, k.data_ptr(), v.data_ptr(),
+        ints, at = _ints([*seq_ids, *start, *count])
+        h, dk, dv = self._kv_heads, self._dims["k"], self._dims["v"]
+        if dk == dv:
+            k, v = torch.empty((2, rows, h, dk), dtype=out_dtype, device=self.device).unbind(0)
+        else:
+            k = torch.empty((rows, h, dk), dtype=out_dtype, device=self.device)
+            v = torch.empty((rows, h, dv), dtype=out_dtype, device=self.device)
+        self._check(self._lib.tk_kv_read(self._h, layer, n, at, at + 4 * n, at + 8 * n, k.data_ptr(), v.data_ptr(),
                                          L.TK_FP32 if out_dtype == torch.float32 else self.cfg.io_dtype, self._stream()))
         return k, v
 
@@ -283,7 +294,7 @@ class PagedKVCache:
         """q: [n_seqs, H, D] -> out [n_seqs, H, D], io dtype."""
         self._check_io(q, self._n_seqs, self._heads, "q")
         if out is None:
-            out = torch.empty(q.shape[0], self._heads, self._out_dim, dtype=q.dtype, device=q.device)
+            out = self._new_out(q, self._n_seqs)
         self._check_io(out, self._n_seqs, self._heads, "out")
         self._check(self._lib.tk_kv_decode(self._h, layer, q.data_ptr(), out.data_ptr(), self._stream()))
         return out
@@ -310,7 +321,7 @@ class PagedKVCache:
         self._check_io(v, self._n_tokens, self._kv_heads, "v")
         self._check_io(q, self._n_seqs, self._heads, "q")
         if out is None:
-            out = torch.empty((self._n_seqs, self._heads, self._out_dim), dtype=self.io_torch_dtype, device=self.device)
+            out = self._new_out(q, self._n_seqs)
         else:
             self._check_io(out, self._n_seqs, self._heads, "out")
         self._check(self._lib.tk_kv_append_decode(self._h, layer, k.data_ptr(), v.data_ptr(), q.data_ptr(),
@@ -324,7 +335,7 @@ class PagedKVCache:
         self._check_io(v, self._n_tokens, self._kv_heads, "v")
         self._check_io(q, self._n_seqs, self._heads, "q")
         if out is None:
-            out = torch.empty((self._n_seqs, self._heads, self._out_dim), dtype=self.io_torch_dtype, device=self.device)
+            out = self._new_out(q, self._n_seqs)
         else:
             self._check_io(out, self._n_seqs, self._heads, "out")
         self._check(self._lib.tk_kv_rope_append_decode(self._h, layer, k.data_ptr(), v.data_ptr(), q.data_ptr(),
@@ -344,7 +355,7 @@ class PagedKVCache:
         """Causal attention for every token the step appended: q, out [n_tokens, H, D] (rows as in append)."""
         self._check_io(q, self._n_tokens, self._heads, "q")
         if out is None:
-            out = torch.empty((self._n_tokens, self._heads, self._out_dim), dtype=self.io_torch_dtype, device=self.device)
+            out = self._new_out(q, self._n_tokens)
         else:
             self._check_io(out, self._n_tokens, self._heads, "out")
         self._check(self._lib.tk_kv_decode_multi(self._h, layer, q.data_ptr(), out.data_ptr(), self._stream()))
@@ -357,7 +368,7 @@ class PagedKVCache:
         self._check_io(v, self._n_tokens, self._kv_heads, "v")
         self._check_io(q, self._n_tokens, self._heads, "q")
         if out is None:
-            out = torch.empty((self._n_tokens, self._heads, self._out_dim), dtype=self.io_torch_dtype, device=self.device)
+            out = self._new_out(q, self._n_tokens)
         else:
             self._check_io(out, self._n_tokens, self._heads, "out")
         self._check(self._lib.tk_kv_append_decode_multi(self._h, layer, k.data_ptr(), v.data_ptr(), q.data_ptr(),
