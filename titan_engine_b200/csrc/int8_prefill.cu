@@ -13,10 +13,14 @@
 //   MMA thread       S = Q K^T (M 128, N 64) and O += W V (M 128, N D, W from tensor memory) for both halves
 //   16 softmax warps 16 rows each, as fragments: a speculative pass against the current reference, redone when a score exceeds it
 //                    by 2^8 or the block is cut; only then O is rescaled (prefill_tc.cu describes the scheme)
-// The expansion is what an 8-bit cache costs over a 16-bit one: 2 D values per token, shared here by 256 rows - about an
-// eighth of the issue slots - where two CTAs of 128 rows would each do it.  Tensor memory: per half two S buffers of 64
-// columns and O of D: all 512 columns at D = 128.
-// Bound: tensor pipe and special-function unit together, 512 clocks each per 128 x 64 block at D = 128.
+// The expansion is what an 8-bit cache costs over a 16-bit one: 2 D values per token - about 800 warp instructions a block of
+// some 6200 - shared here by 256 rows where two CTAs of 128 rows would each do it.  Tensor memory: per half two S buffers of
+// 64 columns and O of D: all 512 columns at D = 128.
+// Bound: a block of 256 rows x 64 tokens at D = 128 is 1024 clocks of the tensor pipe and 1024 of the special-function unit.  It
+// takes about 2480: the shared-memory pipe is used by loads and stores for half of them (1337 wavefronts, 768 of which are the
+// softmax warps reading the three numbers of each token) and feeds the operands of the MMAs for 41 %; issue slots 63 %, ALU
+// 46 %, special-function unit 42 %.  Measured: 0.39-0.41 ms for 8 chunks of 1024 tokens on contexts up to 2843 (32 heads, 8 kv
+// heads), 1.12-1.27 ms = 870-980 TFLOP/s for a prompt of 8192 (64 heads).
 // Every wait is bounded; on expiry the status word is set, nothing is written, and the CTA waits for its copies and frees its
 // tensor memory before it returns.  No cluster, no multicast, this GPU's memory only.
 #include "int8_cache.cuh"
@@ -33,10 +37,10 @@ namespace {
 constexpr int kPfRows = kPrefillRowsInt8;       // 256: two halves of kTcRows
 constexpr int kPfBlock = 64;                    // context tokens per block (4 pages)
 constexpr int kPfRaw = 4;                       // stages of raw tiles: K is expanded two blocks ahead of V
-constexpr int kPfGroups = 1;                     // 16-row groups per softmax warp
+constexpr int kPfGroups = 1;                    // 16-row groups per softmax warp: 1 (16 warps) 0.403 / 1.165 ms, 2 (8 warps) 0.417 / 1.282
 constexpr int kPfSoftWarps = kPfRows / (16 * kPfGroups), kPfExpWarps = 4;
 constexpr int kPfMmaWarp = kPfSoftWarps + kPfExpWarps, kPfLoadWarp = kPfMmaWarp + 2;    // an MMA warp for each half
-constexpr int kPfThreads = (kPfSoftWarps + 8) * 32;                  // 6 warpgroups: 4 of softmax, expanders, (two MMA warps, loader, an idle warp)
+constexpr int kPfThreads = (kPfSoftWarps + 8) * 32;     // 6 warpgroups: 4 of softmax, expanders, (two MMA warps, loader, an idle warp)
 constexpr int kPfSoftThreads = kPfSoftWarps * 32;
 constexpr int kPfRegsSoft = 96, kPfRegsOther = 48;
 constexpr int kPfExpThreads = kPfExpWarps * 32;

@@ -12,7 +12,7 @@ constexpr int kTcRows = 128;                    // rows per tile = TMEM lanes
 
 // One lane of a converged warp: a role that issues MMAs runs its loop with the whole warp and elects a lane per issue, so that
 // descriptors and addresses stay warp-uniform (a loop inside `if (lane == 0)` moves each of them to the uniform registers
-// the instruction wants: 130 clocks per MMA measured, against about 30).
+// the instruction wants: 130 clocks per MMA of M 128, N 64 measured, against 60).
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
