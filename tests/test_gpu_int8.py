@@ -579,6 +579,40 @@ def test_captured_step_replays_next_to_eager_calls_on_another_stream():
         other.check_decode(o, [t], qo)
 
 
+def test_captured_chunk_keeps_its_workspace_when_a_larger_step_grows_it():
+    """A split chunk whose workspace the handle has to allocate: refused inside a capture, which lives on; captured after one
+    eager run; a larger step then takes a larger workspace and the graph still has its own."""
+    from titan_engine_b200 import KvError
+    p = Pair(8, 2, 128, pages=512, mpps=256)
+    a, b, new = p.alloc(), p.alloc(), 60
+    p.grow([a, b], [3900, 3300])
+    k, v = p.begin([a], [new])
+    q = p.rows(new, 8)
+    graph, first = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(first):
+        p.c.append(0, k, v)
+        with pytest.raises(KvError, match="workspace"):
+            p.c.decode_multi(0, q)
+    first.replay()
+    want = p.c.decode_multi(0, q).clone()
+    p.check_chunk(want, [a], [new], q)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        got = p.c.decode_multi(0, q)
+    kb, vb = p.begin([b], [2 * new])                        # twice the rows
+    qb = p.rows(2 * new, 8)
+    p.check_chunk(p.c.append_decode_multi(0, kb, vb, qb), [b], [2 * new], qb)
+    p.c.truncate(a, 3900)
+    p.c.step_begin([a], [new])                              # the captured step again; the rows that truncate cut are gone
+    p.c.append(0, k, v)
+    for _ in range(2):
+        got.zero_()
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
 def test_pending_timeout_leaves_the_output_alone():
     p = Pair(8, 2, 128)
     s = p.alloc()

@@ -157,6 +157,7 @@ struct tk_kv {
     float* d_xpartial = nullptr;         // this rank's merged partial rows for tk_kv_decode_exchange
     float* d_multi_partials = nullptr;   // split-KV rows of multi-token steps that outgrow d_partials
     size_t multi_partials_floats = 0;
+    std::vector<float*> old_multi_partials;   // smaller ones that a captured graph may still name; freed with the handle
     bool mla_mma = false;
 
     // cold tier (hot_window > 0): pages older than the window live in pinned host memory and are
@@ -231,6 +232,7 @@ void release(tk_kv* h) {
         if (h->d_partials) cudaFree(h->d_partials);
         if (h->d_xpartial) cudaFree(h->d_xpartial);
         if (h->d_multi_partials) cudaFree(h->d_multi_partials);
+        for (float* p : h->old_multi_partials) cudaFree(p);
         if (h->d_status) cudaFree(h->d_status);
         if (h->d_counters) cudaFree(h->d_counters);
         if (h->d_pf_counters) cudaFree(h->d_pf_counters);
@@ -1065,16 +1067,24 @@ int tk_kv_decode_partial(tk_kv* h, int32_t layer, const void* q, float* partial,
 }
 
 // Split-KV workspace of a multi-token step: the handle's own when `floats` fit it, else a buffer that is
-// allocated (and grown) on demand - the one device allocation a step may make after creation.
+// allocated (and grown) on demand - the one device allocation a step may make after creation.  A buffer that is outgrown
+// lives on with the handle (each is twice its predecessor, so they add up to less than the current one): a graph captured
+// with it keeps its pointer.  A capture cannot allocate: a step that would grow the buffer is refused there, the capture lives on.
 static float* multi_workspace(tk_kv* h, size_t floats, cudaStream_t stream) {
     if (floats <= (size_t)h->max_partial_rows * h->cfg.num_heads * (h->cfg.v_head_dim + 2)) return h->d_partials;
     if (floats > h->multi_partials_floats) {
-        if (cudaSetDevice(h->device) != cudaSuccess) { fail(h, TK_CUDA_ERROR, "cudaSetDevice failed"); return nullptr; }
-        if (h->d_multi_partials) { cudaStreamSynchronize(stream); cudaFree(h->d_multi_partials); }
-        h->d_multi_partials = nullptr; h->multi_partials_floats = 0;
-        cudaError_t e = cudaMalloc((void**)&h->d_multi_partials, floats * sizeof(float));
-        if (e != cudaSuccess) { fail(h, TK_CUDA_ERROR, "split-KV workspace of %zu bytes: %s", floats * sizeof(float), cudaGetErrorString(e)); return nullptr; }
-        h->multi_partials_floats = floats;
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(stream, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone) {
+            fail(h, TK_CUDA_ERROR, "decode_multi: the step needs a larger split-KV workspace, which a stream capture cannot allocate: run it once before");
+            return nullptr;
+        }
+        const size_t grown = std::max(floats, 2 * h->multi_partials_floats);
+        float* p = nullptr;
+        cudaError_t e = cudaMalloc((void**)&p, grown * sizeof(float));
+        if (e != cudaSuccess) { fail(h, TK_CUDA_ERROR, "split-KV workspace of %zu bytes: %s", grown * sizeof(float), cudaGetErrorString(e)); return nullptr; }
+        if (h->d_multi_partials) h->old_multi_partials.push_back(h->d_multi_partials);
+        h->d_multi_partials = p;
+        h->multi_partials_floats = grown;
     }
     return h->d_multi_partials;
 }
