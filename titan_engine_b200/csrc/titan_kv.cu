@@ -223,6 +223,16 @@ int fail(tk_kv* h, int status, const char* fmt, ...) {
             return fail(h, TK_CUDA_ERROR, "%s failed: %s", #call, cudaGetErrorString(e_));       \
     } while (0)
 
+// Makes the handle's device current for a launch (the default stream belongs to whichever device is) and puts the caller's back.
+struct OnDevice {
+    int back = -1;
+    explicit OnDevice(int device) {
+        int now = -1;
+        if (cudaGetDevice(&now) == cudaSuccess && now != device && cudaSetDevice(device) == cudaSuccess) back = now;
+    }
+    ~OnDevice() { if (back >= 0) cudaSetDevice(back); }
+};
+
 void release(tk_kv* h) {
     if (!h) return;
     if (!h->host_only) {
@@ -876,6 +886,7 @@ int tk_kv_append(tk_kv* h, int32_t layer, const void* k, const void* v, int64_t*
     if (!h->have_step) return fail(h, TK_INVALID_ARG, "append: no step in progress (call tk_kv_step_begin)");
     if (h->dev.n_tokens == 0) return TK_OK;
     if (!k || !v) return fail(h, TK_INVALID_ARG, "append: null k/v");
+    const OnDevice current(h->device);
     int n = 0;
     cudaError_t e = tk::launch_append(h->geo, h->layer(layer), h->dev, h->d_table, k, v, slots_out,
                                       (cudaStream_t)stream, &n);
@@ -884,18 +895,11 @@ int tk_kv_append(tk_kv* h, int32_t layer, const void* k, const void* v, int64_t*
     return TK_OK;
 }
 
-// Rows of token ranges, dequantised, in the order of the ranges.
-int tk_kv_read(tk_kv* h, int32_t layer, int32_t n_ranges, const int32_t* seq_ids, const int32_t* start, const int32_t* count,
-               void* k_out, void* v_out, int32_t out_dtype, void* stream) {
-    if (!h || layer < 0 || layer >= h->cfg.num_layers || n_ranges < 0 || (n_ranges > 0 && !seq_ids)) return TK_INVALID_ARG;
-    if (const int fs = host_flush(h)) return fs;               // launches the host-buffer calls still hold back come first
-    if (h->host_only) return fail(h, TK_CUDA_ERROR, "read: handle has no device (bookkeeping only)");
-    if (out_dtype != TK_FP32 && out_dtype != h->cfg.io_dtype)
-        return fail(h, TK_INVALID_ARG, "read: out dtype must be FP32 or the handle's io dtype");
-    std::lock_guard<std::mutex> lock(h->mgr_mu);
+// The pages that hold the ranges' rows, in order; the caller holds mgr_mu.
+static int read_items(tk_kv* h, int n_ranges, const int32_t* seq_ids, const int32_t* start, const int32_t* count,
+                      std::vector<tk::ReadItem>* items) {
     const int ps = h->cfg.page_size;
     const bool fp8 = h->cfg.dtype == TK_FP8_E4M3;
-    std::vector<tk::ReadItem> items;
     int64_t rows = 0;
     for (int i = 0; i < n_ranges; i++) {
         const int seq = seq_ids[i], len = h->mgr->seq_len(seq);
@@ -909,13 +913,32 @@ int tk_kv_read(tk_kv* h, int32_t layer, int32_t n_ranges, const int32_t* seq_ids
             const int r = (int)(at % ps), m = (int)std::min<int64_t>(ps - r, lo + n - at);
             const int32_t page = at < sealed ? pages[at / ps] : -1 - seq;
             if (at < sealed && page < 0) return fail(h, TK_UNSUPPORTED, "read: token %lld of sequence %d lies in a cold page", (long long)at, seq);
-            items.push_back(tk::ReadItem{page, r, m, (int)rows});
+            items->push_back(tk::ReadItem{page, r, m, (int)rows});
             rows += m;
             at += m;
         }
     }
-    if (rows == 0) return TK_OK;
+    return TK_OK;
+}
+
+// Rows of token ranges, dequantised, in the order of the ranges.
+int tk_kv_read(tk_kv* h, int32_t layer, int32_t n_ranges, const int32_t* seq_ids, const int32_t* start, const int32_t* count,
+               void* k_out, void* v_out, int32_t out_dtype, void* stream) {
+    if (!h || layer < 0 || layer >= h->cfg.num_layers || n_ranges < 0 || (n_ranges > 0 && !seq_ids)) return TK_INVALID_ARG;
+    if (const int fs = host_flush(h)) return fs;               // launches the host-buffer calls still hold back come first
+    if (h->host_only) return fail(h, TK_CUDA_ERROR, "read: handle has no device (bookkeeping only)");
+    if (out_dtype != TK_FP32 && out_dtype != h->cfg.io_dtype)
+        return fail(h, TK_INVALID_ARG, "read: out dtype must be FP32 or the handle's io dtype");
+    std::lock_guard<std::mutex> lock(h->mgr_mu);
+    std::vector<tk::ReadItem> items;
+    try {
+        if (const int st = read_items(h, n_ranges, seq_ids, start, count, &items)) return st;
+    } catch (const std::bad_alloc&) {
+        return fail(h, TK_INVALID_ARG, "read: the ranges' list of pages does not fit the host's memory: read fewer in one call");
+    }
+    if (items.empty()) return TK_OK;
     if (!k_out || !v_out) return fail(h, TK_INVALID_ARG, "read: null output");
+    const OnDevice current(h->device);
     int n = 0;
     const cudaError_t e = tk::launch_read_rows(h->geo, h->layer(layer), items.data(), (int)items.size(), k_out, v_out, out_dtype,
                                                (cudaStream_t)stream, &n);
@@ -933,6 +956,7 @@ static int decode_impl(tk_kv* h, int layer, const void* q, void* out, float* par
     if (!h->have_step) return fail(h, TK_INVALID_ARG, "decode: no step in progress (call tk_kv_step_begin)");
     if (h->dev.n_seqs == 0) return TK_OK;
     if (!q || (!out && !partial_out)) return fail(h, TK_INVALID_ARG, "decode: null q/out");
+    const OnDevice current(h->device);
     tk::LayerPtrs lp = h->layer(layer);
     cudaError_t e = cudaSuccess;
     const bool cold = h->mgr->cold_enabled() && h->mgr->cold_high_water() > 0;
@@ -1038,6 +1062,7 @@ int tk_kv_rope_append_decode(tk_kv* h, int32_t layer, const void* k, const void*
     if (h->host_only) return fail(h, TK_CUDA_ERROR, "rope_append_decode: handle has no device (bookkeeping only)");
     if (!h->have_step) return fail(h, TK_INVALID_ARG, "rope_append_decode: no step in progress (call tk_kv_step_begin)");
     if (!q || !out || (h->dev.n_tokens > 0 && (!k || !v))) return fail(h, TK_INVALID_ARG, "rope_append_decode: null argument");
+    const OnDevice current(h->device);
     const bool fusable = h->use_mma && h->cfg.dtype != TK_FP8_E4M3 && h->plan.one_token_steps &&
                          h->dev.chunk_tokens <= 2048 && h->dev.n_tokens > 0 && h->dev.n_seqs > 0 &&
                          !h->plan.has_empty_seq && !(h->cfg.dtype == TK_INT8 && h->plan.capped);
@@ -1100,6 +1125,7 @@ static int decode_multi_impl(tk_kv* h, int32_t layer, const void* q, void* out, 
     if (!h->have_step) return fail(h, TK_INVALID_ARG, "decode_multi: no step in progress (call tk_kv_step_begin)");
     if (h->dev.n_seqs == 0) return TK_OK;
     if (!q || !out) return fail(h, TK_INVALID_ARG, "decode_multi: null q/out");
+    const OnDevice current(h->device);
     const tk::StepPlan& p = h->plan;
     if (p.nq_min < 1) return fail(h, TK_INVALID_ARG, "decode_multi: every sequence of the step must append at least one token");
     if (h->cfg.dtype == TK_INT8) {
