@@ -51,7 +51,7 @@ enum { TK_FP32 = 0, TK_FP16 = 1, TK_BF16 = 2, TK_FP8_E4M3 = 3 };
  * cut (tk_kv_truncate), forked and attended to (tk_kv_step_begin_capped, tk_kv_decode_multi) at any token.  head_dim 64
  * or 128 (v_head_dim equal), page_size 16, chunk_tokens at most 2048, no cold tier, no TK_DECODE_SIMT.  Pool of a layer:
  * [num_pages][Hkv] tiles of 32 * head_dim + 128 bytes: K codes [16][D], V codes [16][D], f32 K scales [16], V scales
- * [16]; a code is stored as the unsigned byte code + 128. */
+ * [16]; a code is stored as the unsigned byte code + 128.  k, v, q and out must be 16-byte aligned (a split-KV partial 8-byte). */
 enum { TK_INT8 = 32 };
 
 /* which decode kernel tk_kv_decode launches */
@@ -221,7 +221,7 @@ int tk_kv_append(tk_kv* h, int32_t layer, const void* k, const void* v, int64_t*
  * inside its sequence's tokens; a sequence may be named several times.  Reads what the layer's appends before it on
  * `stream` have written, under the page table of the moment of the call (a fork or truncation since the last step counts);
  * it needs no step, uploads nothing and may be captured into a graph, which then replays with those pages.
- * TK_UNSUPPORTED for a token in a cold page.  (The reference hands out the slab: KVCache::k_cache / v_cache,
+ * Outputs must be 16-byte aligned.  TK_UNSUPPORTED for a token in a cold page.  (The reference hands out the slab: KVCache::k_cache / v_cache,
  * src/inference/kv_cache.h:42-48.) */
 int tk_kv_read(tk_kv* h, int32_t layer, int32_t n_ranges, const int32_t* seq_ids, const int32_t* start, const int32_t* count,
                void* k_out, void* v_out, int32_t out_dtype, void* stream);

@@ -227,6 +227,30 @@ def test_read_refusals():
         p.c.read(3, [a])
 
 
+def test_unaligned_views_are_refused():
+    """A contiguous view that starts inside a 16-byte vector, for every tensor of every call."""
+    from titan_engine_b200 import KvError
+    p = Pair(4, 2, 64)
+    a = p.alloc()
+    p.grow([a], [20])
+    k, v = p.begin([a], [1])
+    q = p.rows(1, 4)
+
+    def off(x):
+        return torch.cat([x.flatten()[:1], x.flatten()])[1:].view(x.shape)
+
+    calls = {"append": (p.c.append, [k, v]), "decode": (p.c.decode, [q, q.clone()]),
+             "append_decode": (p.c.append_decode, [k, v, q, q.clone()]), "decode_multi": (p.c.decode_multi, [q, q.clone()]),
+             "append_decode_multi": (p.c.append_decode_multi, [k, v, q, q.clone()])}
+    for name, (call, args) in calls.items():
+        for i in range(len(args)):
+            with pytest.raises(KvError, match="aligned"):
+                call(0, *[off(x) if i == j else x for j, x in enumerate(args)])
+    with pytest.raises(KvError, match="aligned"):
+        p.c.rope_append_decode(0, off(k), v, q, 10000.0)
+    p.check_decode(p.c.append_decode(0, k, v, q), [a], q)
+
+
 def test_read_after_fork_and_truncation_needs_no_step():
     p = Pair(8, 2, 64)
     a = p.alloc()
@@ -548,6 +572,44 @@ def test_rope_and_host_buffer_paths():
     out = torch.empty(2, 8, 64, dtype=torch.float16).pin_memory()
     p.c.append_decode_host(0, hk, hv, hq, out)
     assert torch.equal(out, want.cpu())
+
+
+@pytest.mark.parametrize("io,D", [("bf16", 64), ("bf16", 128), ("fp16", 64), ("fp16", 128)])
+def test_rope_append_decode_against_64_bits(io, D):
+    """The rows that rope_append_decode leaves in the cache, and its result, against rotations in 64 bits.  An angle (position x
+    inverse frequency) carries a few FP32 roundings, far below a step of the 16-bit type: a rotated value is the nearest 16-bit
+    number or its neighbour, a distance of at most one step u = eps of the type, relative.  A stored row is then within
+    half a code plus u of the rotation; a score of query q and key k within d = u sum |q_i k_i| / sqrt(D), which moves every
+    probability by at most a factor e^(2 d)."""
+    p = Pair(8, 2, D, io)
+    seqs, held = [p.alloc() for _ in range(3)], [0, 20, 300]
+    p.grow(seqs, held)
+    k, v = p.begin(seqs, [1, 1, 1])
+    q = p.rows(3, 8)
+    got = p.c.rope_append_decode(0, k, v, q, 10000.0).float().cpu().numpy().astype(np.float64)
+    u = torch.finfo(TYPES[io]).eps
+
+    def rot(x, pos):                                        # one token's heads [h, D]
+        x = x.double().cpu().numpy()
+        ang = pos / 10000.0 ** (np.arange(0, D, 2) / D)
+        y = np.empty_like(x)
+        y[:, 0::2] = x[:, 0::2] * np.cos(ang) - x[:, 1::2] * np.sin(ang)
+        y[:, 1::2] = x[:, 0::2] * np.sin(ang) + x[:, 1::2] * np.cos(ang)
+        return y
+
+    for i, (s, n) in enumerate(zip(seqs, held)):
+        ks, vs = (x.double().cpu().numpy() for x in p.c.read(0, [s], out_dtype=torch.float32))
+        want = rot(k[i], n)
+        amax = np.abs(want).max(-1, keepdims=True) * (1 + u)
+        assert (np.abs(ks[n] - want) <= amax * (0.51 / 127 + u)).all()
+        np.testing.assert_array_equal(vs[n], p.v[s][n])
+        np.testing.assert_array_equal(ks[:n], p.k[s][:n])
+        qr = torch.from_numpy(rot(q[i], n)).to(TYPES[io]).double().numpy()
+        out, bound = attention(qr[None], ks, vs, [n + 1], io)
+        kk, vv = np.repeat(ks, 4, 1), np.repeat(np.abs(vs), 4, 1)              # [tokens, H, D]
+        d = (u * np.abs(qr[None] * kk).sum(-1) / np.sqrt(D)).max(0)            # per head
+        top = (np.exp(2 * d) - 1)[:, None] * vv.max(0)
+        assert (np.abs(got[i] - out[0]) <= bound[0] + top).all()
 
 
 def test_captured_step_replays_next_to_eager_calls_on_another_stream():

@@ -109,6 +109,27 @@ def test_compute_calls_need_a_device():
     assert c._lib.tk_kv_decode_multi(c._h, 0, None, None, None) == L.TK_CUDA_ERROR
 
 
+def test_unaligned_tensors_are_refused_before_anything_runs():
+    """The kernels move 16-byte vectors; an address is looked at, never read."""
+    c = _cache()
+    c.step_begin([c.seq_alloc()], [1])
+    lib, h, at, off = c._lib, c._h, 4096, 4096 + 2
+    for i in range(2):
+        kv = [off if i == j else at for j in range(2)]
+        assert lib.tk_kv_append(h, 0, *kv, None, None) == L.TK_INVALID_ARG
+        assert lib.tk_kv_decode(h, 0, *kv, None) == L.TK_INVALID_ARG
+        assert lib.tk_kv_decode_multi(h, 0, *kv, None) == L.TK_INVALID_ARG
+        assert lib.tk_kv_append_decode(h, 0, at, at, *kv, None) == L.TK_INVALID_ARG
+        assert lib.tk_kv_append_decode_multi(h, 0, at, at, *kv, None) == L.TK_INVALID_ARG
+        assert lib.tk_kv_append_decode_multi(h, 0, *kv, at, at, None) == L.TK_INVALID_ARG
+        assert lib.tk_kv_read(h, 0, 0, None, None, None, *kv, L.TK_BF16, None) == L.TK_INVALID_ARG
+    assert lib.tk_kv_decode_partial(h, 0, at, at + 4, None) == L.TK_INVALID_ARG
+    for i in range(4):
+        args = [off if i == j else at for j in range(4)]
+        assert lib.tk_kv_rope_append_decode(h, 0, *args, 10000.0, 1.0, None) == L.TK_INVALID_ARG
+    assert lib.tk_kv_decode(h, 0, at, at, None) == L.TK_CUDA_ERROR          # aligned: the next check answers
+
+
 @pytest.mark.parametrize("shape", [(32, 8), (64, 8), (16, 1), (6, 3), (4, 4)])
 @pytest.mark.parametrize("lens", [
     ([0, 5000, 33, 0, 40000, 700, 17], [300, 1, 4096, 70, 37, 3, 129]),

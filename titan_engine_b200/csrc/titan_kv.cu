@@ -233,6 +233,9 @@ struct OnDevice {
     ~OnDevice() { if (back >= 0) cudaSetDevice(back); }
 };
 
+// The kernels over INT8 pools and the read-back move rows as 16-byte vectors (split-KV rows of D + 2 values as 8-byte ones).
+bool unaligned(const void* p, size_t to = 16) { return ((uintptr_t)p & (to - 1)) != 0; }
+
 void release(tk_kv* h) {
     if (!h) return;
     if (!h->host_only) {
@@ -882,6 +885,7 @@ int tk_kv_step_prefill_plan(const tk_kv* h, int32_t cap, int32_t* items, int32_t
 int tk_kv_append(tk_kv* h, int32_t layer, const void* k, const void* v, int64_t* slots_out, void* stream) {
     if (!h || layer < 0 || layer >= h->cfg.num_layers) return TK_INVALID_ARG;
     if (const int fs = host_flush(h)) return fs;               // launches the host-buffer calls still hold back come first
+    if (h->cfg.dtype == TK_INT8 && (unaligned(k) || unaligned(v))) return fail(h, TK_INVALID_ARG, "append: k and v must be 16-byte aligned");
     if (h->host_only) return fail(h, TK_CUDA_ERROR, "append: handle has no device (bookkeeping only)");
     if (!h->have_step) return fail(h, TK_INVALID_ARG, "append: no step in progress (call tk_kv_step_begin)");
     if (h->dev.n_tokens == 0) return TK_OK;
@@ -926,6 +930,7 @@ int tk_kv_read(tk_kv* h, int32_t layer, int32_t n_ranges, const int32_t* seq_ids
                void* k_out, void* v_out, int32_t out_dtype, void* stream) {
     if (!h || layer < 0 || layer >= h->cfg.num_layers || n_ranges < 0 || (n_ranges > 0 && !seq_ids)) return TK_INVALID_ARG;
     if (const int fs = host_flush(h)) return fs;               // launches the host-buffer calls still hold back come first
+    if (unaligned(k_out) || unaligned(v_out)) return fail(h, TK_INVALID_ARG, "read: outputs must be 16-byte aligned");
     if (h->host_only) return fail(h, TK_CUDA_ERROR, "read: handle has no device (bookkeeping only)");
     if (out_dtype != TK_FP32 && out_dtype != h->cfg.io_dtype)
         return fail(h, TK_INVALID_ARG, "read: out dtype must be FP32 or the handle's io dtype");
@@ -952,6 +957,8 @@ static int decode_impl(tk_kv* h, int layer, const void* q, void* out, float* par
                        const tk::PeerCtx* peer_ctx = nullptr) {
     if (!h || layer < 0 || layer >= h->cfg.num_layers) return TK_INVALID_ARG;
     if (const int fs = host_flush(h)) return fs;               // launches the host-buffer calls still hold back come first
+    if (h->cfg.dtype == TK_INT8 && (unaligned(q) || unaligned(out) || unaligned(partial_out, 8) || unaligned(fuse_k) || unaligned(fuse_v)))
+        return fail(h, TK_INVALID_ARG, "decode: q, out, k and v must be 16-byte aligned, partial 8-byte");
     if (h->host_only) return fail(h, TK_CUDA_ERROR, "decode: handle has no device (bookkeeping only)");
     if (!h->have_step) return fail(h, TK_INVALID_ARG, "decode: no step in progress (call tk_kv_step_begin)");
     if (h->dev.n_seqs == 0) return TK_OK;
@@ -1039,6 +1046,7 @@ int tk_kv_append_decode(tk_kv* h, int32_t layer, const void* k, const void* v, c
                         void* stream) {
     if (!h || layer < 0 || layer >= h->cfg.num_layers) return TK_INVALID_ARG;
     if (const int fs = host_flush(h)) return fs;               // launches the host-buffer calls still hold back come first
+    if (h->cfg.dtype == TK_INT8 && (unaligned(q) || unaligned(out))) return fail(h, TK_INVALID_ARG, "append_decode: q and out must be 16-byte aligned");
     if (h->host_only) return fail(h, TK_CUDA_ERROR, "append_decode: handle has no device (bookkeeping only)");
     if (!h->have_step) return fail(h, TK_INVALID_ARG, "append_decode: no step in progress (call tk_kv_step_begin)");
     // 16-bit storage: the new row goes into the page the kernel is about to read.  FP8 storage: it
@@ -1059,6 +1067,8 @@ int tk_kv_append_decode(tk_kv* h, int32_t layer, const void* k, const void* v, c
 int tk_kv_rope_append_decode(tk_kv* h, int32_t layer, const void* k, const void* v, const void* q, void* out,
                              float theta, float scaling, void* stream) {
     if (!h || layer < 0 || layer >= h->cfg.num_layers) return TK_INVALID_ARG;
+    if (h->cfg.dtype == TK_INT8 && (unaligned(q) || unaligned(out) || unaligned(k) || unaligned(v)))
+        return fail(h, TK_INVALID_ARG, "rope_append_decode: q, out, k and v must be 16-byte aligned");
     if (h->host_only) return fail(h, TK_CUDA_ERROR, "rope_append_decode: handle has no device (bookkeeping only)");
     if (!h->have_step) return fail(h, TK_INVALID_ARG, "rope_append_decode: no step in progress (call tk_kv_step_begin)");
     if (!q || !out || (h->dev.n_tokens > 0 && (!k || !v))) return fail(h, TK_INVALID_ARG, "rope_append_decode: null argument");
@@ -1121,6 +1131,7 @@ static int decode_multi_impl(tk_kv* h, int32_t layer, const void* q, void* out, 
     if (const int fs = host_flush(h)) return fs;               // launches the host-buffer calls still hold back come first
     if (out_dtype != TK_FP32 && out_dtype != h->cfg.io_dtype)
         return fail(h, TK_INVALID_ARG, "decode_multi: out dtype must be FP32 or the handle's io dtype");
+    if (h->cfg.dtype == TK_INT8 && (unaligned(q) || unaligned(out))) return fail(h, TK_INVALID_ARG, "decode_multi: q and out must be 16-byte aligned");
     if (h->host_only) return fail(h, TK_CUDA_ERROR, "decode_multi: handle has no device (bookkeeping only)");
     if (!h->have_step) return fail(h, TK_INVALID_ARG, "decode_multi: no step in progress (call tk_kv_step_begin)");
     if (h->dev.n_seqs == 0) return TK_OK;
@@ -1217,6 +1228,7 @@ int tk_kv_decode_multi_ex(tk_kv* h, int32_t layer, const void* q, void* out, int
 
 int tk_kv_append_decode_multi(tk_kv* h, int32_t layer, const void* k, const void* v, const void* q, void* out,
                               void* stream) {
+    if (h && h->cfg.dtype == TK_INT8 && (unaligned(q) || unaligned(out))) return fail(h, TK_INVALID_ARG, "append_decode_multi: q and out must be 16-byte aligned");
     int st = tk_kv_append(h, layer, k, v, nullptr, stream);
     if (st != TK_OK) return st;
     return tk_kv_decode_multi(h, layer, q, out, stream);
