@@ -19,8 +19,10 @@
 // Bound: a block of 256 rows x 64 tokens at D = 128 is 1024 clocks of the tensor pipe and 1024 of the special-function unit.  It
 // takes about 2480: the shared-memory pipe is used by loads and stores for half of them (1337 wavefronts, 768 of which are the
 // softmax warps reading the three numbers of each token) and feeds the operands of the MMAs for 41 %; issue slots 63 %, ALU
-// 46 %, special-function unit 42 %.  Measured: 0.39-0.41 ms for 8 chunks of 1024 tokens on contexts up to 2843 (32 heads, 8 kv
-// heads), 1.12-1.27 ms = 870-980 TFLOP/s for a prompt of 8192 (64 heads).
+// 46 %, special-function unit 42 %.  A CTA's start and end take as long as 5 blocks: reading its item, 64 KB of queries (by bulk
+// copies, 64 of them, it took longer), the first expansion and the first block's look at the scores, the output's way out.
+// Measured: 0.37-0.39 ms for 8 chunks of 1024 tokens on contexts up to 2843 (32 heads, 8 kv heads), 1.12-1.27 ms = 870-980 TFLOP/s
+// for a prompt of 8192 (64 heads).
 // Every wait is bounded; on expiry the status word is set, nothing is written, and the CTA waits for its copies and frees its
 // tensor memory before it returns.  No cluster, no multicast, this GPU's memory only.
 #include "int8_cache.cuh"
@@ -105,11 +107,64 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(policy) : "memory");
 }
 
+// What an expander thread does to every block: the same 16 columns of every 16th (D = 64: 32nd) row, all addresses constants away
+// from `from` and `to`.
+template <int D>
+struct PfExpander {
+    static constexpr int CPR = D / 16, ROWS = kPfExpThreads / CPR;      // 16-code chunks per row, rows per pass
+    int et;
+    bool swap;
+    uint32_t from, to_lo, to_hi;
+    __device__ __forceinline__ PfExpander() {
+        uint32_t tid;
+        asm volatile("mov.u32 %0, %%tid.x;" : "=r"(tid));
+        et = (int)tid - kPfSoftWarps * 32;
+        const int er = et / CPR, ec = et % CPR;
+        from = (uint32_t)((er / kI8Page) * i8_tile_bytes(D) + (er % kI8Page) * D + ec * 16);
+        // 16 codes = two 16-byte chunks of the fp16 row.  At D = 128 a quarter warp stores one row: lanes of the second dim half
+        // store their chunks in the other order, or both halves would meet in the same banks.
+        swap = D == 128 && ec >= 4;
+        to_lo = (uint32_t)((ec >> 2) * PfCfg<D>::HALF + er * 128) + (((2 * (ec & 3) + (swap ? 1 : 0)) ^ (er & 7)) << 4);
+        to_hi = to_lo ^ 16u;
+    }
+    __device__ __forceinline__ void operator()(uint32_t raw, int kv, uint32_t slab) const {
+#pragma unroll
+        for (int i = 0; i < kPfBlock / ROWS; i++) {
+            const uint4 w = lds128(raw + from + i * (ROWS / kI8Page) * i8_tile_bytes(D) + i8_row_off(D, kv, 0));
+            const uint32_t a0 = swap ? w.z : w.x, a1 = swap ? w.w : w.y, b0 = swap ? w.x : w.z, b1 = swap ? w.y : w.w;
+            sts128(slab + to_lo + i * ROWS * 128, make_uint4(i8_expand<0x4140>(a0), i8_expand<0x4342>(a0), i8_expand<0x4140>(a1), i8_expand<0x4342>(a1)));
+            sts128(slab + to_hi + i * ROWS * 128, make_uint4(i8_expand<0x4140>(b0), i8_expand<0x4342>(b0), i8_expand<0x4140>(b1), i8_expand<0x4342>(b1)));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+};
+
+// An item of the work list and where its rows are.  Read at the start of a CTA and again behind its loop over the context: kept,
+// these would be a dozen registers that the loop does not have.
+struct PfItem {
+    int b, chunk, kvh, tile, seq, len, nq, ct, q_base, poff, cbase;
+    int tok_first, tok_cnt, p_last;
+    bool split;                                             // the tile's context is more than one chunk
+    __device__ __forceinline__ PfItem(const PrefillDev& pf, int sh) {
+        ld(pf.items + blockIdx.x, b, chunk, kvh, tile);
+        ld(pf.info + 2 * blockIdx.x, seq, len, nq, ct);
+        int unused;
+        ld(pf.info + 2 * blockIdx.x + 1, q_base, poff, cbase, unused);
+        tok_first = tile * (kPfRows >> sh);
+        tok_cnt = min(nq - tok_first, kPfRows >> sh);
+        p_last = len - nq + tok_first + tok_cnt - 1;
+        split = p_last >= ct;
+    }
+    static __device__ __forceinline__ void ld(const int4* p, int& x, int& y, int& z, int& w) {
+        asm volatile("ld.global.nc.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(x), "=r"(y), "=r"(z), "=r"(w) : "l"(p));
+    }
+};
+
 template <int D, bool IO_BF16>
 __global__ void __launch_bounds__(kPfThreads, 1)
 prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf, const int32_t* __restrict__ page_table,
                     const uint16_t* __restrict__ q, void* __restrict__ out, int out_dtype, float* __restrict__ partials,
-                    int* __restrict__ counters, int* __restrict__ status) {
+                    int* __restrict__ counters, int* __restrict__ status, int sh /* log2 of the heads per kv head */) {
     using C = PfCfg<D>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -122,31 +177,23 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
              *bar_s = bars + 16 /* [half][2] */, *p_ready = bars + 20 /* [half][2] */, *bar_o = bars + 24 /* [half] */;
     uint32_t* s_tmem = (uint32_t*)(bars + 26);
     int* s_flag = (int*)(s_tmem + 1);
-    uint32_t* s_wmax = (uint32_t*)(bars + 28);              // [24 warps] prologue: largest query magnitude
+    uint32_t* s_wmax = (uint32_t*)(bars + 28);              // [16 softmax warps] prologue: largest query magnitude
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int G = g.H / g.Hkv;
-    const int4 it = pf.items[blockIdx.x], i0 = pf.info[2 * blockIdx.x], i1 = pf.info[2 * blockIdx.x + 1];
-    const int b = it.x, chunk = it.y, kvh = it.z, tile = it.w;
-    const int seq = i0.x, len = i0.y, nq = i0.z, ct = i0.w;
-    const int q_base = i1.x, poff = i1.y, cbase = i1.z;
-    const int tpt = kPfRows / G;                            // query tokens per tile
-    const int tok_first = tile * tpt;
-    const int tok_cnt = min(nq - tok_first, tpt);
+    const int G = 1 << sh;
+    const PfItem it(pf, sh);
+    const int len = it.len, tok_first = it.tok_first, tok_cnt = it.tok_cnt, kvh = it.kvh, q_base = it.q_base;
     const int halves = tok_cnt * G > kTcRows ? 2 : 1;
-    const int base_pos = len - nq;
-    const int p_last = base_pos + tok_first + tok_cnt - 1;
-    const int t0 = chunk * ct, t1 = min(t0 + ct, p_last + 1);
+    const int base_pos = len - it.nq;
+    const int t0 = it.chunk * it.ct, t1 = min(t0 + it.ct, it.p_last + 1);
     const int n_pages = (t1 - t0 + kI8Page - 1) / kI8Page;
     const int n_blocks = (n_pages + 3) / 4;
-    const int n_chunks = p_last / ct + 1;
-    const int32_t* pt_row = page_table + (size_t)seq * g.max_pages_per_seq + t0 / kI8Page;
+    const int32_t* pt_row = page_table + (size_t)it.seq * g.max_pages_per_seq + t0 / kI8Page;
 
     // ---- prologue ----
     constexpr int LPR = D / 8, QV = kPfRows * LPR / kPfSoftThreads;      // 16-byte vectors per query row, per softmax thread
     uint4 qv[QV];
     if (tid < kPfSoftThreads) {
-        const int sh = __ffs(G) - 1;                        // G divides 128: a power of two
 #pragma unroll
         for (int i = 0; i < QV; i++) {
             const int r = (i * kPfSoftThreads + tid) / LPR, c = tid % LPR;
@@ -185,43 +232,49 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
+        asm volatile("bar.arrive 3, %0;" ::"n"(kPfExpThreads + 32) : "memory");      // the expander warps may wait on them
         for (int blk = 0; blk < kPfRaw && blk < n_blocks; blk++) load_block(blk, pt_row);
     }
     for (int i = tid; i < n_pages; i += kPfThreads) s_pages[i] = pt_row[i];
+
+    const uint32_t raw_u = smem_u32(s_raw), k_u = smem_u32(s_k), v_u = smem_u32(s_v);
     // bf16 queries as fp16: the largest element of the tile becomes 2^14 .. 2^15, one power of two 2^e0 for all rows.  Elements
     // below fp16's normal range are off by at most 2^-40 of that largest element, a score by 2^-40 of what it could make of
     // the key: nothing, unless such scores pass 2^28.  Where a query reaches 2^15 (`wide`) every row therefore has a power of
     // its own, and its scores are multiplied by it.
     int e0 = 0;
     bool wide = false;
-    uint32_t row_max[QV];                                  // bf16 pattern of each of this thread's vectors' rows' largest magnitude
-    if (IO_BF16) {
+    auto tile_power = [&]() {                               // from what the softmax warps left
         uint32_t m_all = 0;
-        if (tid < kPfSoftThreads) {
-#pragma unroll
-            for (int i = 0; i < QV; i++) {
-                uint32_t m = i8_absmax8(qv[i]);
-#pragma unroll
-                for (int off = LPR / 2; off > 0; off >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
-                row_max[i] = m;
-                m_all = max(m_all, m);
-            }
-        }
-        m_all = __reduce_max_sync(0xFFFFFFFFu, m_all);
-        if (lane == 0) s_wmax[warp] = m_all;
-        __syncthreads();
 #pragma unroll
         for (int i = 0; i < kPfSoftWarps; i++) m_all = max(m_all, s_wmax[i]);
         e0 = m_all ? max((int)(m_all >> 7) - 127 - 14, -100) : 0;
         wide = e0 > 0;                                      // some |q| >= 2^15
-    }
-    if (tid < kPfSoftThreads) {
+    };
+    bool staged = true;                                     // expander: no wait of the prologue ran out
+    if (warp < kPfSoftWarps) {
+        if (IO_BF16) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < QV; i++) m = max(m, i8_absmax8(qv[i]));
+            m = __reduce_max_sync(0xFFFFFFFFu, m);
+            if (lane == 0) s_wmax[warp] = m;
+            asm volatile("bar.sync 2, %0;" ::"n"(kPfSoftThreads) : "memory");
+            tile_power();
+        }
 #pragma unroll
         for (int i = 0; i < QV; i++) {
             const int r = (i * kPfSoftThreads + tid) / LPR, c = tid % LPR;
             uint4 x = qv[i];
             if (IO_BF16) {
-                const int e = wide ? (row_max[i] ? max((int)(row_max[i] >> 7) - 127 - 14, -100) : 0) : e0;
+                int e = e0;
+                if (wide) {                                 // uniform
+                    uint32_t rm = i8_absmax8(x);
+#pragma unroll
+                    for (int off = LPR / 2; off > 0; off >>= 1) rm = max(rm, __shfl_xor_sync(0xFFFFFFFFu, rm, off));
+                    e = rm ? max((int)(rm >> 7) - 127 - 14, -100) : 0;
+                    if (c == 0) s_e[r] = pf_pow2i(e);
+                }
                 const float down = pf_pow2i(-e);
                 uint32_t* w = &x.x;
 #pragma unroll
@@ -229,17 +282,30 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                     const float2 f = i8_unpack2<true>(w[u]);
                     w[u] = pack2<false>(f.x * down, f.y * down);
                 }
-                if (c == 0) s_e[r] = pf_pow2i(e);
             }
             // 128-byte-swizzled K-major rows: 16-byte chunk c of a row sits at chunk c ^ (row & 7)
             *reinterpret_cast<uint4*>(s_q + ((r / kTcRows) * C::HALVES + (c >> 3)) * (kTcRows * 128) + (r % kTcRows) * 128 +
                                       (((c & 7) ^ (r & 7)) << 4)) = x;
         }
+    } else if (warp < kPfMmaWarp) {
+        asm volatile("bar.sync 3, %0;" ::"n"(kPfExpThreads + 32) : "memory");
+        // meanwhile: the slabs of K(0), K(1) and V(0); the numbers of the tokens follow when the queries' power of two is known
+        // (the CTA's first S 1200 clocks earlier)
+        const PfExpander<D> expand;
+        auto raw_here = [&](int blk) { return mbar_wait_bounded_tight(smem_u32(&rawfull[blk]), 0u, status); };
+        staged = __all_sync(0xFFFFFFFFu, raw_here(0));
+        if (staged) expand(raw_u, 0, k_u);
+        if (staged && n_blocks > 1) {
+            staged = __all_sync(0xFFFFFFFFu, raw_here(1));
+            if (staged) expand(raw_u + C::RAW, 0, k_u + C::SLAB);
+        }
+        if (staged) expand(raw_u, 1, v_u);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // generic writes above -> visible to the MMAs
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (IO_BF16) tile_power();
     const uint32_t tmem = *s_tmem;
 
     bool alive = true;
@@ -334,37 +400,15 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     if (warp >= kPfSoftWarps) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPfRegsOther));
         // ===== expander warps: codes -> fp16 slabs =====
-        const int et = tid - kPfSoftWarps * 32;
         const float sc2E = kLog2e / sqrtf((float)D) * (IO_BF16 && !wide ? pf_pow2i(e0) : 1.0f);
-        // A thread expands the same 16 columns of every 16th (D = 64: 32nd) row: all its addresses are constants away from these.
-        constexpr int CPR = D / 16, ROWS = kPfExpThreads / CPR;     // 16-code chunks per row, rows per pass
-        const int er = et / CPR, ec = et % CPR;
-        const uint32_t from = (uint32_t)((er / kI8Page) * C::TILE + (er % kI8Page) * D + ec * 16);
-        // 16 codes = two 16-byte chunks of the fp16 row.  At D = 128 a quarter warp stores one row: lanes of the second dim half
-        // store their chunks in the other order, or both halves would meet in the same banks.
-        const bool swap = D == 128 && ec >= 4;
-        const uint32_t to = (uint32_t)((ec >> 2) * C::HALF + er * 128);
-        const uint32_t to_lo = to + (((2 * (ec & 3) + (swap ? 1 : 0)) ^ (er & 7)) << 4), to_hi = to_lo ^ 16u;
-        const uint32_t raw_u = smem_u32(s_raw), k_u = smem_u32(s_k), v_u = smem_u32(s_v), sc_u = smem_u32(s_sc);
-            auto expand = [&](uint32_t raw, int kv, uint32_t slab) {
-#pragma unroll
-            for (int i = 0; i < kPfBlock / ROWS; i++) {
-                const uint4 w = lds128(raw + from + i * (ROWS / kI8Page) * C::TILE + i8_row_off(D, kv, 0));
-                const uint32_t a0 = swap ? w.z : w.x, a1 = swap ? w.w : w.y, b0 = swap ? w.x : w.z, b1 = swap ? w.y : w.w;
-                sts128(slab + to_lo + i * ROWS * 128, make_uint4(i8_expand<0x4140>(a0), i8_expand<0x4342>(a0), i8_expand<0x4140>(a1), i8_expand<0x4342>(a1)));
-                sts128(slab + to_hi + i * ROWS * 128, make_uint4(i8_expand<0x4140>(b0), i8_expand<0x4342>(b0), i8_expand<0x4140>(b1), i8_expand<0x4342>(b1)));
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        };
-        auto expand_k = [&](int blk) {
-            const int s = blk & 1, rs = blk % kPfRaw;
-            const uint32_t raw = raw_u + rs * C::RAW;
-            if (!mbar_wait_bounded_tight(smem_u32(&rawfull[rs]), (uint32_t)((blk / kPfRaw) & 1), status)) return false;
-            if (blk >= 2 && !mbar_wait_bounded_tight(smem_u32(&kempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
+        const PfExpander<D> expand;                          // (again: its registers were not kept over the barrier)
+        const int et = expand.et;
+        const uint32_t sc_u = smem_u32(s_sc);
+        auto numbers = [&](int blk) {
             if (et < kPfBlock) {
                 // (the numbers of block blk - 4 are out of use: S of block blk - 2, whose slab was just handed back, was
                 // issued after every row's W of block blk - 4)
-                const uint32_t t = raw + (et / kI8Page) * C::TILE;
+                const uint32_t t = raw_u + (blk % kPfRaw) * C::RAW + (et / kI8Page) * C::TILE;
                 const bool in = t0 + blk * kPfBlock + et < t1;      // behind the range: whatever the page's last owner left
                 const float ks = lds32(t + i8_scale_off(D, 0, et % kI8Page)), vs = lds32(t + i8_scale_off(D, 1, et % kI8Page));
                 const uint32_t o = sc_u + (((blk & 3) * 3 * kPfBlock + et) << 2);
@@ -372,21 +416,34 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                 sts32(o + 4 * kPfBlock, in ? pf_lg2(vs) : 0.0f);
                 sts32(o + 8 * kPfBlock, in ? __fdividef(1.0f, vs) : 0.0f);
             }
-            expand(raw, 0, k_u + s * C::SLAB);
+        };
+        auto expand_k = [&](int blk) {
+            const int s = blk & 1, rs = blk % kPfRaw;
+            if (!mbar_wait_bounded_tight(smem_u32(&rawfull[rs]), (uint32_t)((blk / kPfRaw) & 1), status)) return false;
+            if (!mbar_wait_bounded_tight(smem_u32(&kempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
+            numbers(blk);
+            expand(raw_u + rs * C::RAW, 0, k_u + s * C::SLAB);
             warp_arrive(&kfull[s]);
             return true;
+        };
+        auto give_v = [&](int blk) {
+            warp_arrive(&vfull[blk & 1]);
+            if (lane == 0) mbar_arrive(smem_u32(&rawempty[blk % kPfRaw]));
         };
         auto expand_v = [&](int blk) {
             const int s = blk & 1, rs = blk % kPfRaw;
             if (blk >= 2 && !mbar_wait_bounded_tight(smem_u32(&vempty[s]), (uint32_t)(((blk >> 1) - 1) & 1), status)) return false;
             expand(raw_u + rs * C::RAW, 1, v_u + s * C::SLAB);
-            warp_arrive(&vfull[s]);
-            if (lane == 0) mbar_arrive(smem_u32(&rawempty[rs]));
+            give_v(blk);
             return true;
         };
+        bool ok = staged;
+        if (ok) {                                            // what the prologue has expanded
+            for (int blk = 0; blk < 2 && blk < n_blocks; blk++) { numbers(blk); warp_arrive(&kfull[blk]); }
+            give_v(0);
+        }
         // W V of block i - 2 and S of block i end together: they hand back the slabs of V(i) and K(i + 2), needed in this order
-        bool ok = expand_k(0) && (n_blocks < 2 || expand_k(1));
-        for (int blk = 0; blk < n_blocks && ok; blk++) ok = expand_v(blk) && (blk + 2 >= n_blocks || expand_k(blk + 2));
+        for (int blk = 0; blk < n_blocks && ok; blk++) ok = (blk == 0 || expand_v(blk)) && (blk + 2 >= n_blocks || expand_k(blk + 2));
         leave();
         return;
     }
@@ -413,11 +470,11 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
             m2[rr] = -1e30f;
             l2[rr] = 0ull;
             // (rows without a token: zero queries, nothing of theirs is written; unmasked, so that they cost no careful pass)
-            lim[rr] = row / G < tok_cnt ? base_pos + tok_first + row / G + 1 : len;
+            lim[rr] = (row >> sh) < tok_cnt ? base_pos + tok_first + (row >> sh) + 1 : len;
         }
         const uint32_t e_u = smem_u32(s_e) + 4 * row0;       // the rows' powers of two, 8 rows apart
         auto power = [&](int rr) { const float e = IO_BF16 && wide ? lds32(e_u + 32 * rr) : 1.0f; return pack_x2(e, e); };
-        const bool idle = (row0 - (lane >> 2)) / G >= tok_cnt;   // no row of this warp has a token: whatever W holds, nobody reads its O
+        const bool idle = ((row0 - (lane >> 2)) >> sh) >= tok_cnt;   // no row of this warp has a token: whatever W holds, nobody reads its O
         int lim_min = lim[0];
 #pragma unroll
         for (int rr = 1; rr < NR; rr++) lim_min = min(lim_min, lim[rr]);
@@ -570,6 +627,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
 
         const bool poisoned = __any_sync(0xFFFFFFFFu, !alive || __ldcg(status) != 0);   // fail closed, whole warps at a time
         if (!poisoned && !idle) {
+            const PfItem it(pf, sh);
             float f[NR];
             float* prow[NR];
             size_t qo[NR];
@@ -580,13 +638,13 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                 float l = lf.x + lf.y;
                 l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
                 l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-                const int row = row0 + 8 * rr, tok = tok_first + row / G, head = kvh * G + row % G;
-                valid[rr] = row / G < tok_cnt;
-                qo[rr] = ((size_t)(q_base + tok) * g.H + head) * D;
+                const int row = row0 + 8 * rr, tok = it.tok_first + (row >> sh), head = it.kvh * G + (row & (G - 1));
+                valid[rr] = (row >> sh) < it.tok_cnt;
+                qo[rr] = ((size_t)(it.q_base + tok) * g.H + head) * D;
                 prow[rr] = nullptr;
                 f[rr] = l == 0.0f ? 0.0f : 1.0f / l;         // l counts weights over value scales: at least one term of any size
-                if (n_chunks > 1) {                          // (o, m, l) of this chunk, brought to l in [1, 2)
-                    prow[rr] = partials + (size_t)poff * g.H * (D + 2) + partial_off(chunk, tok * g.H + head, nq * g.H, D);
+                if (it.split) {                                 // (o, m, l) of this chunk, brought to l in [1, 2)
+                    prow[rr] = partials + (size_t)it.poff * g.H * (D + 2) + partial_off(it.chunk, tok * g.H + head, it.nq * g.H, D);
                     const uint32_t ex = (__float_as_uint(l) >> 23) & 0xFFu;
                     const int k = ex == 0 || ex >= 254 ? 0 : (int)ex - 127;
                     f[rr] = pf_pow2i(-k);
@@ -594,6 +652,10 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                         *reinterpret_cast<float2*>(prow[rr] + D) = make_float2(l == 0.0f ? -1e30f : (m2[rr] + (float)k) * 0.6931471805599453f, l * f[rr]);
                 }
             }
+            // 16-bit rows go through shared memory, where this warp's query rows were (every product of its half is done), and leave
+            // as 16 bytes per lane; written from the fragments, four bytes per lane, they took 4000 clocks per tile
+            const bool staged_out = !it.split && out_dtype != DT_FP32;
+            const uint32_t s_o = smem_u32(s_q + half * C::HALVES * kTcRows * 128);
 #pragma unroll
             for (int part = 0; part < D / 32; part++)
 #pragma unroll
@@ -603,28 +665,42 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
                     tc_wait_ld16(of);
 #pragma unroll
                     for (int hh = 0; hh < 2; hh++) {
-                        const int rr = 2 * gi + hh;
-                        if (!valid[rr]) continue;
+                        const int rr = 2 * gi + hh, row = lane0 + (lane >> 2) + 8 * rr;
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             const float o0 = __uint_as_float(of[4 * k + 2 * hh]) * f[rr], o1 = __uint_as_float(of[4 * k + 2 * hh + 1]) * f[rr];
                             const int c = 32 * part + 8 * k + 2 * quad;
-                            if (n_chunks > 1)                *reinterpret_cast<float2*>(prow[rr] + c) = make_float2(o0, o1);
-                            else if (out_dtype == DT_FP32)   *reinterpret_cast<float2*>((float*)out + qo[rr] + c) = make_float2(o0, o1);
-                            else                             *reinterpret_cast<uint32_t*>((uint16_t*)out + qo[rr] + c) = pack2<IO_BF16>(o0, o1);
+                            if (staged_out)      sts32(s_o + (c >> 6) * (kTcRows * 128) + row * 128 + ((((c >> 3) & 7) ^ (row & 7)) << 4) + 4 * quad,
+                                                       __uint_as_float(pack2<IO_BF16>(o0, o1)));
+                            else if (!valid[rr]) continue;
+                            else if (it.split)      *reinterpret_cast<float2*>(prow[rr] + c) = make_float2(o0, o1);
+                            else                 *reinterpret_cast<float2*>((float*)out + qo[rr] + c) = make_float2(o0, o1);
                         }
                     }
                 }
+            if (staged_out) {
+                __syncwarp();
+                constexpr int LPO = D / 8;                   // lanes per row
+#pragma unroll
+                for (int i = 0; i < 16 * kPfGroups * LPO / 32; i++) {
+                    const int r = lane0 + (i * 32 + lane) / LPO, c = lane % LPO, row = half * kTcRows + r;
+                    if ((row >> sh) >= it.tok_cnt) continue;
+                    const uint4 x = lds128(s_o + (c >> 3) * (kTcRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+                    *reinterpret_cast<uint4*>((uint16_t*)out + ((size_t)(it.q_base + it.tok_first + (row >> sh)) * g.H + it.kvh * G + (row & (G - 1))) * D + c * 8) = x;
+                }
+            }
         }
     }
 
     leave();
-    if (n_chunks == 1) return;
+    const PfItem fin(pf, sh);
+    if (!fin.split) return;
+    const int n_chunks = fin.p_last / fin.ct + 1;
     // the CTA that arrives last for the tile merges its chunks (nothing is written while the status word is set)
     if (tid == 0) {
         __threadfence();
-        const int tiles = (nq + tpt - 1) / tpt;
-        int* c = counters + cbase + kvh * tiles + tile;
+        const int tiles = (fin.nq + (kPfRows >> sh) - 1) / (kPfRows >> sh);
+        int* c = counters + fin.cbase + fin.kvh * tiles + fin.tile;
         const int last = atomicAdd(c, 1) == n_chunks - 1;
         if (last) *c = 0;
         *s_flag = last;
@@ -633,13 +709,13 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
     if (!*s_flag) return;
     __threadfence();                                        // see the other CTAs' rows
     if (__ldcg(status) != 0) return;
-    const int rows = G * tok_cnt;
-    const size_t chunk_stride = (size_t)nq * g.H * (D + 2);
-    const float* region = partials + (size_t)poff * g.H * (D + 2);
-    auto column = [&](int row) { return (size_t)(tok_first + row / G) * g.H + kvh * G + row % G; };
+    const int rows = G * fin.tok_cnt;
+    const size_t chunk_stride = (size_t)fin.nq * g.H * (D + 2);
+    const float* region = partials + (size_t)fin.poff * g.H * (D + 2);
+    auto column = [&](int row) { return (size_t)(fin.tok_first + (row >> sh)) * g.H + fin.kvh * G + (row & (G - 1)); };
     if (rows * n_chunks * 4 > C::OFF_BARS) {                // (more weights than shared memory)
         const MergeOut mo{nullptr, out, nullptr, out_dtype, nullptr, status};
-        merge_rows(g, mo, b, kvh, G, 0, n_chunks, region, MergeMap{rows, nq * g.H, q_base + tok_first, tok_first, 0}, kPfSoftWarps);
+        merge_rows(g, mo, fin.b, fin.kvh, G, 0, n_chunks, region, MergeMap{rows, fin.nq * g.H, fin.q_base + fin.tok_first, fin.tok_first, 0}, kPfSoftWarps);
         return;
     }
     // The merge of tk_merge.cuh for all rows at once (row after row its chain of L2 loads took 22 us for 256 rows): a thread per row
@@ -688,7 +764,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
         for (int u = 0; u < U; u++) {
             const int row = row_a + u * PER;
             if (row >= rows) break;
-            const size_t at = ((size_t)(q_base + tok_first + row / G) * g.H + kvh * G + row % G) * D + d;
+            const size_t at = ((size_t)(fin.q_base + fin.tok_first + (row >> sh)) * g.H + fin.kvh * G + (row & (G - 1))) * D + d;
             if (out_dtype == DT_FP32) *reinterpret_cast<float2*>((float*)out + at) = acc[u];
             else                      *reinterpret_cast<uint32_t*>((uint16_t*)out + at) = pack2<IO_BF16>(acc[u].x, acc[u].y);
         }
@@ -699,6 +775,9 @@ template <int D, bool IO_BF16>
 cudaError_t launch_d(const Geometry& g, const LayerPtrs& lp, const PrefillDev& pf, const int32_t* page_table, const void* q, void* out,
                      int out_dtype, float* partials, int* counters, int* status, cudaStream_t s) {
     auto kern = prefill_int8_kernel<D, IO_BF16>;
+    int sh = 0;                                             // the planner lays out these items for powers of two only
+    while (g.Hkv << sh < g.H) sh++;
+    if (g.Hkv << sh != g.H || sh > 7) return cudaErrorInvalidValue;
     static bool attr_done[64] = {};                         // per instantiation and device
     int dev = 0;
     cudaGetDevice(&dev);
@@ -708,7 +787,7 @@ cudaError_t launch_d(const Geometry& g, const LayerPtrs& lp, const PrefillDev& p
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
     kern<<<pf.n_items, kPfThreads, PfCfg<D>::SMEM, s>>>(g, (const uint8_t*)lp.pool, pf, page_table, (const uint16_t*)q, out, out_dtype, partials,
-                                                        counters, status);
+                                                        counters, status, sh);
     return cudaGetLastError();
 }
 
