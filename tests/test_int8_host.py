@@ -96,6 +96,19 @@ def test_any_length_may_be_cut_adopted_and_capped():
     assert c._lib.tk_kv_step_begin_capped(c._h, 2, p(a), p(b), p(cap), None) == L.TK_OK
 
 
+@pytest.mark.parametrize("tokens,heads,chunk", [
+    (300, 64, 256), (8192, 64, 512), (16384, 64, 896), (32768, 64, 896), (40000, 64, 1024), (65536, 64, 2048), (131072, 64, 2048),
+    (152000, 64, 2048), (170000, 64, 1536), (300000, 64, 2048), (131072, 128, 1536)])
+def test_chunk_of_a_decode_step(tokens, heads, chunk):
+    """One sequence on 8 kv heads: two items per SM of 148 (where it would be less than 1.7, down to 896 tokens each), and no launch
+    of a little more than one wave: of 592 items, or of 444 where the rows of a kv head are two column blocks."""
+    c = PagedKVCache(1, heads, 8, 128, 20000, 1, 20000, dtype="int8", io_dtype="bf16", max_step_tokens=tokens, host_only=True)
+    s = c.seq_alloc()
+    c.step_begin([s], [tokens - 1])
+    c.step_begin([s], [1])
+    assert c.step_chunk_tokens == chunk
+
+
 def test_compute_calls_need_a_device():
     c = _cache()
     s = c.seq_alloc()

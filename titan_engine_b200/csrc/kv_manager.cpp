@@ -381,7 +381,17 @@ int PageManager::plan_step(int n_seqs, const int32_t* seqs, const int32_t* n_new
         // one wave of equal items is the worst schedule.  So: the largest chunk, unless that leaves
         // between 0.9 and 1.5 waves (then the largest chunk of at least 1024 tokens that gives 1.5
         // waves) or fewer than 128 items (then the largest chunk, down to 256 tokens, that gives 128).
-        const int64_t slots = std::max<int64_t>(1, (int64_t)target_items * 3 / 8);   // target = 8 per SM, 3 CTAs per SM
+        //
+        // The INT8 kernel with one column block (one token per sequence, up to 8 heads per kv head) has 4 CTAs per SM, and its worst
+        // schedules start at 1.05 waves: one sequence, 64 heads on 8, D = 128: 131072 tokens as 512 items 86 us, as 688 111; 152000 as
+        // 600 items 93, as 1192 106; 170000 as 672 items 130, as 888 116.  Below 1.7 items per SM it gains from two of them, down to 896
+        // tokens each: 32768 tokens as 128 items 42.5 us, as 296 40.0; 40000 as 160 items 51.5, as 320 45.7; 65536 as 256 items 50.6,
+        // as 296 50.2.
+        const bool int8 = prefill_rows == kPrefillRowsInt8;
+        int most_new = 1;
+        for (int i = 0; n_new && i < n_seqs; i++) most_new = std::max(most_new, n_new[i]);
+        const bool four = int8 && (int64_t)heads_per_kv * most_new <= 8;
+        const int64_t slots = std::max<int64_t>(1, (int64_t)target_items * (four ? 4 : 3) / 8);   // target = 8 per SM, 3 or 4 CTAs per SM
         std::vector<int> cands;                         // descending, multiples of the page size
         for (int c : {2048, 1792, 1536, 1280, 1024, 896, 768, 640, 512, 384, 256, 128}) {
             const int r = c / ps * ps;
@@ -394,14 +404,14 @@ int PageManager::plan_step(int n_seqs, const int32_t* seqs, const int32_t* n_new
             if (fits(cands[i], &items_max)) { first = i; break; }
         if (first == cands.size()) return ST_INVALID_ARG;
         chunk = cands[first];
-        if (items_max * 10 > slots * 9 && items_max * 2 < slots * 3) {
+        if (items_max * 20 > slots * (four ? 21 : 18) && items_max * 2 < slots * 3) {
             for (size_t i = first + 1; i < cands.size() && cands[i] >= 1024; i++) {
                 int64_t items = 0;
                 if (fits(cands[i], &items) && items * 2 >= slots * 3) { chunk = cands[i]; break; }
             }
-        } else if (items_max < 128) {
+        } else if (items_max < 128 || (int8 && items_max * 80 < (int64_t)target_items * 17)) {
             int64_t items = items_max;
-            for (size_t i = first + 1; i < cands.size() && cands[i] >= 256 && items < 128; i++)
+            for (size_t i = first + 1; i < cands.size() && cands[i] >= 256 && items < (int8 && cands[i] >= 896 ? target_items / 4 : 128); i++)
                 if (fits(cands[i], &items)) chunk = cands[i];
         }
     } else if (rows_for(chunk, nullptr) > max_partial_rows) {
