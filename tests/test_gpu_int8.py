@@ -612,6 +612,31 @@ def test_rope_append_decode_against_64_bits(io, D):
         assert (np.abs(got[i] - out[0]) <= bound[0] + top).all()
 
 
+def test_read_in_several_launches_captured_and_on_two_streams():
+    """A read of more pages than one launch lists, replayed from a graph, next to an eager one of the same rows on another stream."""
+    p = Pair(2, 1, 64, "bf16", pages=2100, seqs=2, mpps=2100, max_step_tokens=40000, poison=False)
+    a = p.alloc()
+    n = 2050 * 16 - 3
+    k, v = p.begin([a], [n])
+    p.c.append(0, k, v)
+    want = [x.clone() for x in p.c.read(0, [a, a], [0, 5], [n, 40])]
+    np.testing.assert_array_equal(want[0][:n].double().cpu().numpy(), torch.from_numpy(p.k[a]).to(torch.bfloat16).double().numpy())
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        got = p.c.read(0, [a, a], [0, 5], [n, 40])
+    for x in got:
+        x.zero_()
+    torch.cuda.synchronize()
+    graph.replay()
+    with torch.cuda.stream(side):
+        there = p.c.read(0, [a, a], [0, 5], [n, 40])
+    graph.replay()
+    torch.cuda.synchronize()
+    for x, y, z in zip(want, got, there):
+        assert torch.equal(x, y) and torch.equal(x, z) and torch.equal(x[n:], x[5:45])
+
+
 def test_captured_step_replays_next_to_eager_calls_on_another_stream():
     p = Pair(8, 2, 128, "bf16", layers=2)
     other = Pair(8, 2, 128, "bf16", seed=9)

@@ -16,8 +16,8 @@
 // the codes.  A tile brings its scales along (int8_cache.cuh): one TMA box per page.  On decode steps the warp that holds
 // the last page quantises the new token into shared memory and into the pool: no append launch.
 // Bound: HBM (D + 4 bytes per token and kv head for K and for V).  Measured at D = 128: 32 sequences of 32768 tokens, 64 heads
-// on 8: 354-384 us = 5.8-6.2 TB/s (issue slots 60 %, tensor pipe 18 %); 64 sequences of 1024-8192, 32 heads: 102-107 us, of which
-// about 10 are the launch's start and drain; one sequence of 65536 tokens: 40 us, where starting and merging are a third.
+// on 8: 337-387 us = 5.7-6.6 TB/s (issue slots 60 %, tensor pipe 18 %); 64 sequences of 1024-8192, 32 heads: 102-107 us, of which
+// about 10 are the launch's start and drain; one sequence of 65536 tokens: 39 us, where starting and merging are a third.
 #include "int8_cache.cuh"
 #include "tk_merge.cuh"
 #include "tk_mma.cuh"
@@ -28,7 +28,8 @@ namespace {
 
 // One column block (128 registers) leaves room for 4 CTAs per SM, two (168) for 3; the stages share out the shared memory.  Measured
 // at D = 128, one block: 2 stages x 4 CTAs 364 us, 3 x 3 377, 4 x 2 438 (32 sequences of 32768 tokens, 64 heads); two blocks:
-// 3 x 3 168 us, 2 x 4 (spilling) 175 (64 sequences, 4 tokens each).
+// 3 x 3 168 us, 2 x 4 (spilling) 175 (64 sequences, 4 tokens each; with the queries' fragments in shared memory 2 x 4 is 1 % faster than 3 x 3,
+// less than it adds).
 template <int D, int NB>
 struct I8Cfg {
     static constexpr int CTAS = NB == 1 ? 4 : 3;

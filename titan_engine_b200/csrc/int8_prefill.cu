@@ -21,7 +21,7 @@
 // softmax warps reading the three numbers of each token) and feeds the operands of the MMAs for 41 %; issue slots 63 %, ALU
 // 46 %, special-function unit 42 %.  A CTA's start and end take as long as 5 blocks: reading its item, 64 KB of queries (by bulk
 // copies, 64 of them, it took longer), the first expansion and the first block's look at the scores, the output's way out.
-// Measured: 0.37-0.39 ms for 8 chunks of 1024 tokens on contexts up to 2843 (32 heads, 8 kv heads), 1.12-1.27 ms = 870-980 TFLOP/s
+// Measured: 0.37-0.40 ms for 8 chunks of 1024 tokens on contexts up to 2843 (32 heads, 8 kv heads), 1.13-1.28 ms = 860-970 TFLOP/s
 // for a prompt of 8192 (64 heads).
 // Every wait is bounded; on expiry the status word is set, nothing is written, and the CTA waits for its copies and frees its
 // tensor memory before it returns.  No cluster, no multicast, this GPU's memory only.
