@@ -230,21 +230,25 @@ def _prepare_own(c, seed):
             cache.step_begin([sid], [m])
             cache.append(0, old_k[at:at + m], old_v[at:at + m])
             at += m
-    if c["op"] != "read":
-        cache.step_begin(seqs, new)
     return {"op": c["op"], "cache": cache, "seqs": seqs, "start": start, "count": new, "new": (k, v, q)}
 
 
 def _run_own(s):
+    """A step from its beginning: pages for the new tokens, the plan and its upload, then the layer's call."""
     cache, (k, v, q) = s["cache"], s["new"]
     if s["op"] == "read":
         return cache.read(0, s["seqs"], s["start"], s["count"])
+    cache.step_begin(s["seqs"], s["count"])
     if s["op"] == "write":
         cache.append(0, k, v)
-        return cache.read(0, s["seqs"], s["start"], s["count"])
-    if s["op"] == "decode":
-        return cache.append_decode(0, k, v, q)
-    return cache.append_decode_multi(0, k, v, q)
+        out = cache.read(0, s["seqs"], s["start"], s["count"])
+    elif s["op"] == "decode":
+        out = cache.append_decode(0, k, v, q)
+    else:
+        out = cache.append_decode_multi(0, k, v, q)
+    for seq, held in zip(s["seqs"], s["start"]):            # the step is taken back, so that the next pass finds what this one found
+        cache.truncate(seq, held)
+    return out
 
 
 def prepare(case, seed):
