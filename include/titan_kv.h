@@ -221,8 +221,9 @@ int tk_kv_append(tk_kv* h, int32_t layer, const void* k, const void* v, int64_t*
  * inside its sequence's tokens; a sequence may be named several times.  Reads what the layer's appends before it on
  * `stream` have written, under the page table of the moment of the call (a fork or truncation since the last step counts);
  * it needs no step, uploads nothing and may be captured into a graph, which then replays with those pages.
- * Outputs must be 16-byte aligned.  TK_UNSUPPORTED for a token in a cold page.  (The reference hands out the slab: KVCache::k_cache / v_cache,
- * src/inference/kv_cache.h:42-48.) */
+ * Outputs must be 16-byte aligned.  TK_UNSUPPORTED for a token in a cold page, and on an FP8 pool for a token of a page that
+ * the current step completes until this layer's append has been called: before it the page has no codes.  (The
+ * reference hands out the slab: KVCache::k_cache / v_cache, src/inference/kv_cache.h:42-48.) */
 int tk_kv_read(tk_kv* h, int32_t layer, int32_t n_ranges, const int32_t* seq_ids, const int32_t* start, const int32_t* count,
                void* k_out, void* v_out, int32_t out_dtype, void* stream);
 /* cuda::attention_decode (src/compute/cuda/attention.cu:315-330) for every sequence

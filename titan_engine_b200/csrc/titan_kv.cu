@@ -173,6 +173,7 @@ struct tk_kv {
     tk::StepPlan plan;
     tk::StepDev dev{};
     bool have_step = false;
+    std::vector<uint8_t> appended;       // layers whose append was called since the step began
     int n_pool_items = 0;                // items of kind 0 come first
 
     // optional timing of the dominant decode kernel: one event pair per launch
@@ -693,6 +694,7 @@ int tk_kv_state_load(tk_kv* h, const int32_t* image, int64_t n) {
         return fail(h, TK_UNSUPPORTED, "state_load: a device handle with a cold tier cannot take an image (the host pool's contents are not part of it)");
     const int st = h->mgr->load(image, (size_t)n);
     if (st != TK_OK) return fail(h, st, "state_load: the image does not belong to a cache of this geometry, or is damaged");
+    h->plan.seals.clear();                                  // no step completes pages of the loaded state
     h->have_step = false;
     return TK_OK;
 }
@@ -731,6 +733,7 @@ static int step_begin_impl(tk_kv* h, int32_t n_seqs, const int32_t* seq_ids, con
                               int8 ? 1 : tk::kDecodeMaxTokenGroups);
     if (st != TK_OK) return fail(h, st, "step_begin: %s", tk_status_str(st));
     tk::StepPlan& p = h->plan;
+    h->appended.assign((size_t)h->cfg.num_layers, 0);
     if (chunk == 0 && p.chunk_tokens > 2048) {
         return fail(h, TK_INVALID_ARG, "internal: chunk %d too large", p.chunk_tokens);
     }
@@ -896,15 +899,23 @@ int tk_kv_append(tk_kv* h, int32_t layer, const void* k, const void* v, int64_t*
                                       (cudaStream_t)stream, &n);
     h->launches += n;
     if (e != cudaSuccess) return fail(h, TK_CUDA_ERROR, "append launch: %s", cudaGetErrorString(e));
+    h->appended[layer] = 1;
     return TK_OK;
 }
 
 // The pages that hold the ranges' rows, in order; the caller holds mgr_mu.
-static int read_items(tk_kv* h, int n_ranges, const int32_t* seq_ids, const int32_t* start, const int32_t* count,
+static int read_items(tk_kv* h, int layer, int n_ranges, const int32_t* seq_ids, const int32_t* start, const int32_t* count,
                       std::vector<tk::ReadItem>* items) {
     const int ps = h->cfg.page_size;
     const bool fp8 = h->cfg.dtype == TK_FP8_E4M3;
     int64_t rows = 0;
+    // FP8: a page that the step completes gets its codes from the layer's append.  Before that call its older tokens are in the
+    // 16-bit open page and the pool page holds what its last owner left (pages, not sequences: a fork may share it)
+    std::vector<uint8_t> incomplete;
+    if (!h->plan.seals.empty() && !h->appended[layer]) {
+        incomplete.assign((size_t)h->cfg.num_pages, 0);
+        for (const tk::SealItem& s : h->plan.seals) incomplete[s.page] = 1;
+    }
     for (int i = 0; i < n_ranges; i++) {
         const int seq = seq_ids[i], len = h->mgr->seq_len(seq);
         const int64_t lo = start ? start[i] : 0, n = count ? count[i] : len - lo;
@@ -917,6 +928,9 @@ static int read_items(tk_kv* h, int n_ranges, const int32_t* seq_ids, const int3
             const int r = (int)(at % ps), m = (int)std::min<int64_t>(ps - r, lo + n - at);
             const int32_t page = at < sealed ? pages[at / ps] : -1 - seq;
             if (at < sealed && page < 0) return fail(h, TK_UNSUPPORTED, "read: token %lld of sequence %d lies in a cold page", (long long)at, seq);
+            if (!incomplete.empty() && page >= 0 && incomplete[page])
+                return fail(h, TK_UNSUPPORTED, "read: token %lld of sequence %d lies in a page that this step completes: append the layer's rows first",
+                            (long long)at, seq);
             items->push_back(tk::ReadItem{page, r, m, (int)rows});
             rows += m;
             at += m;
@@ -931,16 +945,16 @@ int tk_kv_read(tk_kv* h, int32_t layer, int32_t n_ranges, const int32_t* seq_ids
     if (!h || layer < 0 || layer >= h->cfg.num_layers || n_ranges < 0 || (n_ranges > 0 && !seq_ids)) return TK_INVALID_ARG;
     if (const int fs = host_flush(h)) return fs;               // launches the host-buffer calls still hold back come first
     if (unaligned(k_out) || unaligned(v_out)) return fail(h, TK_INVALID_ARG, "read: outputs must be 16-byte aligned");
-    if (h->host_only) return fail(h, TK_CUDA_ERROR, "read: handle has no device (bookkeeping only)");
     if (out_dtype != TK_FP32 && out_dtype != h->cfg.io_dtype)
         return fail(h, TK_INVALID_ARG, "read: out dtype must be FP32 or the handle's io dtype");
     std::lock_guard<std::mutex> lock(h->mgr_mu);
     std::vector<tk::ReadItem> items;
     try {
-        if (const int st = read_items(h, n_ranges, seq_ids, start, count, &items)) return st;
+        if (const int st = read_items(h, layer, n_ranges, seq_ids, start, count, &items)) return st;
     } catch (const std::bad_alloc&) {
         return fail(h, TK_INVALID_ARG, "read: the ranges' list of pages does not fit the host's memory: read fewer in one call");
     }
+    if (h->host_only) return fail(h, TK_CUDA_ERROR, "read: handle has no device (bookkeeping only)");
     if (items.empty()) return TK_OK;
     if (!k_out || !v_out) return fail(h, TK_INVALID_ARG, "read: null output");
     const OnDevice current(h->device);
