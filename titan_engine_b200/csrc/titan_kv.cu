@@ -224,12 +224,16 @@ int fail(tk_kv* h, int status, const char* fmt, ...) {
             return fail(h, TK_CUDA_ERROR, "%s failed: %s", #call, cudaGetErrorString(e_));       \
     } while (0)
 
-// Makes the handle's device current for a launch (the default stream belongs to whichever device is) and puts the caller's back.
+// Makes the handle's device current for a call (allocations, events and the default stream belong to whichever device is) and puts the
+// caller's back at its end.
 struct OnDevice {
     int back = -1;
-    explicit OnDevice(int device) {
+    cudaError_t err = cudaSuccess;
+    explicit OnDevice(const tk_kv* h) {
         int now = -1;
-        if (cudaGetDevice(&now) == cudaSuccess && now != device && cudaSetDevice(device) == cudaSuccess) back = now;
+        if (h->host_only || (err = cudaGetDevice(&now)) != cudaSuccess || now == h->device) return;
+        err = cudaSetDevice(h->device);
+        if (err == cudaSuccess) back = now;
     }
     ~OnDevice() { if (back >= 0) cudaSetDevice(back); }
 };
@@ -240,7 +244,7 @@ bool unaligned(const void* p, size_t to = 16) { return ((uintptr_t)p & (to - 1))
 void release(tk_kv* h) {
     if (!h) return;
     if (!h->host_only) {
-        cudaSetDevice(h->device);
+        const OnDevice current(h);
         if (h->owns_arena && h->arena) cudaFree(h->arena);
         if (h->d_table) cudaFree(h->d_table);
         if (h->d_partials) cudaFree(h->d_partials);
@@ -342,7 +346,8 @@ int create_impl(const tk_kv_config* cfg_in, void* arena, size_t arena_bytes, boo
             return fail(nullptr, TK_CUDA_ERROR, "%s failed: %s", #call, cudaGetErrorString(e_)); \
         }                                                                                        \
     } while (0)
-    CREATE_CUDA(cudaSetDevice(h->device));
+    const OnDevice current(h);
+    CREATE_CUDA(current.err);
     cudaDeviceProp prop;
     CREATE_CUDA(cudaGetDeviceProperties(&prop, h->device));
     h->num_sms = prop.multiProcessorCount;
@@ -575,7 +580,10 @@ int tk_kv_create_external(const tk_kv_config* cfg, void* arena, size_t bytes, tk
 }
 int tk_kv_destroy(tk_kv* h) {
     if (!h) return TK_INVALID_ARG;
-    if (!h->host_only) { cudaSetDevice(h->device); cudaDeviceSynchronize(); }
+    if (!h->host_only) {
+        const OnDevice current(h);
+        cudaDeviceSynchronize();
+    }
     release(h);
     return TK_OK;
 }
@@ -643,6 +651,7 @@ int tk_kv_seq_fork(tk_kv* h, int32_t parent, int32_t* child_out, void* stream) {
     *child_out = child;
     if (h->host_only || dst < 0) return TK_OK;
     // the partly filled last page is private: copy it for every layer (FP8: it is the open page)
+    const OnDevice current(h);
     cudaError_t e;
     if (h->cfg.dtype == TK_FP8_E4M3) {
         const size_t open_tile = h->page_bytes * 2;       // 16-bit rows
@@ -752,7 +761,7 @@ static int step_begin_impl(tk_kv* h, int32_t n_seqs, const int32_t* seq_ids, con
     if (h->host_only) { h->mgr->delta().clear(); h->have_step = true; return TK_OK; }
 
     cudaStream_t s = (cudaStream_t)stream;
-    TK_CUDA(h, cudaSetDevice(h->device));
+    const OnDevice current(h);
     h->mgr->compact_delta();
     auto& delta = h->mgr->delta();
     int n_delta = (int)delta.size();
@@ -893,7 +902,7 @@ int tk_kv_append(tk_kv* h, int32_t layer, const void* k, const void* v, int64_t*
     if (!h->have_step) return fail(h, TK_INVALID_ARG, "append: no step in progress (call tk_kv_step_begin)");
     if (h->dev.n_tokens == 0) return TK_OK;
     if (!k || !v) return fail(h, TK_INVALID_ARG, "append: null k/v");
-    const OnDevice current(h->device);
+    const OnDevice current(h);
     int n = 0;
     cudaError_t e = tk::launch_append(h->geo, h->layer(layer), h->dev, h->d_table, k, v, slots_out,
                                       (cudaStream_t)stream, &n);
@@ -957,7 +966,7 @@ int tk_kv_read(tk_kv* h, int32_t layer, int32_t n_ranges, const int32_t* seq_ids
     if (h->host_only) return fail(h, TK_CUDA_ERROR, "read: handle has no device (bookkeeping only)");
     if (items.empty()) return TK_OK;
     if (!k_out || !v_out) return fail(h, TK_INVALID_ARG, "read: null output");
-    const OnDevice current(h->device);
+    const OnDevice current(h);
     int n = 0;
     const cudaError_t e = tk::launch_read_rows(h->geo, h->layer(layer), items.data(), (int)items.size(), k_out, v_out, out_dtype,
                                                (cudaStream_t)stream, &n);
@@ -977,7 +986,7 @@ static int decode_impl(tk_kv* h, int layer, const void* q, void* out, float* par
     if (!h->have_step) return fail(h, TK_INVALID_ARG, "decode: no step in progress (call tk_kv_step_begin)");
     if (h->dev.n_seqs == 0) return TK_OK;
     if (!q || (!out && !partial_out)) return fail(h, TK_INVALID_ARG, "decode: null q/out");
-    const OnDevice current(h->device);
+    const OnDevice current(h);
     tk::LayerPtrs lp = h->layer(layer);
     cudaError_t e = cudaSuccess;
     const bool cold = h->mgr->cold_enabled() && h->mgr->cold_high_water() > 0;
@@ -1086,7 +1095,7 @@ int tk_kv_rope_append_decode(tk_kv* h, int32_t layer, const void* k, const void*
     if (h->host_only) return fail(h, TK_CUDA_ERROR, "rope_append_decode: handle has no device (bookkeeping only)");
     if (!h->have_step) return fail(h, TK_INVALID_ARG, "rope_append_decode: no step in progress (call tk_kv_step_begin)");
     if (!q || !out || (h->dev.n_tokens > 0 && (!k || !v))) return fail(h, TK_INVALID_ARG, "rope_append_decode: null argument");
-    const OnDevice current(h->device);
+    const OnDevice current(h);
     const bool fusable = h->use_mma && h->cfg.dtype != TK_FP8_E4M3 && h->plan.one_token_steps &&
                          h->dev.chunk_tokens <= 2048 && h->dev.n_tokens > 0 && h->dev.n_seqs > 0 &&
                          !h->plan.has_empty_seq && !(h->cfg.dtype == TK_INT8 && h->plan.capped);
@@ -1150,7 +1159,7 @@ static int decode_multi_impl(tk_kv* h, int32_t layer, const void* q, void* out, 
     if (!h->have_step) return fail(h, TK_INVALID_ARG, "decode_multi: no step in progress (call tk_kv_step_begin)");
     if (h->dev.n_seqs == 0) return TK_OK;
     if (!q || !out) return fail(h, TK_INVALID_ARG, "decode_multi: null q/out");
-    const OnDevice current(h->device);
+    const OnDevice current(h);
     const tk::StepPlan& p = h->plan;
     if (p.nq_min < 1) return fail(h, TK_INVALID_ARG, "decode_multi: every sequence of the step must append at least one token");
     if (h->cfg.dtype == TK_INT8) {
@@ -1264,6 +1273,7 @@ int tk_kv_decode_exchange(tk_kv* h, int32_t layer, const void* q, tk_peer* peer,
     if (tk::peer_row_floats(peer) != dv + 2 || n_rows > tk::peer_max_rows(peer))
         return fail(h, TK_INVALID_ARG, "decode_exchange: %d rows of %d floats do not fit the mailbox", n_rows, dv + 2);
     if (h->dev.n_seqs == 0) return TK_OK;
+    const OnDevice current(h);
     // a merging CTA waits for its peers while it holds a CTA slot: keep those few against the slots of a
     // launch, or ranks could fill their GPUs with CTAs that wait for CTAs the other ranks cannot start
     const bool in_kernel = h->cfg.dtype != TK_INT8 && !h->plan.has_empty_seq && !h->separate_combine && h->dev.n_items > 0 &&
@@ -1274,10 +1284,7 @@ int tk_kv_decode_exchange(tk_kv* h, int32_t layer, const void* q, tk_peer* peer,
         return st;
     }
     const size_t need = (size_t)h->cfg.max_seqs * h->cfg.num_heads * (h->cfg.v_head_dim + 2) * sizeof(float);
-    if (!h->d_xpartial) {                                   // first use only
-        TK_CUDA(h, cudaSetDevice(h->device));
-        TK_CUDA(h, cudaMalloc((void**)&h->d_xpartial, need));
-    }
+    if (!h->d_xpartial) TK_CUDA(h, cudaMalloc((void**)&h->d_xpartial, need));    // first use only
     int st = decode_impl(h, layer, q, nullptr, h->d_xpartial, (cudaStream_t)stream);
     if (st != TK_OK) return st;
     st = tk::peer_exchange(peer, h->d_xpartial, n_rows, dv, out, h->cfg.io_dtype, stream);
@@ -1307,6 +1314,7 @@ int tk_combine_partials(const float* parts, int32_t n_parts, int32_t n_rows, int
 static int host_flush(tk_kv* h) {
     if (h->host_flushing || h->host_pending.empty()) return TK_OK;
     h->host_flushing = true;
+    const OnDevice current(h);
     std::vector<tk_kv::HostPending> pend;
     pend.swap(h->host_pending);
     cudaStream_t s = h->host_pending_stream;
@@ -1351,6 +1359,7 @@ static int append_decode_host_impl(tk_kv* h, int32_t layer, const void* k_host, 
         const int st = host_flush(h);
         if (st != TK_OK) return st;
     }
+    const OnDevice current(h);
     const int set = (int)(h->host_calls++ % (uint64_t)h->host_sets);
     TK_CUDA(h, cudaStreamWaitEvent(h->st_in, h->ev_free[set], 0));
     if (kv_bytes) {
@@ -1382,6 +1391,7 @@ int tk_kv_host_wait(tk_kv* h, void* stream) {
     if (!h || h->host_only) return TK_INVALID_ARG;
     const int st = host_flush(h);
     if (st != TK_OK) return st;
+    const OnDevice current(h);
     TK_CUDA(h, cudaStreamWaitEvent((cudaStream_t)stream, h->ev_out_all, 0));
     return TK_OK;
 }
@@ -1397,7 +1407,7 @@ int tk_kv_append_decode_host_async(tk_kv* h, int32_t layer, const void* k_host, 
 
 int tk_kv_profile_enable(tk_kv* h, int32_t max_launches) {
     if (!h || h->host_only || max_launches < 0) return TK_INVALID_ARG;
-    TK_CUDA(h, cudaSetDevice(h->device));
+    const OnDevice current(h);
     while (h->prof_ev.size() < 2 * (size_t)max_launches) {
         cudaEvent_t e;
         TK_CUDA(h, cudaEventCreate(&e));
@@ -1409,6 +1419,7 @@ int tk_kv_profile_enable(tk_kv* h, int32_t max_launches) {
 }
 int tk_kv_profile_read(tk_kv* h, double* total_ms, int64_t* launches) {
     if (!h || h->host_only || !total_ms || !launches) return TK_INVALID_ARG;
+    const OnDevice current(h);
     double sum = 0.0;
     for (size_t i = 0; i + 1 < h->prof_used; i += 2) {
         TK_CUDA(h, cudaEventSynchronize(h->prof_ev[i + 1]));
@@ -1424,6 +1435,7 @@ int tk_kv_profile_read(tk_kv* h, double* total_ms, int64_t* launches) {
 
 int tk_kv_profile_read_each(tk_kv* h, float* ms_out, int32_t cap, int32_t* launches) {
     if (!h || h->host_only || !launches || cap < 0 || (cap > 0 && !ms_out)) return TK_INVALID_ARG;
+    const OnDevice current(h);
     int32_t n = 0;
     for (size_t i = 0; i + 1 < h->prof_used; i += 2, n++) {
         TK_CUDA(h, cudaEventSynchronize(h->prof_ev[i + 1]));
@@ -1439,6 +1451,7 @@ int tk_kv_profile_read_each(tk_kv* h, float* ms_out, int32_t cap, int32_t* launc
 int tk_kv_device_status(tk_kv* h, void* stream) {
     if (!h || h->host_only) return TK_INVALID_ARG;
     if (const int fs = host_flush(h)) return fs;               // launches the host-buffer calls still hold back come first
+    const OnDevice current(h);
     int st = 0;
     TK_CUDA(h, cudaMemcpyAsync(&st, h->d_status, sizeof(int), cudaMemcpyDeviceToHost, (cudaStream_t)stream));
     TK_CUDA(h, cudaStreamSynchronize((cudaStream_t)stream));
@@ -1454,6 +1467,7 @@ int tk_kv_device_status(tk_kv* h, void* stream) {
 
 int tk_kv_selftest_bounded_wait(tk_kv* h, int32_t limit_ms, void* stream) {
     if (!h || h->host_only || limit_ms <= 0 || limit_ms > 2000) return TK_INVALID_ARG;
+    const OnDevice current(h);
     cudaError_t e = tk::launch_bounded_wait_selftest(h->d_status, (unsigned long long)limit_ms * 1000000ull,
                                                      (cudaStream_t)stream);
     h->launches++;
@@ -1463,6 +1477,7 @@ int tk_kv_selftest_bounded_wait(tk_kv* h, int32_t limit_ms, void* stream) {
 int tk_kv_selftest_set_status(tk_kv* h, int32_t value, void* stream) {
     if (!h || h->host_only) return TK_INVALID_ARG;
     if (value != TK_OK && value != TK_TIMEOUT) return fail(h, TK_INVALID_ARG, "selftest_set_status: value must be TK_OK or TK_TIMEOUT");
+    const OnDevice current(h);
     TK_CUDA(h, cudaMemcpyAsync(h->d_status, &value, sizeof(int), cudaMemcpyHostToDevice, (cudaStream_t)stream));
     TK_CUDA(h, cudaStreamSynchronize((cudaStream_t)stream));      // `value` lives on this call's stack
     return TK_OK;
@@ -1470,7 +1485,7 @@ int tk_kv_selftest_set_status(tk_kv* h, int32_t value, void* stream) {
 
 int tk_kv_check_canaries(tk_kv* h, void* stream) {
     if (!h || h->host_only) return TK_INVALID_ARG;
-    TK_CUDA(h, cudaSetDevice(h->device));
+    const OnDevice current(h);
     TK_CUDA(h, cudaStreamSynchronize((cudaStream_t)stream));
     std::vector<uint8_t> buf(kCanaryBytes);
     for (const auto& cn : h->canaries) {
