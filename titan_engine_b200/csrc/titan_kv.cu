@@ -643,6 +643,7 @@ int tk_kv_seq_adopt(tk_kv* h, int32_t seq, const int32_t* pages, int32_t n_pages
 }
 int tk_kv_seq_fork(tk_kv* h, int32_t parent, int32_t* child_out, void* stream) {
     if (!h || !child_out) return TK_INVALID_ARG;
+    if (const int fs = host_flush(h)) return fs;               // the child's copy holds what held-back calls append to the parent
     std::lock_guard<std::mutex> lock(h->mgr_mu);
     int child = -1;
     int32_t src = -1, dst = -1;
