@@ -241,6 +241,13 @@ class PagedKVCache:
         if t.numel() != rows * heads * self._dims[what]:
             raise KvError(L.TK_INVALID_ARG, f"{what}: expected [{rows}, {heads}, {self._dims[what]}]")
 
+    def _check_out(self, t: torch.Tensor, rows: int) -> None:
+        """A given output may have more rows than the step (one buffer for every step of a loop): the first are written."""
+        if t.get_device() != self._dev_index or t.dtype != self.io_torch_dtype or not t.is_contiguous():
+            raise KvError(L.TK_INVALID_ARG, f"out: need a contiguous {self.io_torch_dtype} tensor on {self.device}")
+        if t.numel() < rows * self._heads * self._out_dim:
+            raise KvError(L.TK_INVALID_ARG, f"out: need room for [{rows}, {self._heads}, {self._out_dim}]")
+
     def _new_out(self, q: torch.Tensor, rows: int) -> torch.Tensor:
         """Output rows for queries that _check_io has seen."""
         if q.dim() == 3 and self._out_dim == self._dims["q"]:
@@ -323,7 +330,7 @@ class PagedKVCache:
         if out is None:
             out = self._new_out(q, self._n_seqs)
         else:
-            self._check_io(out, self._n_seqs, self._heads, "out")
+            self._check_out(out, self._n_seqs)
         self._check(self._lib.tk_kv_append_decode(self._h, layer, k.data_ptr(), v.data_ptr(), q.data_ptr(),
                                                   out.data_ptr(), self._stream()))
         return out
@@ -337,7 +344,7 @@ class PagedKVCache:
         if out is None:
             out = self._new_out(q, self._n_seqs)
         else:
-            self._check_io(out, self._n_seqs, self._heads, "out")
+            self._check_out(out, self._n_seqs)
         self._check(self._lib.tk_kv_rope_append_decode(self._h, layer, k.data_ptr(), v.data_ptr(), q.data_ptr(),
                                                        out.data_ptr(), theta, scaling, self._stream()))
         return out
@@ -357,7 +364,7 @@ class PagedKVCache:
         if out is None:
             out = self._new_out(q, self._n_tokens)
         else:
-            self._check_io(out, self._n_tokens, self._heads, "out")
+            self._check_out(out, self._n_tokens)
         self._check(self._lib.tk_kv_decode_multi(self._h, layer, q.data_ptr(), out.data_ptr(), self._stream()))
         return out
 
@@ -370,7 +377,7 @@ class PagedKVCache:
         if out is None:
             out = self._new_out(q, self._n_tokens)
         else:
-            self._check_io(out, self._n_tokens, self._heads, "out")
+            self._check_out(out, self._n_tokens)
         self._check(self._lib.tk_kv_append_decode_multi(self._h, layer, k.data_ptr(), v.data_ptr(), q.data_ptr(),
                                                         out.data_ptr(), self._stream()))
         return out
