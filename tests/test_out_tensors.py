@@ -43,3 +43,14 @@ def test_an_output_larger_than_the_step_is_taken_and_a_bad_one_is_not(cache, nam
         with pytest.raises(KvError) as e:
             call(bad)
         assert e.value.status == L.TK_INVALID_ARG
+
+
+@pytest.mark.parametrize("shape", [(TOKENS, H, D), (TOKENS, HKV, H // HKV * D), (TOKENS, 1, H * D), (1, TOKENS, H * D), (TOKENS, H * D),
+                                   (TOKENS, HKV, H // HKV, D), (TOKENS * H * D,)])
+def test_a_new_output_has_the_shape_that_is_documented(cache, shape):
+    """[rows, H, Dv], however the queries are split."""
+    cache._check = lambda status: None                      # (the calls end with "no device")
+    k, v, q = _t(TOKENS, HKV, D), _t(TOKENS, HKV, D), _t(*shape)
+    for out in (cache.decode(0, q), cache.append_decode(0, k, v, q), cache.rope_append_decode(0, k, v, q, 10000.0), cache.decode_multi(0, q),
+                cache.append_decode_multi(0, k, v, q)):
+        assert out.shape == (TOKENS, H, D) and out.dtype == q.dtype and out.is_contiguous()

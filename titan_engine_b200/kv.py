@@ -249,8 +249,8 @@ class PagedKVCache:
             raise KvError(L.TK_INVALID_ARG, f"out: need room for [{rows}, {self._heads}, {self._out_dim}]")
 
     def _new_out(self, q: torch.Tensor, rows: int) -> torch.Tensor:
-        """Output rows for queries that _check_io has seen."""
-        if q.dim() == 3 and self._out_dim == self._dims["q"]:
+        """Output rows [rows, H, Dv] for queries that _check_io has seen."""
+        if q.shape == (rows, self._heads, self._out_dim):
             return torch.empty_like(q)                      # (half the host time of naming shape, type and device)
         return q.new_empty((rows, self._heads, self._out_dim))
 
