@@ -415,6 +415,9 @@ int tk_kv_selftest_bounded_wait(tk_kv* h, int32_t limit_ms, void* stream);
  * host, as a timed-out device wait would.  While the word is set, attention launches on the handle write no
  * output; tk_kv_device_status reports and clears it. */
 int tk_kv_selftest_set_status(tk_kv* h, int32_t value, void* stream);
+/* Test hook: allocations of split-KV workspaces for multi-token steps fail, as on a full device, where together with those the
+ * handle still holds they would exceed `bytes` (0: no limit). */
+int tk_kv_selftest_workspace_limit(tk_kv* h, int64_t bytes);
 /* Stray-write check (the reference relies on external memory checkers; this is built in): 4 KiB of guard
  * bytes sit behind the pool arena (when the handle allocated it, or an external arena is 4 KiB larger than
  * tk_kv_arena_bytes), the page table, the split-KV workspace and the step metadata.  Drains `stream`,

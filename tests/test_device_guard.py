@@ -7,7 +7,7 @@ import re
 SOURCE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "titan_engine_b200", "csrc", "titan_kv.cu")
 
 # reached only from functions that hold the guard
-GUARDED_BY_CALLER = {"run_evictions", "prefetch_layer", "multi_workspace"}
+GUARDED_BY_CALLER = {"run_evictions", "prefetch_layer", "multi_workspace", "workspace_alloc"}
 # takes no handle: the caller's current device is the one that is meant
 NO_HANDLE = {"tk_combine_partials"}
 HARMLESS = ("cudaGetErrorString", "cudaGetDevice")

@@ -117,6 +117,7 @@ SIGNATURES = {
     "tk_kv_device_status": (C.c_int, [_P, _P]),
     "tk_kv_selftest_bounded_wait": (C.c_int, [_P, C.c_int32, _P]),
     "tk_kv_selftest_set_status": (C.c_int, [_P, C.c_int32, _P]),
+    "tk_kv_selftest_workspace_limit": (C.c_int, [_P, C.c_int64]),
     "tk_kv_check_canaries": (C.c_int, [_P, _P]),
     "tk_peer_check_canaries": (C.c_int, [_P, _P]),
     "tk_kv_launch_count": (C.c_int64, [_P]),

@@ -157,7 +157,10 @@ struct tk_kv {
     float* d_xpartial = nullptr;         // this rank's merged partial rows for tk_kv_decode_exchange
     float* d_multi_partials = nullptr;   // split-KV rows of multi-token steps that outgrow d_partials
     size_t multi_partials_floats = 0;
+    bool multi_captured = false;         // a graph may name it
     std::vector<float*> old_multi_partials;   // smaller ones that a captured graph may still name; freed with the handle
+    size_t old_multi_floats = 0;              // ... and what they hold together
+    size_t multi_limit_bytes = 0;             // selftest: memory for these buffers ends here (0: where the device's does)
     bool mla_mma = false;
 
     // cold tier (hot_window > 0): pages older than the window live in pinned host memory and are
@@ -1125,26 +1128,50 @@ int tk_kv_decode_partial(tk_kv* h, int32_t layer, const void* q, float* partial,
     return decode_impl(h, layer, q, nullptr, partial, (cudaStream_t)stream);
 }
 
+// cudaMalloc of a split-KV workspace, or what it answers when the device is full.
+static cudaError_t workspace_alloc(tk_kv* h, size_t floats, float** out) {
+    const size_t held = h->old_multi_floats + (h->d_multi_partials ? h->multi_partials_floats : 0);
+    if (h->multi_limit_bytes && (held + floats) * sizeof(float) > h->multi_limit_bytes) return cudaErrorMemoryAllocation;
+    return cudaMalloc((void**)out, floats * sizeof(float));
+}
+
 // Split-KV workspace of a multi-token step: the handle's own when `floats` fit it, else a buffer that is
-// allocated (and grown) on demand - the one device allocation a step may make after creation.  A buffer that is outgrown
-// lives on with the handle (each is twice its predecessor, so they add up to less than the current one): a graph captured
-// with it keeps its pointer.  A capture cannot allocate: a step that would grow the buffer is refused there, the capture lives on.
+// allocated (and grown) on demand - the one device allocation a step may make after creation.  A buffer that a capture was
+// given lives on with the handle when it is outgrown (its graph keeps the pointer) and its successor is twice as large where the
+// device has room, so that the kept ones add up to less than the current one; any other is freed first.  A capture cannot
+// allocate: a step that would grow the buffer is refused there, the capture lives on.
 static float* multi_workspace(tk_kv* h, size_t floats, cudaStream_t stream) {
     if (floats <= (size_t)h->max_partial_rows * h->cfg.num_heads * (h->cfg.v_head_dim + 2)) return h->d_partials;
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    const bool capturing = cudaStreamIsCapturing(stream, &status) != cudaSuccess || status != cudaStreamCaptureStatusNone;
     if (floats > h->multi_partials_floats) {
-        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(stream, &capturing) != cudaSuccess || capturing != cudaStreamCaptureStatusNone) {
+        if (capturing) {
+            cudaGetLastError();                             // (what the default stream answers while another one captures)
             fail(h, TK_CUDA_ERROR, "decode_multi: the step needs a larger split-KV workspace, which a stream capture cannot allocate: run it once before");
             return nullptr;
         }
-        const size_t grown = std::max(floats, 2 * h->multi_partials_floats);
+        size_t grown = floats;
+        if (h->d_multi_partials && h->multi_captured) {
+            grown = std::max(floats, 2 * h->multi_partials_floats);
+        } else if (h->d_multi_partials) {
+            cudaStreamSynchronize(stream);
+            cudaFree(h->d_multi_partials);
+            h->d_multi_partials = nullptr; h->multi_partials_floats = 0;
+        }
         float* p = nullptr;
-        cudaError_t e = cudaMalloc((void**)&p, grown * sizeof(float));
-        if (e != cudaSuccess) { fail(h, TK_CUDA_ERROR, "split-KV workspace of %zu bytes: %s", grown * sizeof(float), cudaGetErrorString(e)); return nullptr; }
-        if (h->d_multi_partials) h->old_multi_partials.push_back(h->d_multi_partials);
+        cudaError_t e = workspace_alloc(h, grown, &p);
+        if (e != cudaSuccess && grown > floats) e = workspace_alloc(h, grown = floats, &p);
+        if (e != cudaSuccess) {
+            cudaGetLastError();                             // reported here, not by the next launch
+            fail(h, TK_CUDA_ERROR, "split-KV workspace of %zu bytes: %s", grown * sizeof(float), cudaGetErrorString(e));
+            return nullptr;
+        }
+        if (h->d_multi_partials) { h->old_multi_partials.push_back(h->d_multi_partials); h->old_multi_floats += h->multi_partials_floats; }
         h->d_multi_partials = p;
         h->multi_partials_floats = grown;
+        h->multi_captured = false;
     }
+    h->multi_captured = h->multi_captured || capturing;
     return h->d_multi_partials;
 }
 
@@ -1481,6 +1508,12 @@ int tk_kv_selftest_set_status(tk_kv* h, int32_t value, void* stream) {
     const OnDevice current(h);
     TK_CUDA(h, cudaMemcpyAsync(h->d_status, &value, sizeof(int), cudaMemcpyHostToDevice, (cudaStream_t)stream));
     TK_CUDA(h, cudaStreamSynchronize((cudaStream_t)stream));      // `value` lives on this call's stack
+    return TK_OK;
+}
+
+int tk_kv_selftest_workspace_limit(tk_kv* h, int64_t bytes) {
+    if (!h || h->host_only || bytes < 0) return TK_INVALID_ARG;
+    h->multi_limit_bytes = (size_t)bytes;
     return TK_OK;
 }
 
