@@ -177,7 +177,7 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
              *bar_s = bars + 16 /* [half][2] */, *p_ready = bars + 20 /* [half][2] */, *bar_o = bars + 24 /* [half] */;
     uint32_t* s_tmem = (uint32_t*)(bars + 26);
     int* s_flag = (int*)(s_tmem + 1);
-    uint32_t* s_wmax = (uint32_t*)(bars + 28);              // [16 softmax warps] prologue: largest query magnitude
+    uint32_t* s_wmax = (uint32_t*)(bars + 28);              // [16 softmax warps] prologue: largest and smallest query magnitudes
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = 1 << sh;
@@ -239,26 +239,33 @@ prefill_int8_kernel(Geometry g, const uint8_t* __restrict__ pool, PrefillDev pf,
 
     const uint32_t raw_u = smem_u32(s_raw), k_u = smem_u32(s_k), v_u = smem_u32(s_v);
     // bf16 queries as fp16: the largest element of the tile becomes 2^14 .. 2^15, one power of two 2^e0 for all rows.  Elements
-    // below fp16's normal range are off by at most 2^-40 of that largest element, a score by 2^-40 of what it could make of
-    // the key: nothing, unless such scores pass 2^28.  Where a query reaches 2^15 (`wide`) every row therefore has a power of
-    // its own, and its scores are multiplied by it.
+    // below fp16's normal range (2^-14) are off by at most 2^-25, so that every eight of them (a 16-byte vector) whose largest comes
+    // to 2^0 or more are as good as FP32.  Where some do not, or where a query reaches 2^15 (`wide`), every row has a power of its
+    // own and its scores are multiplied by it: off by at most 2^-39 of the row's largest element then, far below the rounding of
+    // the row's sums.
     int e0 = 0;
     bool wide = false;
     auto tile_power = [&]() {                               // from what the softmax warps left
-        uint32_t m_all = 0;
+        uint32_t w = 0;
 #pragma unroll
-        for (int i = 0; i < kPfSoftWarps; i++) m_all = max(m_all, s_wmax[i]);
+        for (int i = 0; i < kPfSoftWarps; i++) w = __vmaxu2(w, s_wmax[i]);
+        const uint32_t m_all = w >> 16, least = 0x8000u - (w & 0xFFFFu);      // bf16 patterns; `least` of the vectors that are not zero
         e0 = m_all ? max((int)(m_all >> 7) - 127 - 14, -100) : 0;
-        wide = e0 > 0;                                      // some |q| >= 2^15
+        wide = e0 > 0 || (m_all >> 7) > (least >> 7) + 14;
     };
     bool staged = true;                                     // expander: no wait of the prologue ran out
     if (warp < kPfSoftWarps) {
         if (IO_BF16) {
-            uint32_t m = 0;
+            uint32_t m = 0, n = 0x7FFFu;                    // largest of all vectors; smallest of those that are not zero, minus 1
 #pragma unroll
-            for (int i = 0; i < QV; i++) m = max(m, i8_absmax8(qv[i]));
+            for (int i = 0; i < QV; i++) {
+                const uint32_t v = i8_absmax8(qv[i]);
+                m = max(m, v);
+                n = min(n, v - 1u);
+            }
             m = __reduce_max_sync(0xFFFFFFFFu, m);
-            if (lane == 0) s_wmax[warp] = m;
+            n = __reduce_min_sync(0xFFFFFFFFu, n);
+            if (lane == 0) s_wmax[warp] = m << 16 | (0x7FFFu - n);
             asm volatile("bar.sync 2, %0;" ::"n"(kPfSoftThreads) : "memory");
             tile_power();
         }
