@@ -55,3 +55,15 @@ def test_a_loaded_state_has_no_step_to_wait_for():
     c.step_begin([s], [20])
     c.state_load(c.state_save())
     assert _read(c, s, 0, 16) == L.TK_CUDA_ERROR
+
+
+def test_a_token_in_a_cold_page_is_refused():
+    c = _cache("bf16", hot_window=32, cold_pages=8)
+    s = c.seq_alloc()
+    c.step_begin([s], [100])
+    c.step_begin([s], [1])                                  # the first pages leave for the host's pool
+    cold = int((c.page_table(s) < 0).sum())
+    assert 0 < cold < 6
+    assert _read(c, s, 0, 1) == L.TK_UNSUPPORTED
+    assert _read(c, s, 16 * cold - 1, 2) == L.TK_UNSUPPORTED
+    assert _read(c, s, 16 * cold, 101 - 16 * cold) == L.TK_CUDA_ERROR       # hot pages: the next check answers (no device)
