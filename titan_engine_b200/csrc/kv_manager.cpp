@@ -308,23 +308,47 @@ int64_t fair_chunk(const StepPlan& p, int tpt, int num_kv_heads, int sms, const 
     }
     const int64_t share = std::max<int64_t>(4, (blocks + sms - 1) / sms);
     if ((int64_t)tiles.size() * num_kv_heads > 8 * (int64_t)sms) return share * 64;     // many items balance themselves
-    const int64_t whole = tiles.empty() ? share : *std::max_element(tiles.begin(), tiles.end());
+    std::sort(tiles.begin(), tiles.end());
+    const int64_t whole = tiles.empty() ? share : tiles.back();
     int64_t best = share, best_end = INT64_MAX;
-    std::vector<int64_t> cost, load;
+    // Items of one cost (a tile's kv heads, full parts) are dealt out together, to the SMs of one load at a time: an item by itself
+    // cost 60 to 150 us of host time for a thousand of them.  Runs of (cost or load, how many).
+    typedef std::pair<int64_t, int64_t> Run;
+    std::vector<Run> cost, load;
+    int64_t tried[6];
+    int n_tried = 0;
     for (int64_t cap : {whole, share, share * 3 / 4, share / 2, share / 3, share / 4}) {
         cap = std::max<int64_t>(4, cap);
+        if (std::find(tried, tried + n_tried, cap) != tried + n_tried) continue;
+        tried[n_tried++] = cap;
         cost.clear();
-        for (int64_t b : tiles)
-            for (int64_t at = 0; at < b; at += cap)
-                for (int h = 0; h < num_kv_heads; h++) cost.push_back(std::min(cap, b - at) + kItemBlocks + (b > cap ? kSplitBlocks : 0));
-        std::sort(cost.begin(), cost.end(), std::greater<int64_t>());
-        load.assign((size_t)sms, 0);                       // a heap, the least loaded SM on top
-        for (int64_t c : cost) {
-            std::pop_heap(load.begin(), load.end(), std::greater<int64_t>());
-            load.back() += c;
-            std::push_heap(load.begin(), load.end(), std::greater<int64_t>());
+        int64_t total = 0, full = 0;
+        auto add = [&](int64_t c, int64_t n) {
+            total += c * n;
+            if (!cost.empty() && cost.back().first == c) cost.back().second += n;
+            else cost.push_back({c, n});
+        };
+        for (int64_t b : tiles) {
+            if (b <= cap) { add(b + kItemBlocks, num_kv_heads); continue; }
+            full += b / cap * num_kv_heads;
+            if (b % cap) add(b % cap + kItemBlocks + kSplitBlocks, num_kv_heads);
         }
-        const int64_t end = *std::max_element(load.begin(), load.end());
+        if (full) add(cap + kItemBlocks + kSplitBlocks, full);
+        std::sort(cost.begin(), cost.end(), std::greater<Run>());
+        if (cost.empty() || std::max(cost[0].first, (total + sms - 1) / sms) >= best_end) continue;    // no schedule of these is shorter
+        load.assign(1, Run{0, sms});                       // descending, the least loaded SMs last
+        for (const Run& c : cost)
+            for (int64_t left = c.second; left > 0;) {
+                Run& low = load.back();
+                const Run next{low.first + c.first, std::min(low.second, left)};
+                left -= next.second;
+                low.second -= next.second;
+                if (low.second == 0) load.pop_back();
+                auto at = std::lower_bound(load.begin(), load.end(), next.first, [](const Run& r, int64_t v) { return r.first > v; });
+                if (at != load.end() && at->first == next.first) at->second += next.second;
+                else load.insert(at, next);
+            }
+        const int64_t end = load.front().first;
         if (end < best_end) { best_end = end; best = cap; }
     }
     return best * 64;
