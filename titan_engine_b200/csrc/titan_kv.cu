@@ -4,6 +4,7 @@
 
 #include "int8_cache.cuh"
 #include "kv_manager.h"
+#include "launch_chain.h"
 #include "tk_kernels.cuh"
 #include "tk_peer.cuh"
 
@@ -116,10 +117,10 @@ struct tk_kv {
     int* d_pf_counters = nullptr;        // prefill kernel: one per (sequence, kv head, tile) group
     int max_pf_groups = 0, max_pf_items = 0;
     // programmatic dependent launch of back-to-back attention kernels: the launch count right after the last
-    // attention launch, its layer and stream (another launch of this library in between breaks the chain)
+    // attention launch and its stream (another launch of this library in between breaks the chain), the chain's layers and outputs
     int64_t chain_launches = -1;
-    int chain_layer = -1;
     cudaStream_t chain_stream = nullptr;
+    tk::LaunchChain chain;
     tk::PrefillDev pf_dev{};             // device view of the step's prefill work list
     tk::StepDev small_dev{};             // ... and of the decode-kernel share of such a step
 
@@ -747,6 +748,7 @@ static int step_begin_impl(tk_kv* h, int32_t n_seqs, const int32_t* seq_ids, con
     if (st != TK_OK) return fail(h, st, "step_begin: %s", tk_status_str(st));
     tk::StepPlan& p = h->plan;
     h->appended.assign((size_t)h->cfg.num_layers, 0);
+    h->chain.clear();                                          // the upload below lies between: nothing overlaps across it
     if (chunk == 0 && p.chunk_tokens > 2048) {
         return fail(h, TK_INVALID_ARG, "internal: chunk %d too large", p.chunk_tokens);
     }
@@ -1025,11 +1027,14 @@ static int decode_impl(tk_kv* h, int layer, const void* q, void* out, float* par
     if (mma) {
         // FP8: the 16-bit open pages are items of kind 1 of the same launch
         if (h->dev.n_items > 0) {
-            // A launch of ANOTHER layer that directly follows an attention launch of this handle on the same
-            // stream may overlap that launch's tail: its page tiles belong to a pool the earlier kernel does
-            // not touch, and it waits for the earlier kernel before it writes split-KV rows or `out`.
-            const bool overlap = h->cfg.launch_overlap == TK_OVERLAP_AUTO && !cold && !timed &&
-                                 h->chain_launches == h->launches && h->chain_stream == s && h->chain_layer != layer;
+            // A launch that directly follows attention launches of OTHER layers of this handle on the same stream, and reads nothing
+            // that they write, may overlap their tails (launch_chain.h).
+            const size_t n_q = (size_t)h->dev.n_seqs * h->geo.H, n_kv = (size_t)h->dev.n_tokens * h->geo.Hkv;
+            const bool overlap = h->chain.add(
+                h->cfg.launch_overlap == TK_OVERLAP_AUTO && !cold && !timed && h->chain_launches == h->launches && h->chain_stream == s,
+                layer, {{q, n_q * h->geo.D * 2}, {fuse_k, n_kv * h->geo.D * 2}, {fuse_v, n_kv * h->geo.Dv * 2}},
+                partial_out ? tk::MemRange{partial_out, n_q * (h->geo.Dv + 2) * sizeof(float)}
+                            : tk::MemRange{out, n_q * h->geo.Dv * (out_dtype == TK_FP32 ? 4 : 2)});
             if (h->cfg.dtype == TK_INT8)
                 e = tk::launch_decode_int8(h->geo, lp, &h->maps[layer], h->dev, h->d_table, q, h->d_partials, h->d_status, s, mo, fa,
                                            false, overlap);
@@ -1039,7 +1044,7 @@ static int decode_impl(tk_kv* h, int layer, const void* q, void* out, float* par
             else
                 e = tk::launch_decode_mma(h->geo, lp, &h->maps[layer], cold ? &h->stage_maps[slot] : nullptr, h->dev,
                                           h->d_table, q, h->d_partials, h->d_status, s, &mo, &fa, overlap);
-            h->chain_launches = h->launches + 1; h->chain_layer = layer; h->chain_stream = s;
+            h->chain_launches = h->launches + 1; h->chain_stream = s;
             h->launches++;
         }
         if (timed) { cudaEventRecord(h->prof_ev[h->prof_used + 1], s); h->prof_used += 2; }
