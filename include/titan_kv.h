@@ -256,11 +256,14 @@ int tk_kv_decode_ex(tk_kv* h, int32_t layer, const void* q, int32_t q_dtype, voi
  * (src/inference/speculative.cpp:262-272); rejected tokens are dropped with tk_kv_truncate.
  * It is also the attention of a prefill chunk: the reference runs update + attention_decode once per
  * prompt token (src/inference/engine.cpp:182-193, src/inference/batch.cpp:169-198).  When a sequence
- * appends more than 128 / (num_heads / num_kv_heads) tokens, the sequences with many tokens go to a kernel
- * that works on tiles of 64 (token, head) rows sharing each K/V page tile; the others stay with the decode
- * kernel.  16-bit pools with the tensor-core kernels or INT8 pools, every sequence of the step appending at least one
- * token, no cold pages, no capped lengths on an INT8 pool; the MLA shape up to 64 / (num_heads / num_kv_heads) tokens per sequence;
- * TK_UNSUPPORTED otherwise. */
+ * appends more than 128 / (num_heads / num_kv_heads) tokens, the step's sequences of more than
+ * 16 / (num_heads / num_kv_heads) go to a kernel that works on tiles of 64 or 128 (token, head) rows sharing each K/V page
+ * tile; the others stay with the decode kernel.  On an INT8 pool every sequence of more than 16 / (num_heads / num_kv_heads)
+ * tokens goes to such a kernel, in tiles of 256 rows.
+ * 16-bit pools with the tensor-core kernels or INT8 pools, no cold pages, no capped lengths on an INT8 pool; the MLA shape up to
+ * 64 / (num_heads / num_kv_heads) tokens per sequence; TK_UNSUPPORTED otherwise.  TK_INVALID_ARG where a sequence of the step
+ * appends nothing.  A step may need a larger split-KV workspace than the handle has so far, which it allocates then; inside a
+ * stream capture it is refused instead (TK_CUDA_ERROR, the capture lives on): run the step once before. */
 int tk_kv_decode_multi(tk_kv* h, int32_t layer, const void* q, void* out, void* stream);
 /* tk_kv_decode_multi with the output type given: TK_FP32 (the reference's float* interface,
  * src/compute/dispatch.h:73-75) or the handle's io dtype. */
