@@ -16,7 +16,7 @@
 // the codes.  A tile brings its scales along (int8_cache.cuh): one TMA box per page.  On decode steps the warp that holds
 // the last page quantises the new token into shared memory and into the pool: no append launch.
 // Bound: HBM (D + 4 bytes per token and kv head for K and for V).  Measured at D = 128: 32 sequences of 32768 tokens, 64 heads
-// on 8: 337-387 us = 5.7-6.6 TB/s (issue slots 60 %, tensor pipe 18 %); 64 sequences of 1024-8192, 32 heads: 102-107 us, of which
+// on 8: 337-390 us = 5.7-6.6 TB/s (issue slots 60 %, tensor pipe 18 %); 64 sequences of 1024-8192, 32 heads: 101-108 us, of which
 // about 10 are the launch's start and drain; one sequence of 65536 tokens: 39 us, where starting and merging are a third.
 #include "int8_cache.cuh"
 #include "tk_merge.cuh"

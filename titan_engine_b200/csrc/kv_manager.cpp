@@ -410,7 +410,8 @@ int PageManager::plan_step(int n_seqs, const int32_t* seqs, const int32_t* n_new
         // schedules start at 1.05 waves: one sequence, 64 heads on 8, D = 128: 131072 tokens as 512 items 86 us, as 688 111; 152000 as
         // 600 items 93, as 1192 106; 170000 as 672 items 130, as 888 116.  Below 1.7 items per SM it gains from two of them, down to 896
         // tokens each: 32768 tokens as 128 items 42.5 us, as 296 40.0; 40000 as 160 items 51.5, as 320 45.7; 65536 as 256 items 50.6,
-        // as 296 50.2.
+        // as 296 50.2.  The same holds at D = 64: 32768 tokens in chunks of 2048 28.7 us, of 896 26.7, of 512 28.7; 65536 34.9 (2048), 36.9 (1024);
+        // 131072 49.2 (2048), 63.6 (1536); 170000 72.5 (2048), 69 (1536), 80 (1024).
         const bool int8 = prefill_rows == kPrefillRowsInt8;
         int most_new = 1;
         for (int i = 0; n_new && i < n_seqs; i++) most_new = std::max(most_new, n_new[i]);

@@ -323,7 +323,8 @@ class PagedKVCache:
 
     def append_decode(self, layer: int, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor,
                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """append + decode of one layer; a single fused kernel on 16-bit decode steps."""
+        """append + decode of one layer; a single fused kernel on 16-bit and INT8 decode steps.  `out` (here and in the calls below) may
+        have more rows than the step: its first are written."""
         self._check_io(k, self._n_tokens, self._kv_heads, "k")
         self._check_io(v, self._n_tokens, self._kv_heads, "v")
         self._check_io(q, self._n_seqs, self._heads, "q")
